@@ -396,6 +396,77 @@ int ptj_decode(const float* w_emb, const float* b_head, const float* w_pos, cons
                int64_t dim, int64_t layers, int64_t heads, int64_t ffn, int64_t seq, float* workspace,
                size_t workspace_floats, void* stream);
 
+/* ---- serving: paged key-value cache ---------------------------------------------------------------------- */
+/* No counterparts in the reference, whose predict runs the whole sequence for every new token
+ * (loss_and_optimizer_triton.py:203-212).
+ *
+ * One layer's cache: pools of pages [pages, kv_heads, page_size, d_head] (element strides page, head, slot; d_head contiguous)
+ * and a page table. Key j of sequence b lies in slot j % page_size of page table[b * table_ld + j / page_size]. lengths[b]
+ * counts the sequence's keys, the new tokens of the call among them. Table entries behind the last key are not read.
+ * The tables and lengths live on the device, where the host cannot check them: a page outside [0, pages) is skipped (its keys
+ * count as absent, nothing is written to it) and ptj_last_kernel_fault reports 0x3201; a length outside
+ * [0, table_width * page_size] or a count outside [0, tokens] is brought to the nearer bound and reported as 0x3202.
+ * Sequences may share pages that are only read; a page that is written belongs to one sequence. */
+typedef struct {
+  void *k, *v;
+  const int32_t *table, *lengths;
+  int64_t batch, kv_heads, d_head;             /* d_head <= 256 */
+  int64_t pages, page_size, table_width, table_ld;
+  int64_t k_strides[3], v_strides[3];
+  int dtype;                                   /* PTJ_F32 or PTJ_BF16: pools and new tokens */
+} ptj_kv_cache;
+/* The new tokens of a call: token t < counts[b] of sequence b sits at position lengths[b] - counts[b] + t; counts == NULL: all
+ * `tokens` of every sequence. Views [batch, heads, tokens, d_head] with element strides batch, head, token. */
+typedef struct {
+  const void *q, *k, *v;                       /* k, v: NULL where the cache holds the new rows already */
+  void* out;
+  const int32_t* counts;
+  int64_t heads, tokens;                       /* heads: a multiple of kv_heads; query head i reads key head i / (heads / kv_heads) */
+  int64_t q_strides[3], o_strides[3], k_strides[3], v_strides[3];
+} ptj_new_tokens;
+/* Writes the rows k, v of the new tokens into their pages; positions below 0 (a count above the length) are left out. */
+int ptj_kv_append(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, void* stream);
+/* Attention of the new tokens over the cache, evaluation semantics (the output is multiplied by 1 - p):
+ *   out = (1 - p) softmax(q K^T / sqrt(d_head)) V over keys 0 .. position of the token.
+ * With tokens->k and ->v the new rows are written to their pages as by ptj_kv_append and attended to. A token behind counts[b]
+ * or below position 0 attends nothing: a zero row. Rows read only the keys they attend: what lies in other slots, an infinity
+ * or a NaN included, reaches no output. Softmax statistics and sums are float32.
+ * weights_out (optional, float[batch, kv_heads, weights_ld], weights_ld >= table_width * page_size): the attention that each
+ * key received, summed over the query heads of its key head and the new tokens, plus weights (same layout; NULL = 0; may be
+ * weights_out itself) for keys that are not new. Slots from lengths[b] on are left as they were.
+ * workspace: ptj_attn_decode_workspace_bytes bytes, 16-byte aligned, contents irrelevant before and after; bit-reproducible. */
+size_t ptj_attn_decode_workspace_bytes(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, int with_weights);
+int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, float p, const float* weights,
+                    float* weights_out, int64_t weights_ld, void* workspace, size_t workspace_bytes, void* stream);
+/* Cuts every sequence with more than `budget` keys down to `budget`, for each key head on its own: the last `recent` keys stay
+ * (recent <= budget) and of the others those with the largest weights (float[batch, kv_heads, weights_ld], weights_ld >=
+ * table_width * page_size), the lowest positions among equals; a NaN ranks below everything. Keys stay in order: key kept[i]
+ * becomes key i of dst_table (rows of dst_ld entries; dst_table == cache->table: in place). Other sequences are only copied
+ * to dst_table. Destination pages of different sequences differ, and unless in place they are no source pages.
+ *   kept         int32[batch, kv_heads, budget]: positions that stay, -1 behind them
+ *   new_lengths  int32[batch]: min(lengths, budget); not the array `lengths`
+ *   weights_out  float[batch, kv_heads, weights_out_ld]: weights of the kept keys (may be weights itself, with its leading
+ *                dimension); slots behind them are left as they were. NULL: not wanted */
+int ptj_kv_evict(const ptj_kv_cache* cache, const int32_t* dst_table, int64_t dst_width, int64_t dst_ld, int64_t budget,
+                 int64_t recent, const float* weights, int64_t weights_ld, float* weights_out, int64_t weights_out_ld,
+                 int32_t* kept, int32_t* new_lengths, void* stream);
+
+/* ---- serving: drafted tokens --------------------------------------------------------------------------- */
+/* Accepts or replaces `drafts` drafted tokens per sequence so that what comes out is distributed as the target's tokens.
+ *   target    [batch, drafts + 1, vocab] of dtype, strides target_strides (sequence, draft): probabilities after each draft
+ *   draft     [batch, drafts, vocab]: the probabilities the drafts were drawn from; NULL: every draft had probability 1
+ *   tokens    int32[batch, drafts], counts int32[batch] (NULL: all `drafts`): drafts of each sequence
+ *   uniforms  float[batch, drafts + 1] in [0, 1)
+ * Draft i is accepted while uniforms[i] * draft[i][x] < target[i][x] (exact; a token outside [0, vocab) is not). At the first
+ * rejection n, or behind the last draft, the next token is the first j at which the running sum of
+ * w = max(target[n] - draft[n], 0), or of target[n] behind the last draft, passes uniforms[drafts] times its total (sums and
+ * products in float64; terms that are NaN count as 0; where all are 0: the largest target[n], the first among equals).
+ *   out       int32[batch, drafts + 1]: the accepted drafts, the next token, 0 (padding) behind it
+ *   accepted  int32[batch]: n */
+int ptj_verify_drafts(const void* target, const int64_t target_strides[2], const void* draft, const int64_t draft_strides[2],
+                      const int32_t* tokens, const int32_t* counts, const float* uniforms, int32_t* out, int32_t* accepted,
+                      int64_t batch, int64_t drafts, int64_t vocab, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

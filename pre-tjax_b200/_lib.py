@@ -52,6 +52,18 @@ class LayerActs(ctypes.Structure):
                                         "h_act")]
 
 
+class KvCache(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("table", c_void_p), ("lengths", c_void_p), ("batch", c_int64),
+                ("kv_heads", c_int64), ("d_head", c_int64), ("pages", c_int64), ("page_size", c_int64), ("table_width", c_int64),
+                ("table_ld", c_int64), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3), ("dtype", c_int)]
+
+
+class NewTokens(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("counts", c_void_p), ("heads", c_int64),
+                ("tokens", c_int64), ("q_strides", c_int64 * 3), ("o_strides", c_int64 * 3), ("k_strides", c_int64 * 3),
+                ("v_strides", c_int64 * 3)]
+
+
 _P = c_void_p
 _SIGNATURES = {
     "ptj_version": (c_int, []),
@@ -107,6 +119,12 @@ _SIGNATURES = {
     "ptj_decode_workspace_floats": (c_size_t, [c_int64] * 7),
     "ptj_decode": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_float, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                            c_int64, _P, c_size_t, _P]),
+    "ptj_kv_append": (c_int, [POINTER(KvCache), POINTER(NewTokens), _P]),
+    "ptj_attn_decode_workspace_bytes": (c_size_t, [POINTER(KvCache), POINTER(NewTokens), c_int]),
+    "ptj_attn_decode": (c_int, [POINTER(KvCache), POINTER(NewTokens), c_float, _P, _P, c_int64, _P, c_size_t, _P]),
+    "ptj_kv_evict": (c_int, [POINTER(KvCache), _P, c_int64, c_int64, c_int64, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P]),
+    "ptj_verify_drafts": (c_int, [_P, POINTER(c_int64 * 2), _P, POINTER(c_int64 * 2), _P, _P, _P, _P, _P, c_int64, c_int64,
+                                  c_int64, c_int, _P]),
     "ptj_cast_f32_to_bf16": (c_int, [_P, _P, c_int64, _P]),
 }
 

@@ -500,6 +500,204 @@ def t_scaled_dot_prod_attn_bkwd3_t(dloss_dx, acts, qkv: torch.Tensor, mask: torc
     return dq, dk, dv
 
 
+# ---- paged key-value cache ----------------------------------------------------------------------------------------------
+def _on_current_device(*tensors):
+    """Launches go to the current device's stream: tensors elsewhere are refused."""
+    dev = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("tensors must live on a CUDA device: there is no CPU implementation")
+        if t.get_device() != dev:
+            raise RuntimeError(f"tensor on cuda:{t.get_device()}, but cuda:{dev} is the current device")
+
+
+def _ints(t, shape, name):
+    """An int32 tensor of this shape; rows of a table may be strided."""
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must be an int32 tensor of shape {list(shape)} with contiguous rows")
+    return t
+
+
+def _kv_cache(k_pages, v_pages, page_table, lengths):
+    """The descriptor of a paged cache, after the checks that its tensors allow."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must share one shape [pages, kv_heads, page_size, d_head]")
+    if k_pages.dtype != v_pages.dtype:
+        raise TypeError("k_pages and v_pages must share a dtype")
+    pages, heads, page_size, d = k_pages.shape
+    sk, sv = k_pages.stride(), v_pages.stride()
+    if d > 1 and (sk[3] != 1 or sv[3] != 1):
+        raise ValueError("d_head must be contiguous")
+    B, width = page_table.shape
+    _ints(page_table, (B, width), "page_table")
+    _ints(lengths, (B,), "lengths")
+    return _lib.KvCache(_ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(lengths), B, heads, d, pages, page_size, width,
+                        page_table.stride(0) if B > 1 else width, sk[:3], sv[:3], _dt(k_pages))
+
+
+def _new_tokens(cache, q, k, v, out, counts, dtype):
+    B, Hk, d = cache.batch, cache.kv_heads, cache.d_head
+    some = q if q is not None else k
+    if some.dim() != 4:
+        raise ValueError("new tokens must be [batch, heads, tokens, d_head]")
+    T = some.shape[2]
+    views = []
+    for t, heads, name in ((q, None, "q"), (out, None, "out"), (k, Hk, "k"), (v, Hk, "v")):
+        if t is None:
+            views.append((0, (0, 0, 0)))
+            continue
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must have the cache's dtype {dtype}")
+        heads = some.shape[1] if heads is None else heads
+        if tuple(t.shape) != (B, heads, T, d) or (d > 1 and t.stride(3) != 1):
+            raise ValueError(f"{name} must be [{B}, {heads}, {T}, {d}] with d_head contiguous")
+        views.append((t.data_ptr(), t.stride()[:3]))
+    if counts is not None:
+        _ints(counts, (B,), "counts")
+    if q is not None and (some.shape[1] % Hk or some.shape[1] < 1):
+        raise ValueError(f"{some.shape[1]} query heads do not share {Hk} key heads evenly")
+    (qp, qs), (op, os), (kp, ks), (vp, vs) = views
+    return _lib.NewTokens(qp, kp, vp, op, _ptr(counts), some.shape[1], T, qs, os, ks, vs)
+
+
+def _attended(weights, cache, name):
+    cap = cache.table_width * cache.page_size
+    if weights.dtype != torch.float32 or weights.dim() != 3 or not weights.is_contiguous() or \
+            tuple(weights.shape[:2]) != (cache.batch, cache.kv_heads) or weights.shape[2] < cap:
+        raise ValueError(f"{name} must be a contiguous float32 tensor [{cache.batch}, {cache.kv_heads}, >= {cap}]")
+
+
+def kv_append(k, v, k_pages, v_pages, page_table, lengths, counts=None):
+    """Writes the keys and values of new tokens, views [B, kv_heads, T, d_head], into a paged cache.
+
+    k_pages, v_pages: pools [pages, kv_heads, page_size, d_head] (d_head contiguous); page_table int32 [B, width]: key j of
+    sequence b lies in slot j % page_size of page page_table[b, j // page_size]; lengths int32 [B]: keys of each sequence, the
+    new ones among them. Row t of sequence b goes to position lengths[b] - counts[b] + t; counts int32 [B] (default T)
+    says how many of the T rows are tokens. Pages, lengths and counts out of range are skipped or clamped and reported by
+    last_kernel_fault."""
+    _on_current_device(k, v, k_pages, v_pages, page_table, lengths, counts)
+    cache = _kv_cache(k_pages, v_pages, page_table, lengths)
+    new = _new_tokens(cache, None, k, v, None, counts, k_pages.dtype)
+    if cache.batch == 0 or new.tokens == 0:
+        return
+    _lib.check(_lib.lib().ptj_kv_append(ctypes.byref(cache), ctypes.byref(new), _stream()), "ptj_kv_append")
+
+
+def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, counts=None, weights=None, weights_out=None,
+                out=None, p=None, workspace=None):
+    """Attention of the newest tokens of each sequence over a paged cache, train=False: [B, H, T, d_head] (strided views).
+
+    Cache and counts as for kv_append; k and v, when given, are appended first. Token t of sequence b attends keys
+    0 .. lengths[b] - counts[b] + t; tokens behind counts[b] and those below position 0 attend nothing (zero rows). Query head
+    i reads key head i // (H / kv_heads). The output is multiplied by 1 - p (default DROPOUT_RATE), as everywhere in evaluation.
+    weights float32 [B, kv_heads, capacity]: the attention that every key received so far; the call adds its own, summed over
+    the query heads of a key head and the new tokens, into weights_out (default: weights; weights None counts as zeros). What
+    weights holds for new keys does not matter. workspace: optional uint8 tensor, see ptj_attn_decode_workspace_bytes."""
+    _on_current_device(q, k_pages, v_pages, page_table, lengths, k, v, counts, weights, weights_out, out, workspace)
+    cache = _kv_cache(k_pages, v_pages, page_table, lengths)
+    if out is None:
+        out = torch.empty_like(q)
+        if out.dim() == 4 and out.stride(3) != 1:
+            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    new = _new_tokens(cache, q, k, v, out, counts, k_pages.dtype)
+    if cache.batch == 0 or new.tokens == 0:
+        return out
+    if weights_out is None:
+        weights_out = weights
+    ld = 0
+    if weights_out is not None:
+        _attended(weights_out, cache, "weights_out")
+        ld = weights_out.shape[2]
+        if weights is not None:
+            _attended(weights, cache, "weights")
+            if weights.shape[2] != ld:
+                raise ValueError("weights and weights_out must share one shape")
+    lib = _lib.lib()
+    need = lib.ptj_attn_decode_workspace_bytes(ctypes.byref(cache), ctypes.byref(new), int(weights_out is not None))
+    if need and workspace is None:
+        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+    _lib.check(lib.ptj_attn_decode(ctypes.byref(cache), ctypes.byref(new), DROPOUT_RATE if p is None else p, _ptr(weights),
+                                   _ptr(weights_out), ld, _ptr(workspace),
+                                   0 if workspace is None else workspace.numel() * workspace.element_size(), _stream()),
+               "ptj_attn_decode")
+    return out
+
+
+def kv_evict(k_pages, v_pages, page_table, lengths, weights, budget, recent=0, *, dst_table=None, weights_out=None):
+    """Cuts the sequences of a paged cache down to `budget` keys, each key head on its own: the last `recent` keys stay, and of
+    the others those with the largest accumulated weights (attn_decode), the lowest positions among equals (a NaN ranks below
+    everything). Returns (kept int32 [B, kv_heads, budget]: positions that stayed, in order, -1 behind them; new lengths
+    int32 [B]). The kept rows become rows 0 .. of the pages of dst_table (default: page_table, in place), which also get
+    the sequences that are short enough; their weights become the first ones of weights_out (default: weights)."""
+    _on_current_device(k_pages, v_pages, page_table, lengths, weights, dst_table, weights_out)
+    cache = _kv_cache(k_pages, v_pages, page_table, lengths)
+    _attended(weights, cache, "weights")
+    budget, recent = int(budget), int(recent)
+    if not 0 <= recent <= budget or budget < 1:
+        raise ValueError("kv_evict needs 0 <= recent <= budget and budget >= 1")
+    most = min(budget, cache.table_width * cache.page_size)
+    weights_out = weights if weights_out is None else weights_out
+    if weights_out.dtype != torch.float32 or weights_out.dim() != 3 or not weights_out.is_contiguous() or \
+            tuple(weights_out.shape[:2]) != (cache.batch, cache.kv_heads) or weights_out.shape[2] < most:
+        raise ValueError(f"weights_out must be a contiguous float32 tensor [{cache.batch}, {cache.kv_heads}, >= {most}]")
+    dst_table = page_table if dst_table is None else dst_table
+    if dst_table.dim() != 2 or dst_table.shape[1] * cache.page_size < most:
+        raise ValueError(f"dst_table must list pages for {most} keys of each sequence")
+    _ints(dst_table, (cache.batch, dst_table.shape[1]), "dst_table")
+    kept = torch.empty((cache.batch, cache.kv_heads, budget), device=weights.device, dtype=torch.int32)
+    new_lengths = torch.empty_like(lengths)
+    if cache.batch == 0:
+        return kept, new_lengths
+    _lib.check(_lib.lib().ptj_kv_evict(ctypes.byref(cache), _ptr(dst_table), dst_table.shape[1],
+                                       dst_table.stride(0) if cache.batch > 1 else dst_table.shape[1], budget, recent, _ptr(weights),
+                                       weights.shape[2], _ptr(weights_out), weights_out.shape[2], _ptr(kept), _ptr(new_lengths),
+                                       _stream()), "ptj_kv_evict")
+    return kept, new_lengths
+
+
+# ---- drafted tokens -----------------------------------------------------------------------------------------------------
+def _rows_of(probs, name, shape, dtype):
+    if probs.dtype != dtype or tuple(probs.shape) != shape or (shape[2] > 1 and probs.stride(2) != 1):
+        raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} with contiguous rows")
+    return (ctypes.c_int64 * 2)(probs.stride(0), probs.stride(1))
+
+
+def verify_drafts(target_probs, draft_tokens, uniforms, draft_probs=None, counts=None):
+    """(tokens int32 [B, K + 1], accepted int32 [B]) for K drafted tokens per sequence, int32 [B, K].
+
+    target_probs [B, K + 1, V]: the target model's probabilities at each draft and behind the last one; draft_probs [B, K, V]:
+    those the drafts were drawn from (None: each draft had probability 1, a lookup or a greedy guess); uniforms float32
+    [B, K + 1] in [0, 1); counts int32 [B]: drafts of each sequence (default K). Draft i is accepted while
+    uniforms[i] * draft_probs[i, x] < target_probs[i, x]. The token behind the accepted ones is drawn with uniforms[K] from
+    max(target - draft, 0) at the first rejection, from the target behind the last draft: the first token at which the running
+    sum passes uniforms[K] times the total, in float64. tokens: the accepted drafts, that token, and 0 behind it."""
+    _on_current_device(target_probs, draft_tokens, uniforms, draft_probs, counts)
+    if target_probs.dim() != 3 or target_probs.shape[1] < 1:
+        raise ValueError("target_probs must be [batch, drafts + 1, vocab]")
+    B, K, V = target_probs.shape
+    K -= 1
+    ts = _rows_of(target_probs, "target_probs", (B, K + 1, V), target_probs.dtype)
+    ds = None if draft_probs is None else _rows_of(draft_probs, "draft_probs", (B, K, V), target_probs.dtype)
+    if draft_tokens.dtype != torch.int32 or tuple(draft_tokens.shape) != (B, K):
+        raise ValueError(f"draft_tokens must be an int32 tensor of shape [{B}, {K}]")
+    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (B, K + 1):
+        raise ValueError(f"uniforms must be a float32 tensor of shape [{B}, {K + 1}]")
+    if counts is not None:
+        counts = _ints(counts, (B,), "counts").contiguous()
+    draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
+    tokens = torch.empty((B, K + 1), device=target_probs.device, dtype=torch.int32)
+    accepted = torch.empty(B, device=target_probs.device, dtype=torch.int32)
+    if B == 0:
+        return tokens, accepted
+    _lib.check(_lib.lib().ptj_verify_drafts(_ptr(target_probs), ctypes.byref(ts), _ptr(draft_probs),
+                                            None if ds is None else ctypes.byref(ds), _ptr(draft_tokens), _ptr(counts),
+                                            _ptr(uniforms), _ptr(tokens), _ptr(accepted), B, K, V, _dt(target_probs),
+                                            _stream()), "ptj_verify_drafts")
+    return tokens, accepted
+
+
 # ---- cross entropy -----------------------------------------------------------------------------------------------------
 def cross_entropy(labels, logits, cols=None, want_grad=True, in_place=False, n_valid=None, want_rows=False):
     """Fused CE forward(+backward). logits [rows, ld]; returns (stats float[3] = loss, accuracy, valid fraction;
