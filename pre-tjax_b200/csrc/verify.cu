@@ -2,12 +2,18 @@
 //
 // Accepting draft x with probability min(1, p(x) / q(x)) and replacing the first rejected one by a token drawn from
 // max(p - q, 0) leaves the target's distribution p unchanged: q(x) min(1, p/q) + (sum of rejections) max(p - q, 0) / total = p(x).
-#include "common.cuh"
+//
+// Of all the probabilities only one row per sequence (two with a draft's distribution) is read whole: the one the next token is
+// drawn from. A cluster of C blocks shares it. Each block sums its slice, the sums meet through distributed shared memory, and
+// the block in whose slice the running sum passes the mark looks for the place: a warp's chunk, 256 elements of it, 32, one.
+// Sums are float64, products of two float32 in float64 are exact: decisions then agree with a sum in any other order except for
+// marks within 1e-13 or so of a border.
+#include "cluster.cuh"
 
 namespace ptj {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 
 struct Verify {
   const void *target, *draft;
@@ -18,95 +24,183 @@ struct Verify {
   int K, V;
 };
 
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+  return v;
+}
+
+// What the next token is drawn from.
 template <typename E>
+struct Weights {
+  const E *row, *sub;  // sub: NULL, or what is taken off
+  int skip;            // an element without weight, -1: none
+  __device__ __forceinline__ double operator()(int j) const {
+    double w = Elem<E>::load(row + j);
+    if (sub != nullptr) w -= static_cast<double>(Elem<E>::load(sub + j));
+    return w > 0.0 && j != skip ? w : 0.0;  // (a NaN has none)
+  }
+};
+
+template <typename E, int C>
 __global__ void __launch_bounds__(kThreads)
 verify_kernel(const __grid_constant__ Verify p) {
   grid_dep_sync();
-  __shared__ double sums[kThreads];
-  __shared__ int n_s, pick_s;
-  __shared__ float best_s[32];
-  __shared__ int arg_s[32];
-  const int tid = threadIdx.x;
-  const int64_t b = blockIdx.x;
+  __shared__ double chunk_s[kWarps], total_s;
+  __shared__ int n_s;
+  __shared__ float best_s[kWarps];
+  __shared__ int arg_s[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = static_cast<int>(cluster_rank<C>());
+  const int64_t b = blockIdx.x / C;
   const E* target = static_cast<const E*>(p.target) + b * p.ts[0];
   const E* draft = p.draft == nullptr ? nullptr : static_cast<const E*>(p.draft) + b * p.ds[0];
   const int32_t* tokens = p.tokens + b * p.K;
   const float* u = p.uniforms + b * (p.K + 1);
-  int count = p.counts == nullptr ? p.K : min(max(p.counts[b], 0), p.K);
-  if (tid == 0) {
-    int n = 0;
-    for (; n < count; ++n) {
-      const int x = tokens[n];
-      if (x < 0 || x >= p.V) break;
-      const double px = Elem<E>::load(target + n * p.ts[1] + x);
-      const double qx = draft == nullptr ? 1.0 : static_cast<double>(Elem<E>::load(draft + n * p.ds[1] + x));
-      if (!(static_cast<double>(u[n]) * qx < px)) break;
-    }
-    n_s = n;
-    pick_s = 0x7fffffff;
-  }
-  __syncthreads();
-  const int n = n_s;
-  const E* row = target + n * p.ts[1];
-  const E* sub = n < count && draft != nullptr ? draft + n * p.ds[1] : nullptr;
-  const int skip = n < count && draft == nullptr ? tokens[n] : -1;
-  auto weight = [&](int j) -> double {
-    double w = Elem<E>::load(row + j);
-    if (sub != nullptr) w -= static_cast<double>(Elem<E>::load(sub + j));
-    return w > 0.0 && j != skip ? w : 0.0;
-  };
-  const int per = (p.V + kThreads - 1) / kThreads, j0 = min(tid * per, p.V), j1 = min(j0 + per, p.V);
-  double s = 0.0;
-  for (int j = j0; j < j1; ++j) s += weight(j);
-  sums[tid] = s;
-  __syncthreads();
-  double before = 0.0, total = 0.0;
-  for (int i = 0; i < kThreads; ++i) {
-    if (i == tid) before = total;
-    total += sums[i];
-  }
-  const double want = static_cast<double>(u[p.K]) * total;
-  if (before + s > want) {
-    double c = before;
-    for (int j = j0; j < j1; ++j) {
-      c += weight(j);
-      if (c > want) {
-        atomicMin(&pick_s, j);
+  const int count = p.counts == nullptr ? p.K : min(max(p.counts[b], 0), p.K);
+  if (warp == 0) {  // every block finds the first rejected draft for itself
+    int n = count;
+    for (int i0 = 0; i0 < count; i0 += 32) {
+      const int i = i0 + lane;
+      bool ok = true;
+      if (i < count) {
+        const int x = tokens[i];
+        ok = x >= 0 && x < p.V;
+        if (ok) {
+          const double px = Elem<E>::load(target + i * p.ts[1] + x);
+          const double qx = draft == nullptr ? 1.0 : static_cast<double>(Elem<E>::load(draft + i * p.ds[1] + x));
+          ok = static_cast<double>(u[i]) * qx < px;
+        }
+      }
+      const unsigned no = __ballot_sync(0xffffffffu, !ok);
+      if (no != 0u) {
+        n = i0 + __ffs(no) - 1;
         break;
       }
     }
-  }
-  // nothing to draw from: the largest probability
-  float best = -INFINITY;
-  int arg = 0;
-  if (!(total > 0.0)) {
-    arg = 0x7fffffff;
-    for (int j = tid; j < p.V; j += kThreads) {
-      const float x = Elem<E>::load(row + j);
-      if (x > best) { best = x; arg = j; }
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-      const float v = __shfl_xor_sync(0xffffffffu, best, o);
-      const int a = __shfl_xor_sync(0xffffffffu, arg, o);
-      if (v > best || (v == best && a < arg)) { best = v; arg = a; }
-    }
-    if ((tid & 31) == 0) { best_s[tid >> 5] = best; arg_s[tid >> 5] = arg; }
+    if (lane == 0) n_s = n;
   }
   __syncthreads();
-  int32_t* out = p.out + b * (p.K + 1);
+  const int n = n_s;
+  const bool rejected = n < count;
+  Weights<E> weight{target + n * p.ts[1], rejected && draft != nullptr ? draft + n * p.ds[1] : nullptr,
+                    rejected && draft == nullptr ? tokens[n] : -1};
+  // contiguous chunks, one per warp of the cluster
+  const int per = (p.V + C * kWarps * 32 - 1) / (C * kWarps * 32) * 32;
+  const int j0 = min((rank * kWarps + warp) * per, p.V), j1 = min(j0 + per, p.V);
+  double s = 0.0;
+#pragma unroll 8
+  for (int j = j0 + lane; j < j1; j += 32) s += weight(j);
+  s = warp_sum_f64(s);
+  if (lane == 0) chunk_s[warp] = s;
+  __syncthreads();
   if (tid == 0) {
-    int pick = pick_s;
-    if (!(total > 0.0)) {
-      best = -INFINITY;
-      pick = 0x7fffffff;
-      for (int i = 0; i < 32; ++i)
-        if (best_s[i] > best || (best_s[i] == best && arg_s[i] < pick)) { best = best_s[i]; pick = arg_s[i]; }
-    }
-    out[n] = pick < p.V ? pick : 0;
-    p.accepted[b] = n;
+    double t = 0.0;
+    for (int w = 0; w < kWarps; ++w) t += chunk_s[w];
+    total_s = t;
   }
-  for (int i = tid; i <= p.K; i += kThreads)
-    if (i != n) out[i] = i < n ? tokens[i] : 0;
+  cluster_barrier<C>();
+  double before = 0.0, total = 0.0;
+#pragma unroll
+  for (int r = 0; r < C; ++r) {
+    const double t = peer_f64<C>(&total_s, r);
+    if (r < rank) before += t;
+    total += t;
+  }
+  cluster_barrier<C>();  // the sums are read: a block may leave
+  int32_t* out = p.out + b * (p.K + 1);
+  if (rank == 0) {
+    for (int i = tid; i <= p.K; i += kThreads)
+      if (i != n) out[i] = i < n ? tokens[i] : 0;
+    if (tid == 0) p.accepted[b] = n;
+  }
+  if (total > 0.0) {
+    const float last_u = u[p.K];
+    double mark = static_cast<double>(last_u < 1.f ? last_u : 1.f - 5.9604645e-8f) * total;
+    if (!(mark >= 0.0)) mark = 0.0;  // (no number, or below 0)
+    // the first slice, and in it the first chunk, at whose end the running sum passes the mark
+    double end = before + total_s;
+    bool mine = before <= mark || rank == 0;
+    if (rank < C - 1) mine = mine && end > mark;
+    if (!mine) return;
+    int w = 0;
+    double at = before;
+    for (; w < kWarps - 1 && !(at + chunk_s[w] > mark); ++w) at += chunk_s[w];
+    // (a mark that rounding puts behind all sums belongs to the last chunk that has any weight)
+    while (w > 0 && !(chunk_s[w] > 0.0)) at -= chunk_s[--w];
+    if (warp != w) return;
+    int pick = -1, last = -1;  // last: the last element with weight so far
+    for (int g = j0; g < j1; g += 256) {
+      double x[8], sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = g + i * 32 + lane;
+        x[i] = j < j1 ? weight(j) : 0.0;
+        sum += x[i];
+      }
+      sum = warp_sum_f64(sum);
+      const bool here = at + sum > mark;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned some = __ballot_sync(0xffffffffu, x[i] > 0.0);
+        if (some != 0u && pick < 0) last = g + i * 32 + 31 - __clz(some);
+        if (here && pick < 0) {
+          double c = x[i];
+#pragma unroll
+          for (int k = 1; k < 32; k <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, c, k);
+            if (lane >= k) c += y;
+          }
+          const unsigned over = __ballot_sync(0xffffffffu, at + c > mark && x[i] > 0.0);
+          if (over != 0u) pick = g + i * 32 + __ffs(over) - 1;
+          at += __shfl_sync(0xffffffffu, c, 31);
+        }
+      }
+      if (pick >= 0 || here) break;
+      at += sum;
+    }
+    if (lane == 0) out[n] = pick >= 0 ? pick : max(last, 0);
+    return;
+  }
+  // nothing to draw from: the largest probability, the first among equals
+  if (rank != 0) return;
+  float best = -INFINITY;
+  int arg = 0x7fffffff;
+  auto better = [&](float v, int a) {
+    if (v > best || (v == best && a < arg)) {
+      best = v;
+      arg = a;
+    }
+  };
+  for (int j = tid; j < p.V; j += kThreads) better(Elem<E>::load(weight.row + j), j);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) {
+    const float v = __shfl_xor_sync(0xffffffffu, best, x);
+    better(v, __shfl_xor_sync(0xffffffffu, arg, x));
+  }
+  if (lane == 0) {
+    best_s[warp] = best;
+    arg_s[warp] = arg;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kWarps; ++w) better(best_s[w], arg_s[w]);
+    out[n] = arg < p.V ? arg : 0;
+  }
+}
+
+template <typename E>
+void launch_verify(const Verify& p, int64_t batch, cudaStream_t st) {
+  // as many blocks per sequence as leave two for each SM, each with a slice worth a round of its threads
+  unsigned c = 8;
+  while (c > 1 && (batch * c > 2 * kNumSMs || p.V < static_cast<int64_t>(c) * kThreads)) c /= 2;
+  const dim3 grid(static_cast<unsigned>(batch) * c);
+  switch (c) {
+    case 8: launch_cluster_k(verify_kernel<E, 8>, grid, kThreads, 8, st, p); break;
+    case 4: launch_cluster_k(verify_kernel<E, 4>, grid, kThreads, 4, st, p); break;
+    case 2: launch_cluster_k(verify_kernel<E, 2>, grid, kThreads, 2, st, p); break;
+    default: launch_k(verify_kernel<E, 1>, grid, kThreads, 0, st, p);
+  }
 }
 
 }  // namespace
@@ -140,9 +234,8 @@ extern "C" int ptj_verify_drafts(const void* target, const int64_t target_stride
   p.K = static_cast<int>(drafts);
   p.V = static_cast<int>(vocab);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int grid = static_cast<int>(batch);
-  if (dtype == PTJ_BF16) launch_k(verify_kernel<__nv_bfloat16>, grid, kThreads, 0, st, p);
-  else launch_k(verify_kernel<float>, grid, kThreads, 0, st, p);
+  if (dtype == PTJ_BF16) launch_verify<__nv_bfloat16>(p, batch, st);
+  else launch_verify<float>(p, batch, st);
   PTJ_CHECK_LAUNCH();
   return PTJ_OK;
 }
