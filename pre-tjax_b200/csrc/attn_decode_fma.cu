@@ -1,0 +1,162 @@
+// Attention of new tokens over a paged cache on CUDA cores, float32 arithmetic: float32 caches and bf16 heads beyond 128.
+//
+// LPK lanes share a key, 16 bytes of the row each, NV times; 32 / LPK keys stand side by side. A row of queries costs a product per
+// element and key twice and log2(LPK) shuffles per key; up to eight rows stay under what memory delivers (4 bytes an element).
+#include "attn_decode.cuh"
+
+namespace ptj {
+namespace {
+
+template <typename E, int DP, int RB>
+struct CoreFma {
+  static constexpr int VEC = 16 / static_cast<int>(sizeof(E)), kDim = DP, kRowBytes = DP * static_cast<int>(sizeof(E)), kRows = RB;
+  static constexpr int LPK = DP / VEC < 32 ? DP / VEC : 32, NV = DP / (VEC * LPK), KPW = 32 / LPK, W = VEC * NV;
+  static constexpr int KS = 4096 / kRowBytes, KB = KS / KPW;  // keys of a step, of a lane
+  static constexpr int kDepth = 3;
+  static constexpr int kBlocks = 2;
+  float q[RB][W], o[RB][W];
+  float ref[RB], sum[RB];
+  int sub_lane, grp;
+
+  __device__ __forceinline__ int elem(int i) const { return (i * LPK + sub_lane) * VEC; }
+
+  __device__ __forceinline__ void init(const DecodeAttn& p, const Segment& sg) {
+    const int lane = threadIdx.x & 31;
+    sub_lane = lane % LPK;
+    grp = lane / LPK;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      ref[r] = -INFINITY;
+      sum[r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) q[r][i] = o[r][i] = 0.f;
+      const int row = sg.rb * kRows + r;
+      if (sg.limit(p, row) < 0) continue;
+      const E* src = reinterpret_cast<const E*>(sg.q_row(p, row));
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (elem(i) + e < p.D) q[r][i * VEC + e] = Elem<E>::load(src + elem(i) + e);
+    }
+  }
+
+  __device__ __forceinline__ void read(const uint8_t* stage, int r, float (&out)[W]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint4 x = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + swizzled(r % KS, i * LPK + sub_lane) * 16);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if constexpr (sizeof(E) == 4) out[i * VEC + e] = __uint_as_float(w[e]);
+        else out[i * VEC + e] = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) {
+    const int j0 = sub * KS;
+    const uint32_t present = present_keys<KS, kRowBytes>(stage);
+    if (j0 + KS > sg.first + 1 || present != (1u << KS) - 1u) step_of<true>(p, sg, j0, stage, present);
+    else step_of<false>(p, sg, j0, stage, present);
+  }
+  template <bool EDGE>
+  __device__ __forceinline__ void step_of(const DecodeAttn& p, const Segment& sg, int j0, const uint8_t* stage, uint32_t present) {
+    float k[KB][W], v[KB][W];
+#pragma unroll
+    for (int e = 0; e < KB; ++e) read(stage, e * KPW + grp, k[e]);
+#pragma unroll
+    for (int e = 0; e < KB; ++e) read(stage, KS + e * KPW + grp, v[e]);
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int row = sg.rb * kRows + r;
+      if (RB > 1 && row >= p.R) break;
+      const int limit = EDGE ? sg.limit(p, row) : 0;
+      float s[KB];
+#pragma unroll
+      for (int e = 0; e < KB; ++e) {
+        s[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) s[e] = fmaf(q[r][i], k[e][i], s[e]);
+      }
+#pragma unroll
+      for (int x = LPK / 2; x > 0; x >>= 1)
+#pragma unroll
+        for (int e = 0; e < KB; ++e) s[e] += __shfl_xor_sync(0xffffffffu, s[e], x);
+      bool over = false;
+#pragma unroll
+      for (int e = 0; e < KB; ++e) {
+        const int i = e * KPW + grp;
+        s[e] *= p.scale;
+        if (EDGE && (!((present >> i) & 1u) || j0 + i > limit)) s[e] = -INFINITY;
+        over |= s[e] > ref[r] + kDecLazy;
+        if (p.scores != nullptr && sub_lane == 0 && j0 + i < sg.n)
+          p.scores[((static_cast<int64_t>(sg.b) * p.Hk + sg.h) * p.R + row) * p.scores_ld + j0 + i] = s[e];
+      }
+      if (__any_sync(0xffffffffu, over)) {
+        float m = s[0];
+#pragma unroll
+        for (int e = 1; e < KB; ++e) m = fmaxf(m, s[e]);
+        m = fmaxf(warp_max(m), ref[r]);
+        const float f = rebase(ref[r], m);
+        ref[r] = m;
+        sum[r] *= f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[r][i] *= f;
+      }
+      const float base = base_of(ref[r]);
+#pragma unroll
+      for (int e = 0; e < KB; ++e) {
+        const float x = ex2(s[e] - base);
+        sum[r] += x;
+        const bool on = !EDGE || j0 + e * KPW + grp <= limit;  // zero times what is not finite is not zero
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[r][i] = fmaf(x, on ? v[e][i] : 0.f, o[r][i]);
+      }
+    }
+  }
+
+  // f(row, element, four sums, reference exponent, sum of the row, true for one call per row)
+  template <typename F>
+  __device__ __forceinline__ void emit(F&& f) {
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      float l = sum[r];
+#pragma unroll
+      for (int x = LPK; x < 32; x <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[r][i] += __shfl_xor_sync(0xffffffffu, o[r][i], x);
+      }
+      if (grp == 0)
+#pragma unroll
+        for (int i = 0; i < W; i += 4)
+          f(r, elem(i / VEC) + i % VEC, make_float4(o[r][i], o[r][i + 1], o[r][i + 2], o[r][i + 3]), ref[r], l, sub_lane == 0 && i == 0);
+    }
+  }
+};
+
+}  // namespace
+
+int decode_fma_blocks(int dim, int rows, int es) {
+  if (es == 2) return dim == 256 && (rows == 1 || rows == 4) ? 2 : 0;
+  return (dim == 64 || dim == 128) && (rows == 1 || rows == 4 || rows == 8) || dim == 256 && (rows == 1 || rows == 4) ? 2 : 0;
+}
+
+int launch_decode_fma(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
+  using B = __nv_bfloat16;
+  if (pl.es == 2)
+    return pl.rows == 1 ? launch_decode<B, CoreFma<B, 256, 1>>(d, pl.split, st) : launch_decode<B, CoreFma<B, 256, 4>>(d, pl.split, st);
+  switch (pl.dim + pl.rows) {
+    case 64 + 1: return launch_decode<float, CoreFma<float, 64, 1>>(d, pl.split, st);
+    case 64 + 4: return launch_decode<float, CoreFma<float, 64, 4>>(d, pl.split, st);
+    case 64 + 8: return launch_decode<float, CoreFma<float, 64, 8>>(d, pl.split, st);
+    case 128 + 1: return launch_decode<float, CoreFma<float, 128, 1>>(d, pl.split, st);
+    case 128 + 4: return launch_decode<float, CoreFma<float, 128, 4>>(d, pl.split, st);
+    case 128 + 8: return launch_decode<float, CoreFma<float, 128, 8>>(d, pl.split, st);
+    case 256 + 1: return launch_decode<float, CoreFma<float, 256, 1>>(d, pl.split, st);
+    default: return launch_decode<float, CoreFma<float, 256, 4>>(d, pl.split, st);
+  }
+}
+
+}  // namespace ptj

@@ -1,0 +1,271 @@
+// Attention of new tokens over a paged cache, bf16 heads of up to 128: tensor cores.
+//
+// S^T = K Q^T and O^T = V^T P^T with m16n8k16: keys, then head elements, are the 16 rows of a product, eight query rows its columns,
+// so one to eight rows cost the same and each further eight half as much again. Which head element sits at which k of a product
+// is free as long as Q and K agree, so a lane's 16 bytes of a key are its operands of two products, and its 16 bytes of four
+// values turn into operands of four products by picking halves of pairs (the transposition that V needs). P^T comes from S^T by
+// transposing 8 x 8 blocks in registers. Probabilities are multiplied in two bf16 parts (16 bits): rounding them to one would
+// cost as much accuracy as rounding the output does. The products of the fourth-generation form suffice: 12 per step of 16 keys
+// at 64 elements, 2 % of their rate at full memory speed.
+#include "attn_decode.cuh"
+
+namespace ptj {
+namespace {
+
+template <int DP, int NR>
+struct CoreTc {
+  static constexpr int KS = 16, kRows = 8 * NR, kDim = DP, kRowBytes = 2 * DP, KU = DP / 32, VW = DP / 64;
+  static constexpr int kDepth = DP == 64 ? 4 : 3;
+  static constexpr int kBlocks = DP == 64 ? 3 : 2;  // resident per SM
+  uint4 q[NR][KU];
+  float o[NR][DP / 16][4];
+  float ref[NR][2], sum[NR][2];
+  int g, c;
+
+  __device__ __forceinline__ void init(const DecodeAttn& p, const Segment& sg) {
+    const int lane = threadIdx.x & 31;
+    g = lane >> 2;
+    c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int r = sg.rb * kRows + i * 8 + g;
+      const bool on = sg.limit(p, r) >= 0;
+      const char* row = on ? sg.q_row(p, r) : nullptr;
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        const int d = 32 * u + 8 * c;
+        q[i][u] = make_uint4(0u, 0u, 0u, 0u);
+        if (!on) continue;
+        if (p.q_wide && d + 8 <= p.D) {
+          q[i][u] = *reinterpret_cast<const uint4*>(row + d * 2);
+        } else {
+          const uint16_t* e = reinterpret_cast<const uint16_t*>(row);
+          auto at = [&](int x) { return d + x < p.D ? static_cast<uint32_t>(e[d + x]) : 0u; };
+          q[i][u] = make_uint4(at(0) | at(1) << 16, at(2) | at(3) << 16, at(4) | at(5) << 16, at(6) | at(7) << 16);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ref[i][e] = -INFINITY;
+        sum[i][e] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][j][e] = 0.f;
+    }
+  }
+
+  // rows of S^T (keys of a step) and k of O^T's products that this lane holds
+  __device__ __forceinline__ int key_of(int i) const { return g + 8 * i; }
+  __device__ __forceinline__ int value_of(int i) const { return 2 * c + (i & 1) + 8 * (i >> 1); }
+  __device__ __forceinline__ uint4 key(const uint8_t* stage, int i, int u) const {
+    const int r = key_of(i);
+    return *reinterpret_cast<const uint4*>(stage + r * kRowBytes + swizzled(r, 4 * u + c) * 16);
+  }
+  __device__ __forceinline__ uint4 value(const uint8_t* stage, int i, int w) const {
+    const int r = value_of(i);
+    return *reinterpret_cast<const uint4*>(stage + (KS + r) * kRowBytes + swizzled(r, 8 * w + g) * 16);
+  }
+
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+  }
+  static __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ void values(float (&acc)[4], const uint4 (&v)[4], int j, const uint32_t (&ph)[2], const uint32_t (&pl)[2]) {
+    const uint32_t v0 = word(v[0], j), v1 = word(v[1], j), v2 = word(v[2], j), v3 = word(v[3], j);
+    const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
+    const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
+    mma(acc, a0, a1, a2, a3, ph[0], ph[1]);
+    mma(acc, a0, a1, a2, a3, pl[0], pl[1]);
+  }
+
+  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) {
+    const int j0 = sub * KS;
+    const bool edge = j0 + KS > sg.first + 1;  // some rows do not attend all of its keys
+    float s[NR][4];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+      const uint4 k0 = key(stage, 0, u), k1 = key(stage, 1, u);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        mma(s[i], k0.x, k1.x, k0.y, k1.y, q[i][u].x, q[i][u].y);
+        mma(s[i], k0.z, k1.z, k0.w, k1.w, q[i][u].z, q[i][u].w);
+      }
+    }
+    const uint32_t present = present_keys<KS, kRowBytes>(stage);
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] *= p.scale;
+    if (edge || present != 0xffffu) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int j = j0 + key_of(x);
+        const bool there = (present >> key_of(x)) & 1u;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!there || j > sg.limit(p, sg.rb * kRows + i * 8 + 2 * c + e)) s[i][2 * x + e] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) over |= s[i][e] > ref[i][e & 1] + kDecLazy;
+    if (p.scores != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = sg.rb * kRows + i * 8 + 2 * c + (e & 1), j = j0 + key_of(e >> 1);
+          if (r < p.R && j < sg.n)
+            p.scores[((static_cast<int64_t>(sg.b) * p.Hk + sg.h) * p.R + r) * p.scores_ld + j] = s[i][e];
+        }
+    }
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = fmaxf(s[i][e], s[i][e + 2]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+          m = fmaxf(m, ref[i][e]);
+          const float f = rebase(ref[i][e], m);
+          ref[i][e] = m;
+          sum[i][e] *= f;
+#pragma unroll
+          for (int j = 0; j < DP / 16; ++j) {
+            o[i][j][e] *= f;
+            o[i][j][e + 2] *= f;
+          }
+        }
+    }
+    uint32_t ph[NR][2], pl[NR][2];
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float x0 = ex2(s[i][2 * k] - base_of(ref[i][0])), x1 = ex2(s[i][2 * k + 1] - base_of(ref[i][1]));
+        sum[i][0] += x0;
+        sum[i][1] += x1;
+        const uint32_t hi = pack(x0, x1);
+        const uint32_t lo = pack(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+        ph[i][k] = transpose8(hi);
+        pl[i][k] = transpose8(lo);
+      }
+    // a value that some rows of the step attend and others do not must be finite to be multiplied by the others' zeros
+    if (edge && not_finite(stage)) {
+      values_by_token(p, sg, j0, stage, ph, pl);
+      return;
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      const uint4 v[4] = {value(stage, 0, w), value(stage, 1, w), value(stage, 2, w), value(stage, 3, w)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < NR; ++i) values(o[i][w * 4 + j], v, j, ph[i], pl[i]);
+    }
+  }
+
+  __device__ __forceinline__ bool not_finite(const uint8_t* stage) const {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint4 v = value(stage, i, w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t x = word(v, j);
+          bad |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+        }
+      }
+    return __any_sync(0xffffffffu, bad);
+  }
+  // The products of a step with values that are not finite: once per new token, with what it does not attend cleared, and added to
+  // its rows only.
+  __device__ __forceinline__ void values_by_token(const DecodeAttn& p, const Segment& sg, int j0, const uint8_t* stage,
+                                                  const uint32_t (&ph)[NR][2], const uint32_t (&pl)[NR][2]) {
+#pragma unroll 1
+    for (int tok = 0; tok < sg.count; ++tok)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i] = j0 + value_of(i) <= sg.first + tok ? value(stage, i, w) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < NR; ++i) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            values(acc, v, j, ph[i], pl[i]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if ((sg.rb * kRows + i * 8 + 2 * c + e) % p.T == tok) {
+                o[i][w * 4 + j][e] += acc[e];
+                o[i][w * 4 + j][e + 2] += acc[e + 2];
+              }
+          }
+      }
+  }
+
+  // f(row, element, four sums, reference exponent, sum of the row, true for one call per row)
+  template <typename F>
+  __device__ __forceinline__ void emit(F&& f) {
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = sum[i][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+            f(i * 8 + 2 * c + e, 64 * w + 8 * g + 4 * hf,
+              make_float4(o[i][w * 4 + 2 * hf][e], o[i][w * 4 + 2 * hf][e + 2], o[i][w * 4 + 2 * hf + 1][e], o[i][w * 4 + 2 * hf + 1][e + 2]),
+              ref[i][e], l, w == 0 && hf == 0 && g == 0);
+      }
+  }
+};
+
+}  // namespace
+
+int decode_tc_blocks(int dim, int rows) {
+  if (dim == 64) return rows == 8 || rows == 16 || rows == 32 ? CoreTc<64, 1>::kBlocks : 0;
+  return dim == 128 && (rows == 8 || rows == 16 || rows == 24) ? CoreTc<128, 1>::kBlocks : 0;
+}
+
+int launch_decode_tc(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
+  using E = __nv_bfloat16;
+  switch (pl.dim + pl.rows) {
+    case 64 + 8: return launch_decode<E, CoreTc<64, 1>>(d, pl.split, st);
+    case 64 + 16: return launch_decode<E, CoreTc<64, 2>>(d, pl.split, st);
+    case 64 + 32: return launch_decode<E, CoreTc<64, 4>>(d, pl.split, st);
+    case 128 + 8: return launch_decode<E, CoreTc<128, 1>>(d, pl.split, st);
+    case 128 + 16: return launch_decode<E, CoreTc<128, 2>>(d, pl.split, st);
+    default: return launch_decode<E, CoreTc<128, 3>>(d, pl.split, st);
+  }
+}
+
+}  // namespace ptj

@@ -17,6 +17,7 @@ struct PagedRows {
   unsigned int* fault;
   int pages, page_size, page_shift;  // page_shift: log2 of the page size, -1 where it is no power of two
   int capacity;                      // keys that a row of the table holds
+  int row_bytes;                     // of a key or a value
   // page and slot of key j; false: the table names no page of the pool
   __device__ __forceinline__ bool locate(const int32_t* row, int j, int64_t& page, int& slot) const {
     int i;
