@@ -119,12 +119,12 @@ _SIGNATURES = {
     "ptj_decode_workspace_floats": (c_size_t, [c_int64] * 7),
     "ptj_decode": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_float, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                            c_int64, _P, c_size_t, _P]),
-    "ptj_kv_append": (c_int, [POINTER(KvCache), POINTER(NewTokens), _P]),
-    "ptj_attn_decode_workspace_bytes": (c_size_t, [POINTER(KvCache), POINTER(NewTokens), c_int]),
-    "ptj_attn_decode": (c_int, [POINTER(KvCache), POINTER(NewTokens), c_float, _P, _P, c_int64, _P, c_size_t, _P]),
-    "ptj_kv_evict": (c_int, [POINTER(KvCache), _P, c_int64, c_int64, c_int64, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P]),
-    "ptj_verify_drafts": (c_int, [_P, POINTER(c_int64 * 2), _P, POINTER(c_int64 * 2), _P, _P, _P, _P, _P, c_int64, c_int64,
-                                  c_int64, c_int, _P]),
+    # (the descriptors KvCache and NewTokens by address, or packed as bytes)
+    "ptj_kv_append": (c_int, [_P, _P, _P]),
+    "ptj_attn_decode_workspace_bytes": (c_size_t, [_P, _P, c_int]),
+    "ptj_attn_decode": (c_int, [_P, _P, c_float, _P, _P, c_int64, _P, c_size_t, _P]),
+    "ptj_kv_evict": (c_int, [_P, _P, c_int64, c_int64, c_int64, c_int64, _P, c_int64, _P, c_int64, _P, _P, _P]),
+    "ptj_verify_drafts": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int, _P]),
     "ptj_cast_f32_to_bf16": (c_int, [_P, _P, c_int64, _P]),
 }
 

@@ -6,7 +6,7 @@
 //
 // The keys of a segment (sequence, key head, block of rows) are taken in steps of KS = 4 to 16. Two ways to share them out:
 //
-// * One block per segment, its eight warps taking steps in turn and joining their sums in shared memory: one launch, no second
+// * One block per segment, its 8 or 16 warps taking steps in turn and joining their sums in shared memory: one launch, no second
 //   pass, for short caches and for few segments.
 // * All steps of the call form one list in which lengths, known on the device only, no longer matter, and every warp of the GPU
 //   takes an equal stretch of it. A warp that holds all steps of a segment writes its output; pieces of a segment (at most two
@@ -22,7 +22,7 @@ namespace ptj {
 
 constexpr int kDecJoinThreads = 256;
 constexpr float kDecLazy = 8.f;
-constexpr int kDecSplitWarps = 4, kDecDirectWarps = 8;
+constexpr int kDecSplitWarps = 4;
 
 struct DecodeAttn {
   PagedRows rows;
@@ -35,7 +35,7 @@ struct DecodeAttn {
   int64_t weights_ld, scores_ld;
   float *part, *part_ml;     // pieces: [warps][2][prows][kDim], [..][2] reference exponent and sum
   float* ml;                 // [segments][prows][2] of segments that one warp did
-  int64_t* starts;           // [B + 1] steps of a key head's block of rows before each sequence
+  int64_t* starts;           // [B + 1]: place of each sequence's first step in the list; steps of a warp's stretch
   float* scores;             // [batch * key heads][R][scores_ld], log2 units; NULL without weights
   float scale, keep;         // log2(e) / sqrt(d); 1 - p
   int B, Hk, G, T, D, R;
@@ -74,11 +74,13 @@ struct Segment {
   int b, h, rb;
   int n, first;  // keys, position of the first new token
   int count;
+  const int32_t* table;
   __device__ __forceinline__ void set_sequence(const DecodeAttn& p, int seq) {
     b = seq;
     n = p.rows.length(p.lengths, b);
     count = p.rows.count(p.counts, p.T, b);
     first = n - count;
+    table = p.rows.table + b * p.rows.table_ld;
   }
   // last key that row r (of all R) attends, -1: none
   __device__ __forceinline__ int limit(const DecodeAttn& p, int r) const {
@@ -88,92 +90,125 @@ struct Segment {
   __device__ __forceinline__ int64_t index(const DecodeAttn& p) const {
     return (static_cast<int64_t>(b) * p.Hk + h) * p.nrb + rb;
   }
+  // scores of row r, and the next row's behind them
+  __device__ __forceinline__ float* score_row(const DecodeAttn& p, int r) const {
+    return p.scores + ((static_cast<int64_t>(b) * p.Hk + h) * p.R + r) * p.scores_ld;
+  }
   __device__ __forceinline__ const char* q_row(const DecodeAttn& p, int r) const {
     return p.q + b * p.qs[0] + (h * p.G + r / p.T) * p.qs[1] + (r % p.T) * p.qs[2];
   }
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const char* src, bool on) {
-  const int n = on ? 16 : 0;  // 0: the destination is filled with zeros, nothing is read
+// n: 16, or 0 to fill the destination with zeros (nothing is read then)
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src, int n) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
-// Place of 16-byte piece c of row r of a step: pieces are swapped so that both ways the tensor-core fragments read a step
-// (a few pieces of eight consecutive rows, a piece of every second row) touch all banks.
-__device__ __forceinline__ int swizzled(int r, int c) { return c ^ ((((r >> 1) & 3) << 1) ^ ((r & 1) << 2)); }
+// Place of 16-byte piece c of row r of a step: c ^ swizzle(r). Pieces are swapped so that both ways the tensor-core fragments read a
+// step (a few pieces of eight consecutive rows, a piece of every second row) touch all banks. swizzle(a ^ b) is swizzle(a) ^
+// swizzle(b), so a lane's addresses of all its rows are few registers and constants apart.
+__host__ __device__ constexpr int swizzle(int r) { return (((r >> 1) & 3) << 1) ^ ((r & 1) << 2); }
 
 template <int KS, int RB>
 __device__ __forceinline__ uint32_t* present_word(uint8_t* stage) { return reinterpret_cast<uint32_t*>(stage + 2 * KS * RB); }
 template <int KS, int RB>
 __device__ __forceinline__ uint32_t present_keys(const uint8_t* stage) { return *reinterpret_cast<const uint32_t*>(stage + 2 * KS * RB); }
 
-// A step: KS rows of keys, KS rows of values, of RB bytes each, and a word that says which of them exist. `sub`: number of the step
-// in its sequence. Rows the table does not place and keys behind the last one become zeros. New rows are taken from where they
-// are and put into their pages.
+// Copies steps: KS rows of keys, KS rows of values, of RB bytes each, and a word that says which of them exist. Rows the table does
+// not place and keys behind the last one become zeros. New rows are taken from where they are and put into their pages.
 template <int KS, int RB>
-__device__ __forceinline__ void fetch_step(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage) {
-  constexpr int PIECES = RB / 16, ROWS = PIECES >= 32 ? 1 : 32 / PIECES, COLS = PIECES >= 32 ? PIECES / 32 : 1;
-  const int lane = threadIdx.x & 31, j0 = sub * KS;
-  const int32_t* table = p.rows.table + sg.b * p.rows.table_ld;
-  const uint32_t to = tc::smem_u32(stage);
-  const int row0 = PIECES >= 32 ? 0 : lane / PIECES, c0 = PIECES >= 32 ? lane : lane % PIECES;
-  if (p.wide && j0 + KS <= sg.first && p.rows.page_size % KS == 0) {  // in one page, nothing new
+struct Fetcher {
+  static constexpr int PIECES = RB / 16, ROWS = PIECES >= 32 ? 1 : 32 / PIECES, COLS = PIECES >= 32 ? PIECES / 32 : 1;
+  int row0, c0;      // this lane's first row and piece
+  uint32_t to;       // its place in a step
+  bool paged, dense; // a step lies in one page; its rows lie one behind the other
+  __device__ __forceinline__ void init(const DecodeAttn& p) {
+    const int lane = threadIdx.x & 31;
+    row0 = PIECES >= 32 ? 0 : lane / PIECES;
+    c0 = PIECES >= 32 ? lane : lane % PIECES;
+    to = row0 * RB + ((c0 ^ swizzle(row0)) << 4);
+    paged = p.wide && p.rows.page_size % KS == 0;
+    dense = p.rows.slot_stride[0] == RB && p.rows.slot_stride[1] == RB;
+  }
+  // sub: number of the step in its sequence
+  __device__ __forceinline__ void fetch(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage) const {
+    const int j0 = sub * KS;
+    if (!paged || j0 + KS > sg.first) {
+      mixed(p, sg, j0, stage);
+      return;
+    }
     int64_t page;
     int slot;
-    const bool on = p.rows.locate(table, j0, page, slot);
-    const char* k = p.k + p.rows.offset(0, page, sg.h, slot) + row0 * p.rows.slot_stride[0];
-    const char* v = p.v + p.rows.offset(1, page, sg.h, slot) + row0 * p.rows.slot_stride[1];
+    const bool on = p.rows.locate(sg.table, j0, page, slot);
+    if ((threadIdx.x & 31) == 0) *present_word<KS, RB>(stage) = on ? (1u << KS) - 1u : 0u;
+    if (!on) page = slot = 0;  // (nothing is read)
+    const char* k = p.k + p.rows.offset(0, page, sg.h, slot);
+    const char* v = p.v + p.rows.offset(1, page, sg.h, slot);
+    if (dense) rows<true>(p, k + (row0 * RB + c0 * 16), v + (row0 * RB + c0 * 16), on, tc::smem_u32(stage));
+    else rows<false>(p, k + row0 * p.rows.slot_stride[0] + c0 * 16, v + row0 * p.rows.slot_stride[1] + c0 * 16, on, tc::smem_u32(stage));
+  }
+  template <bool DENSE>
+  __device__ __forceinline__ void rows(const DecodeAttn& p, const char* k, const char* v, bool on, uint32_t stage) const {
+    const int64_t ks = ROWS * p.rows.slot_stride[0], vs = ROWS * p.rows.slot_stride[1];
 #pragma unroll
     for (int x = 0; x < COLS; ++x) {
-      const int c = c0 + 32 * x;
-      const bool in = on && c * 16 < p.rows.row_bytes;
+      const int n = on && (c0 + 32 * x) * 16 < p.rows.row_bytes ? 16 : 0;
+      const char *kr = k + 512 * x, *vr = v + 512 * x;
 #pragma unroll
       for (int i = 0; i < KS; i += ROWS) {
-        const int r = i + row0;
-        copy16(to + r * RB + swizzled(r, c) * 16, in ? k + i * p.rows.slot_stride[0] + c * 16 : p.k, in);
-        copy16(to + (KS + r) * RB + swizzled(r, c) * 16, in ? v + i * p.rows.slot_stride[1] + c * 16 : p.v, in);
-      }
-    }
-    if (lane == 0) *present_word<KS, RB>(stage) = on ? (1u << KS) - 1u : 0u;
-    return;
-  }
-  uint32_t present = 0;
-#pragma unroll 1
-  for (int i = 0; i < KS; i += ROWS) {
-    const int r = i + row0, j = j0 + r;
-    int64_t page = 0;
-    int slot = 0;
-    const bool on = j < sg.n && p.rows.locate(table, j, page, slot);
-    const bool fresh = on && j >= sg.first && p.kn != nullptr;
-    const unsigned lanes = __ballot_sync(0xffffffffu, on);
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) present |= (lanes >> (k * (PIECES >= 32 ? 0 : PIECES)) & 1u) << (i + k);
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      char* at = (kv == 0 ? p.k : p.v) + p.rows.offset(kv, page, sg.h, slot);
-      const int64_t* s = kv == 0 ? p.kns : p.vns;
-      const char* src = fresh ? (kv == 0 ? p.kn : p.vn) + sg.b * s[0] + sg.h * s[1] + (j - sg.first) * s[2] : at;
-#pragma unroll
-      for (int x = 0; x < COLS; ++x) {
-        const int c = c0 + 32 * x;
-        const int left = on ? p.rows.row_bytes - c * 16 : 0;  // bytes of the row from this piece on
-        uint8_t* dst = stage + (kv * KS + r) * RB + swizzled(r, c) * 16;
-        if (p.wide) {
-          copy16(tc::smem_u32(dst), left > 0 ? src + c * 16 : p.k, left > 0);
-          if (fresh && left > 0 && sg.rb == 0) *reinterpret_cast<uint4*>(at + c * 16) = *reinterpret_cast<const uint4*>(src + c * 16);
-        } else {  // rows that are not on 16-byte boundaries: by 2 bytes (elements are whole numbers of them)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint16_t val = 2 * e < left ? *reinterpret_cast<const uint16_t*>(src + c * 16 + 2 * e) : 0;
-            *reinterpret_cast<uint16_t*>(dst + 2 * e) = val;
-            if (fresh && 2 * e < left && sg.rb == 0) *reinterpret_cast<uint16_t*>(at + c * 16 + 2 * e) = val;
-          }
+        const uint32_t dst = stage + ((to ^ (swizzle(i) << 4)) + i * RB + 512 * x);
+        copy16(dst, DENSE ? kr + i * RB : kr, n);
+        copy16(dst + KS * RB, DENSE ? vr + i * RB : vr, n);
+        if (!DENSE) {
+          kr += ks;
+          vr += vs;
         }
       }
     }
   }
-  if (lane == 0) *present_word<KS, RB>(stage) = present;
-}
+  // a step that is not all in one page, or holds new keys or the last one (arguments by value: nothing of the caller's is
+  // forced into memory)
+  static __device__ __noinline__ void mixed(const DecodeAttn& p, const Segment sg, int j0, uint8_t* stage) {
+    const int lane = threadIdx.x & 31, row0 = PIECES >= 32 ? 0 : lane / PIECES, c0 = PIECES >= 32 ? lane : lane % PIECES;
+    uint32_t present = 0;
+#pragma unroll 1
+    for (int i = 0; i < KS; i += ROWS) {
+      const int r = i + row0, j = j0 + r;
+      int64_t page = 0;
+      int slot = 0;
+      const bool on = j < sg.n && p.rows.locate(sg.table, j, page, slot);
+      const bool fresh = on && j >= sg.first && p.kn != nullptr;
+      const unsigned lanes = __ballot_sync(0xffffffffu, on);
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) present |= (lanes >> (k * (PIECES >= 32 ? 0 : PIECES)) & 1u) << (i + k);
+      if (!on) page = slot = 0;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        char* at = (kv == 0 ? p.k : p.v) + p.rows.offset(kv, page, sg.h, slot);
+        const int64_t* s = kv == 0 ? p.kns : p.vns;
+        const char* src = fresh ? (kv == 0 ? p.kn : p.vn) + sg.b * s[0] + sg.h * s[1] + (j - sg.first) * s[2] : at;
+#pragma unroll
+        for (int x = 0; x < COLS; ++x) {
+          const int c = c0 + 32 * x;
+          const int left = on ? p.rows.row_bytes - c * 16 : 0;  // bytes of the row from this piece on
+          uint8_t* dst = stage + (kv * KS + r) * RB + ((c ^ swizzle(r)) << 4);
+          if (p.wide) {
+            copy16(tc::smem_u32(dst), src + c * 16, left > 0 ? 16 : 0);
+            if (fresh && left > 0 && sg.rb == 0) *reinterpret_cast<uint4*>(at + c * 16) = *reinterpret_cast<const uint4*>(src + c * 16);
+          } else {  // rows that are not on 16-byte boundaries: by 2 bytes (elements are whole numbers of them)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const uint16_t val = 2 * e < left ? *reinterpret_cast<const uint16_t*>(src + c * 16 + 2 * e) : 0;
+              *reinterpret_cast<uint16_t*>(dst + 2 * e) = val;
+              if (fresh && 2 * e < left && sg.rb == 0) *reinterpret_cast<uint16_t*>(at + c * 16 + 2 * e) = val;
+            }
+          }
+        }
+      }
+    }
+    if ((threadIdx.x & 31) == 0) *present_word<KS, RB>(stage) = present;
+  }
+};
 
 // Sum over the rows of a key of exp2(score - reference) / sum for keys [j0, j1) of a sequence's key head, onto the accumulated
 // weights. row_ml(r): reference exponent and reciprocal sum of row r.
@@ -236,10 +271,10 @@ __device__ __forceinline__ int steps_of(int n) { return (n + Core::KS - 1) / Cor
 
 // ---- a block per segment -------------------------------------------------------------------------------------------------
 template <typename E, typename Core>
-__global__ void __launch_bounds__(kDecDirectWarps * 32, 1)
+__global__ void __launch_bounds__(Core::kDirectWarps * 32, 1)
 attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
   grid_dep_sync();
-  constexpr int NW = kDecDirectWarps, LD = Core::kDim + 4, D = Core::kDepth;
+  constexpr int NW = Core::kDirectWarps, LD = Core::kDim + 4, D = Core::kDepth;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float ml[NW][Core::kRows][2], fac[NW][Core::kRows], fin[Core::kRows][2];
   const int tid = threadIdx.x, warp = tid >> 5;
@@ -250,9 +285,11 @@ attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
   sg.rb = hr % p.nrb;
   uint8_t* ring = smem + warp * ring_bytes<Core>();
   const int steps = steps_of<Core>(sg.n);
+  Fetcher<Core::KS, Core::kRowBytes> fetcher;
+  fetcher.init(p);
 #pragma unroll 1
   for (int i = 0; i < D - 1; ++i) {
-    if (warp + i * NW < steps) fetch_step<Core::KS, Core::kRowBytes>(p, sg, warp + i * NW, ring + i * stage_bytes<Core>());
+    if (warp + i * NW < steps) fetcher.fetch(p, sg, warp + i * NW, ring + i * stage_bytes<Core>());
     cp_async_commit();
   }
   Core core;
@@ -262,7 +299,7 @@ attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
     cp_async_wait<D - 2>();
     __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
     const int ahead = s + (D - 1) * NW;
-    if (ahead < steps) fetch_step<Core::KS, Core::kRowBytes>(p, sg, ahead, ring + free_slot * stage_bytes<Core>());
+    if (ahead < steps) fetcher.fetch(p, sg, ahead, ring + free_slot * stage_bytes<Core>());
     cp_async_commit();
     core.step(p, sg, s, ring + slot * stage_bytes<Core>());
     slot = slot + 1 == D ? 0 : slot + 1;
@@ -326,8 +363,7 @@ __device__ __forceinline__ int64_t steps_per_worker(const DecodeAttn& p, int64_t
 template <typename Core>
 struct Cursor {
   Segment sg;
-  int s, steps;
-  int64_t left;
+  int s, steps, left;
   // one step on; false: the stretch ends. `last` says that the step left was its segment's last in the stretch.
   __device__ __forceinline__ bool segment_ends() const { return s + 1 == steps || left == 1; }
   __device__ __forceinline__ void advance(const DecodeAttn& p) {
@@ -375,7 +411,7 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
   int64_t acc = before;
   for (int b = b0; b < b1; ++b) {
     const int64_t t = steps_of<Core>(p.rows.length(p.lengths, b));
-    if (blockIdx.x == 0) p.starts[b] = acc;
+    if (blockIdx.x == 0) p.starts[b] = acc * heads;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const int64_t at = (static_cast<int64_t>(blockIdx.x) * NW + w) * q;
@@ -386,12 +422,12 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
     }
     acc += t;
   }
-  if (blockIdx.x == 0 && tid == 0) p.starts[p.B] = total;
+  if (blockIdx.x == 0 && tid == 0) p.starts[p.B] = q;
   __syncthreads();
   const int64_t worker = static_cast<int64_t>(blockIdx.x) * NW + warp, range0 = worker * q;
   Cursor<Core> cur;
-  cur.left = min(q, all - range0);
-  if (cur.left <= 0) return;
+  cur.left = static_cast<int>(min(q, all - range0));
+  if (range0 >= all) return;
   cur.sg.set_sequence(p, static_cast<int>(start_s[warp][0]));
   cur.steps = steps_of<Core>(cur.sg.n);
   const int64_t in_seq = range0 - start_s[warp][1], hr = divide(in_seq, cur.steps);
@@ -399,11 +435,13 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
   cur.sg.h = static_cast<int>(hr) / p.nrb;
   cur.sg.rb = static_cast<int>(hr) - cur.sg.h * p.nrb;
   uint8_t* ring = smem + warp * ring_bytes<Core>();
+  Fetcher<Core::KS, Core::kRowBytes> fetcher;
+  fetcher.init(p);
   Cursor<Core> ahead = cur;
 #pragma unroll 1
   for (int i = 0; i < D - 1; ++i) {
     if (ahead.left > 0) {
-      fetch_step<Core::KS, Core::kRowBytes>(p, ahead.sg, ahead.s, ring + i * stage_bytes<Core>());
+      fetcher.fetch(p, ahead.sg, ahead.s, ring + i * stage_bytes<Core>());
       ahead.advance(p);
     }
     cp_async_commit();
@@ -418,7 +456,7 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
       cp_async_wait<D - 2>();
       __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
       if (ahead.left > 0) {
-        fetch_step<Core::KS, Core::kRowBytes>(p, ahead.sg, ahead.s, ring + free_slot * stage_bytes<Core>());
+        fetcher.fetch(p, ahead.sg, ahead.s, ring + free_slot * stage_bytes<Core>());
         ahead.advance(p);
       }
       cp_async_commit();
@@ -453,93 +491,113 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
   cp_async_wait<0>();
 }
 
-// Blocks [0, rows_blocks): a query row each, joined where several warps hold pieces of it, zero where there is nothing to attend.
-// The others: the weights of a stretch of one sequence's and key head's keys.
-template <typename E, typename Core>
+// Pieces of a segment: which warps hold some, and where.
+struct Pieces {
+  int64_t w0, w1, t0, q;
+  __device__ __forceinline__ Pieces(const DecodeAttn& p, const Segment& sg, int rb, int steps) {
+    q = p.starts[p.B];
+    t0 = p.starts[sg.b] + (static_cast<int64_t>(sg.h) * p.nrb + rb) * steps;
+    w0 = divide(t0, q);
+    w1 = divide(t0 + steps - 1, q);
+  }
+  // a segment that starts where a warp's stretch starts is its first piece, as is one that started before
+  __device__ __forceinline__ int64_t row(const DecodeAttn& p, int64_t w, int rr) const {
+    return (w * 2 + (t0 <= w * q ? 0 : 1)) * p.prows + rr;
+  }
+};
+
+// Blocks [0, rows_blocks): WPR warps per query row, joined where several warps hold pieces of it, zero where there is nothing to
+// attend. The others: the weights of a stretch of one sequence's and key head's keys.
+template <typename E, typename Core, int WPR>
 __global__ void __launch_bounds__(kDecJoinThreads)
 attn_decode_join_kernel(const __grid_constant__ DecodeAttn p, int rows_blocks, int chunk, int chunks) {
   grid_dep_sync();
-  constexpr int N = kDecJoinThreads, kVecs = Core::kDim / 4, kGroups = N / kVecs;
-  static_assert(kVecs <= N && kGroups <= 32, "");
-  __shared__ float red[33], sums[kGroups];
-  __shared__ float4 part_s[kGroups][kVecs];
-  const int tid = threadIdx.x;
-  const bool row_block = blockIdx.x < rows_blocks;
-  const int id = row_block ? blockIdx.x / p.R : (blockIdx.x - rows_blocks) / chunks;
+  constexpr int N = kDecJoinThreads, PER = N / 32 / WPR;            // rows of a block
+  constexpr int kVecs = Core::kDim / 4, kGroups = WPR * 32 / kVecs > 0 ? WPR * 32 / kVecs : 1, kReach = kVecs > WPR * 32 ? kVecs / (WPR * 32) : 1;
+  const int tid = threadIdx.x, lane = tid & 31;
   Segment sg;
-  sg.set_sequence(p, id / p.Hk);
-  sg.h = id % p.Hk;
-  const int steps = steps_of<Core>(sg.n);
-  const int64_t q = steps_per_worker(p, p.starts[p.B]), t_seq = p.starts[sg.b] * p.Hk * p.nrb;
-  auto pieces = [&](int rb, int64_t& w0, int64_t& w1) {
-    const int64_t t0 = t_seq + (static_cast<int64_t>(sg.h) * p.nrb + rb) * steps;
-    w0 = divide(t0, q);
-    w1 = divide(t0 + steps - 1, q);
-    return t0;
-  };
-  // a segment that starts where a warp's stretch starts is its first piece, as is one that started before
-  auto slot_of = [&](int64_t w, int64_t t0) { return w * 2 + (t0 <= w * q ? 0 : 1); };
-  if (row_block) {
-    const int r = blockIdx.x % p.R;
+  if (blockIdx.x < rows_blocks) {
+    __shared__ float2 sums[PER][kGroups];
+    __shared__ float4 part_s[PER][kGroups][kVecs];
+    const int slot = tid / (WPR * 32), t = tid % (WPR * 32);
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * PER + slot;  // row of all
+    const bool there = id < static_cast<int64_t>(p.B) * p.Hk * p.R;
+    const int bh = there ? static_cast<int>(id / p.R) : 0, r = there ? static_cast<int>(id % p.R) : 0;
+    sg.set_sequence(p, bh / p.Hk);
+    sg.h = bh % p.Hk;
     sg.rb = r / Core::kRows;
-    const int rr = r % Core::kRows, d = tid % kVecs * 4, grp = tid / kVecs;
-    if (sg.limit(p, r) < 0 || steps == 0) {
-      if (grp == 0 && d < p.D) store_out<E>(p, sg, r, d, make_float4(0.f, 0.f, 0.f, 0.f));
-      return;
-    }
-    int64_t w0, w1;
-    const int64_t t0 = pieces(sg.rb, w0, w1);
-    if (w0 == w1) return;
-    float m = -INFINITY;
-    for (int64_t w = w0 + tid; w <= w1; w += N) m = fmaxf(m, p.part_ml[(slot_of(w, t0) * p.prows + rr) * 2]);
-    m = block_max(m, red);
-    float l = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (grp < kGroups) {
+    const int rr = r % Core::kRows, grp = t / kVecs, steps = steps_of<Core>(sg.n);
+    const bool some = there && sg.limit(p, r) >= 0 && steps > 0;
+    const Pieces pc(p, sg, sg.rb, steps > 0 ? steps : 1);
+    const bool split = some && pc.w0 != pc.w1;
+    float m = -INFINITY, l = 0.f;
+    float4 x[kReach];
+#pragma unroll
+    for (int k = 0; k < kReach; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (split) {
+      // every group of lanes takes every kGroups-th piece, relative to a maximum of its own
 #pragma unroll 4
-      for (int64_t w = w0 + grp; w <= w1; w += kGroups) {
-        const int64_t s = slot_of(w, t0) * p.prows + rr;
+      for (int64_t w = pc.w0 + grp; w <= pc.w1; w += kGroups) m = fmaxf(m, p.part_ml[pc.row(p, w, rr) * 2]);
+#pragma unroll 4
+      for (int64_t w = pc.w0 + grp; w <= pc.w1; w += kGroups) {
+        const int64_t s = pc.row(p, w, rr);
         const float f = rebase(p.part_ml[s * 2], m);
         l = fmaf(f, p.part_ml[s * 2 + 1], l);
-        if (d < p.D) {
-          const float4 y = *reinterpret_cast<const float4*>(p.part + s * Core::kDim + d);
-          x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+#pragma unroll
+        for (int k = 0; k < kReach; ++k) {
+          const int d = (t % kVecs + k * WPR * 32) * 4;
+          if (d < p.D) {
+            const float4 y = *reinterpret_cast<const float4*>(p.part + s * Core::kDim + d);
+            x[k].x = fmaf(f, y.x, x[k].x); x[k].y = fmaf(f, y.y, x[k].y); x[k].z = fmaf(f, y.z, x[k].z); x[k].w = fmaf(f, y.w, x[k].w);
+          }
         }
       }
-      part_s[grp][tid % kVecs] = x;
-      if (tid % kVecs == 0) sums[grp] = l;
     }
-    __syncthreads();
-    if (grp == 0 && d < p.D) {
-      float sum = 0.f;
-      x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (kGroups > 1) {
+      part_s[slot][grp][t % kVecs] = x[0];
+      if (t % kVecs == 0) sums[slot][grp] = make_float2(m, l);
+      if constexpr (WPR > 1) __syncthreads();
+      else __syncwarp();
+      if (grp > 0) return;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) m = fmaxf(m, sums[slot][k].x);
+      l = 0.f;
+      x[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
       for (int k = 0; k < kGroups; ++k) {
-        const float4 y = part_s[k][tid];
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-        sum += sums[k];
+        const float f = rebase(sums[slot][k].x, m);
+        const float4 y = part_s[slot][k][t % kVecs];
+        l = fmaf(f, sums[slot][k].y, l);
+        x[0].x = fmaf(f, y.x, x[0].x); x[0].y = fmaf(f, y.y, x[0].y); x[0].z = fmaf(f, y.z, x[0].z); x[0].w = fmaf(f, y.w, x[0].w);
       }
-      store_out<E>(p, sg, r, d, scaled(x, p.keep / sum));
+    }
+    if (!there || (some && !split)) return;
+#pragma unroll
+    for (int k = 0; k < kReach; ++k) {
+      const int d = (t % kVecs + k * WPR * 32) * 4;
+      if (d < p.D) store_out<E>(p, sg, r, d, some ? scaled(x[k], p.keep / l) : make_float4(0.f, 0.f, 0.f, 0.f));
     }
     return;
   }
-  const int j0 = (blockIdx.x - rows_blocks) % chunks * chunk;
+  const int id = (blockIdx.x - rows_blocks) / chunks;
+  sg.set_sequence(p, id / p.Hk);
+  sg.h = id % p.Hk;
+  const int j0 = (blockIdx.x - rows_blocks) % chunks * chunk, steps = steps_of<Core>(sg.n);
   if (j0 >= sg.n) return;
   extern __shared__ float2 row_ml[];  // [R]
-  const int lane = tid & 31;
   for (int r = tid >> 5; r < p.R; r += N / 32) {  // a warp per row
-    int64_t w0, w1;
     const int rb = r / Core::kRows, rr = r % Core::kRows;
-    const int64_t t0 = pieces(rb, w0, w1);
+    const Pieces pc(p, sg, rb, steps);
     float m = -INFINITY, l = 0.f;
-    if (w0 == w1) {
+    if (pc.w0 == pc.w1) {
       const float* s = p.ml + ((static_cast<int64_t>(id) * p.nrb + rb) * p.prows + rr) * 2;
       m = s[0];
       l = s[1];
     } else {
-      for (int64_t w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, p.part_ml[(slot_of(w, t0) * p.prows + rr) * 2]);
+      for (int64_t w = pc.w0 + lane; w <= pc.w1; w += 32) m = fmaxf(m, p.part_ml[pc.row(p, w, rr) * 2]);
       m = warp_max(m);
-      for (int64_t w = w0 + lane; w <= w1; w += 32) {
-        const float* s = p.part_ml + (slot_of(w, t0) * p.prows + rr) * 2;
+      for (int64_t w = pc.w0 + lane; w <= pc.w1; w += 32) {
+        const float* s = p.part_ml + pc.row(p, w, rr) * 2;
         l = fmaf(rebase(s[0], m), s[1], l);
       }
       l = warp_sum(l);
@@ -564,23 +622,27 @@ bool set_smem(K kernel, int bytes) {
 template <typename E, typename Core>
 int launch_decode(const DecodeAttn& d, bool split, cudaStream_t st) {
   if (!split) {
-    constexpr int ring = kDecDirectWarps * ring_bytes<Core>(), sums = kDecDirectWarps * Core::kRows * (Core::kDim + 4) * 4;
+    constexpr int ring = Core::kDirectWarps * ring_bytes<Core>(), sums = Core::kDirectWarps * Core::kRows * (Core::kDim + 4) * 4;
     constexpr int smem = ring > sums ? ring : sums;
     if (!set_smem(attn_decode_direct_kernel<E, Core>, smem)) return PTJ_ERR_LAUNCH;
-    launch_k(attn_decode_direct_kernel<E, Core>, d.B * d.Hk * d.nrb, kDecDirectWarps * 32, smem, st, d);
+    launch_k(attn_decode_direct_kernel<E, Core>, d.B * d.Hk * d.nrb, Core::kDirectWarps * 32, smem, st, d);
     PTJ_CHECK_LAUNCH();
     return PTJ_OK;
   }
   constexpr int smem = kDecSplitWarps * ring_bytes<Core>();
+  // rows that many warps hold pieces of are joined by a block each: where there are few rows
   const int64_t rows = static_cast<int64_t>(d.B) * d.Hk * d.R;
+  const bool few = rows <= 2 * kNumSMs;
+  const int64_t row_blocks = few ? rows : ceil_div(rows, kDecJoinThreads / 32);
   const int64_t chunks = d.scores == nullptr ? 1 : ceil_div(d.rows.capacity, kWeightsChunk);
-  const int64_t blocks = rows + (d.scores == nullptr ? 0 : static_cast<int64_t>(d.B) * d.Hk * chunks);
+  const int64_t blocks = row_blocks + (d.scores == nullptr ? 0 : static_cast<int64_t>(d.B) * d.Hk * chunks);
   if (blocks > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
   if (!set_smem(attn_decode_split_kernel<E, Core>, smem)) return PTJ_ERR_LAUNCH;
   launch_k(attn_decode_split_kernel<E, Core>, d.workers / kDecSplitWarps, kDecSplitWarps * 32, smem, st, d);
   PTJ_CHECK_LAUNCH();
-  launch_k(attn_decode_join_kernel<E, Core>, static_cast<int>(blocks), kDecJoinThreads, d.scores == nullptr ? 0 : d.R * 8, st, d,
-           static_cast<int>(rows), kWeightsChunk, static_cast<int>(chunks));
+  const auto join = few ? attn_decode_join_kernel<E, Core, kDecJoinThreads / 32> : attn_decode_join_kernel<E, Core, 1>;
+  launch_k(join, static_cast<int>(blocks), kDecJoinThreads, d.scores == nullptr ? 0 : d.R * 8, st, d, static_cast<int>(row_blocks),
+           kWeightsChunk, static_cast<int>(chunks));
   PTJ_CHECK_LAUNCH();
   return PTJ_OK;
 }

@@ -13,7 +13,7 @@ struct CoreFma {
   static constexpr int LPK = DP / VEC < 32 ? DP / VEC : 32, NV = DP / (VEC * LPK), KPW = 32 / LPK, W = VEC * NV;
   static constexpr int KS = 4096 / kRowBytes, KB = KS / KPW;  // keys of a step, of a lane
   static constexpr int kDepth = 3;
-  static constexpr int kBlocks = 2;
+  static constexpr int kBlocks = 2, kDirectWarps = 8;
   float q[RB][W], o[RB][W];
   float ref[RB], sum[RB];
   int sub_lane, grp;
@@ -44,7 +44,7 @@ struct CoreFma {
   __device__ __forceinline__ void read(const uint8_t* stage, int r, float (&out)[W]) const {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const uint4 x = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + swizzled(r % KS, i * LPK + sub_lane) * 16);
+      const uint4 x = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + (((i * LPK + sub_lane) ^ swizzle(r % KS)) << 4));
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {

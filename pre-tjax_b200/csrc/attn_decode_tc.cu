@@ -15,17 +15,24 @@ namespace {
 template <int DP, int NR>
 struct CoreTc {
   static constexpr int KS = 16, kRows = 8 * NR, kDim = DP, kRowBytes = 2 * DP, KU = DP / 32, VW = DP / 64;
-  static constexpr int kDepth = DP == 64 ? 4 : 3;
-  static constexpr int kBlocks = DP == 64 ? 3 : 2;  // resident per SM
+  static constexpr int kDepth = DP == 64 ? (NR == 1 ? 3 : 4) : 3;
+  static constexpr int kBlocks = DP == 64 ? (NR == 1 ? 4 : 3) : 2;  // resident per SM
+  static constexpr int kDirectWarps = DP == 64 && NR == 1 ? 16 : 8;
   uint4 q[NR][KU];
   float o[NR][DP / 16][4];
   float ref[NR][2], sum[NR][2];
   int g, c;
+  uint32_t key_at, value_at[2];  // this lane's pieces in a step
+  float* score_at;               // scores of its first row, at the first of its keys of step 0
 
   __device__ __forceinline__ void init(const DecodeAttn& p, const Segment& sg) {
     const int lane = threadIdx.x & 31;
     g = lane >> 2;
     c = lane & 3;
+    key_at = g * kRowBytes + ((c ^ swizzle(g)) << 4);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) value_at[i] = (KS + 2 * c + i) * kRowBytes + ((g ^ swizzle(2 * c + i)) << 4);
+    score_at = p.scores == nullptr ? nullptr : sg.score_row(p, sg.rb * kRows + 2 * c) + g;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int r = sg.rb * kRows + i * 8 + g;
@@ -60,12 +67,10 @@ struct CoreTc {
   __device__ __forceinline__ int key_of(int i) const { return g + 8 * i; }
   __device__ __forceinline__ int value_of(int i) const { return 2 * c + (i & 1) + 8 * (i >> 1); }
   __device__ __forceinline__ uint4 key(const uint8_t* stage, int i, int u) const {
-    const int r = key_of(i);
-    return *reinterpret_cast<const uint4*>(stage + r * kRowBytes + swizzled(r, 4 * u + c) * 16);
+    return *reinterpret_cast<const uint4*>(stage + ((key_at ^ ((u & 1) << 6)) + 8 * i * kRowBytes + (u >> 1) * 128));
   }
   __device__ __forceinline__ uint4 value(const uint8_t* stage, int i, int w) const {
-    const int r = value_of(i);
-    return *reinterpret_cast<const uint4*>(stage + (KS + r) * kRowBytes + swizzled(r, 8 * w + g) * 16);
+    return *reinterpret_cast<const uint4*>(stage + (value_at[i & 1] + 8 * (i >> 1) * kRowBytes + w * 128));
   }
 
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -128,15 +133,16 @@ struct CoreTc {
     for (int i = 0; i < NR; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) over |= s[i][e] > ref[i][e & 1] + kDecLazy;
-    if (p.scores != nullptr) {
+    if (score_at != nullptr) {
 #pragma unroll
       for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = sg.rb * kRows + i * 8 + 2 * c + (e & 1), j = j0 + key_of(e >> 1);
-          if (r < p.R && j < sg.n)
-            p.scores[((static_cast<int64_t>(sg.b) * p.Hk + sg.h) * p.R + r) * p.scores_ld + j] = s[i][e];
-        }
+        for (int e = 0; e < 2; ++e)
+          if (sg.rb * kRows + i * 8 + 2 * c + e < p.R) {
+            float* to = score_at + (i * 8 + e) * p.scores_ld + j0;
+            if (j0 + g < sg.n) to[0] = s[i][e];
+            if (j0 + g + 8 < sg.n) to[8] = s[i][e + 2];
+          }
     }
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll

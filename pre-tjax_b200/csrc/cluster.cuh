@@ -7,10 +7,12 @@ namespace ptj {
 
 // Blocks in consecutive groups of `cluster` (1, 2, 4 or 8; grid.x is a multiple).
 template <typename... KArgs, typename... Args>
-inline void launch_cluster_k(void (*kern)(KArgs...), dim3 grid, dim3 block, unsigned cluster, cudaStream_t st, Args&&... args) {
+inline void launch_cluster_k(void (*kern)(KArgs...), dim3 grid, dim3 block, unsigned cluster, size_t smem, cudaStream_t st,
+                             Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

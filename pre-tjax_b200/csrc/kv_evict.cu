@@ -2,14 +2,15 @@
 //
 // Two launches: one finds the keys that stay, one moves their rows.
 //
-// Which stay: the weights are ordered as unsigned integers; the weight of the last key to stay is found digit by digit (11, 11
-// and 10 bits) from histograms in shared memory. Above it all stay, of its equals the first ones. A cluster of C blocks shares
-// a cache, its histograms and counts meet through distributed shared memory. Bound by the chain of barriers and by the histogram
-// updates of one SM; the weights themselves are read four times, from L2 after the first.
+// Which stay: the weights are ordered as unsigned integers; the weight of the last key to stay is found digit by digit (8
+// bits) from histograms in shared memory. Above it all stay, of its equals the first ones. A cluster of C blocks shares a cache,
+// its histograms and counts meet through distributed shared memory; digits of 8 bits because reading 2048 bins of eight blocks
+// took longer (43 us for 16 caches of 64k keys) than a fourth pass. Bound by the chain of passes and barriers.
 //
 // Moving: memory bounds it. Into other pages, blocks take stretches of rows and everything is independent. In place, the row that
 // goes to place i lies at place i or behind it, so one block moves a column of 32 bytes of all rows in order, reading a round's
-// rows before it writes any: columns are independent of each other, and the next round's rows lie behind all places written.
+// rows before it writes any: columns are independent of each other, and the next round's rows lie behind all places written. A
+// row's page and slot are looked up once per round, not by every thread that copies 16 bytes of it.
 #include "cluster.cuh"
 #include "kv_cache.cuh"
 #include "tc_runtime.h"
@@ -18,8 +19,9 @@ namespace ptj {
 namespace {
 
 constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kMoveThreads = 256;
+constexpr int kDigits = 4, kBins = 256, kCopies = 2;  // weights crowd into few exponents: lanes count in two copies
+constexpr int kCached = 8192;                         // weights of a block that are kept in shared memory
+constexpr int kMoveThreads = 256, kMovePieces = 8, kMoveRows = 512;
 
 struct Evict {
   PagedRows rows;
@@ -34,8 +36,9 @@ struct Evict {
   int budget, recent, Hk;
   int pieces;        // of a row
   int cols, per_col; // columns that a row is cut into, pieces of a column
+  int round;         // rows that are on their way at a time
   int chunk, chunks; // rows of a stretch, stretches
-  int ordered[3];    // keys, values, weights: moved in place
+  int pools_in_place, weights_in_place;
 };
 
 // weights in the order of unsigned integers; a NaN is the lowest, both zeros are equal
@@ -46,42 +49,42 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 }
 
 struct SelectShared {
-  uint32_t hist[3][kBins];
-  uint32_t warp_sum[kSelWarps];
+  uint32_t hist[kDigits][kCopies][kBins];
+  uint32_t cache[kCached];
+  uint32_t warp_sum[kBins / 32];
   uint32_t bin, above;                  // the digit that was found, elements with a larger one
   uint32_t stay[kSelWarps], tie[kSelWarps];
   uint32_t block_stay, block_tie;
 };
 
-// The largest digit such that at least `want` elements have it or a larger one, and the number with a larger one.
+// The largest digit such that at least `want` elements of the cluster have it or a larger one, and the number with a larger one.
 template <int C>
-__device__ __forceinline__ void find_digit(SelectShared& sm, const uint32_t* hist, uint32_t want) {
+__device__ __forceinline__ void find_digit(SelectShared& sm, uint32_t (&hist)[kCopies][kBins], uint32_t want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // thread t: digits from the top, two each
-  uint32_t n[2];
+  uint32_t n = 0, incl = 0;
+  if (tid < kBins) {  // thread t: the t-th digit from the top
+    if constexpr (C > 1) {  // (the copies of a block are its first one by now)
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    n[i] = 0;
+      for (int r = 0; r < C; ++r) n += peer_u32<C>(&hist[0][kBins - 1 - tid], r);
+    } else {
 #pragma unroll
-    for (int r = 0; r < C; ++r) n[i] += peer_u32<C>(hist + (kBins - 1 - (2 * tid + i)), r);
+      for (int k = 0; k < kCopies; ++k) n += hist[k][kBins - 1 - tid];
+    }
+    incl = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, incl, x);
+      if (lane >= x) incl += y;
+    }
+    if (lane == 31) sm.warp_sum[warp] = incl;
   }
-  uint32_t incl = n[0] + n[1];
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, incl, x);
-    if (lane >= x) incl += y;
-  }
-  if (lane == 31) sm.warp_sum[warp] = incl;
   __syncthreads();
-  const uint32_t others = lane < warp ? sm.warp_sum[lane] : 0u;
-  uint32_t before = __reduce_add_sync(0xffffffffu, others) + incl - n[0] - n[1];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (before < want && before + n[i] >= want) {
-      sm.bin = kBins - 1 - (2 * tid + i);
+  if (tid < kBins) {
+    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sm.warp_sum[lane] : 0u) + incl - n;
+    if (before < want && before + n >= want) {
+      sm.bin = kBins - 1 - tid;
       sm.above = before;
     }
-    before += n[i];
   }
   __syncthreads();
 }
@@ -90,7 +93,8 @@ template <int C>
 __global__ void __launch_bounds__(kSelThreads)
 select_kernel(const __grid_constant__ Evict p) {
   grid_dep_sync();
-  __shared__ SelectShared sm;
+  extern __shared__ __align__(16) uint8_t smem[];
+  SelectShared& sm = *reinterpret_cast<SelectShared*>(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(cluster_rank<C>());
   const int seg = blockIdx.x / C, b = seg / p.Hk;
@@ -108,20 +112,30 @@ select_kernel(const __grid_constant__ Evict p) {
   const int per = (n + C * kSelWarps * 32 - 1) / (C * kSelWarps * 32) * 32;
   const int j0 = min((rank * kSelWarps + warp) * per, n), j1 = min(j0 + per, n);
   const int c1 = min(j1, cand);
-  for (int i = tid; i < 3 * kBins; i += kSelThreads) (&sm.hist[0][0])[i] = 0u;
+  const bool cached = per * kSelWarps <= kCached;
+  uint32_t* mine = sm.cache + warp * per - j0;  // ranks of this warp's stretch, if they fit
+  auto rank_at = [&](int j) { return cached ? mine[j] : rank_of(w[j]); };
+  for (int i = tid; i < kDigits * kCopies * kBins; i += kSelThreads) (&sm.hist[0][0][0])[i] = 0u;
   __syncthreads();
   uint32_t thr = 0;  // (want 0: nothing but the recent ones stays)
   int ties = 0;
   if (want > 0) {
     uint32_t left = want;
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-      const uint32_t mask = pass == 2 ? 1023u : 2047u, known = pass == 0 ? 0u : (pass == 1 ? ~0u << 21 : ~0u << 10);
-#pragma unroll 4
+    for (int pass = 0; pass < kDigits; ++pass) {
+      const int shift = 24 - 8 * pass;
+      const uint32_t known = pass == 0 ? 0u : ~0u << (shift + 8);
+#pragma unroll 8
       for (int j = j0 + lane; j < c1; j += 32) {
-        const uint32_t r = rank_of(w[j]);
-        if ((r & known) == thr) atomicAdd(&sm.hist[pass][(r >> shift) & mask], 1u);
+        const uint32_t r = pass == 0 ? rank_of(w[j]) : rank_at(j);
+        if (pass == 0 && cached) mine[j] = r;
+        if ((r & known) == thr) atomicAdd(&sm.hist[pass][lane % kCopies][(r >> shift) & 255u], 1u);
+      }
+      if constexpr (C > 1) {
+        __syncthreads();
+        if (tid < kBins)
+#pragma unroll
+          for (int k = 1; k < kCopies; ++k) sm.hist[pass][0][tid] += sm.hist[pass][k][tid];
       }
       cluster_barrier<C>();
       find_digit<C>(sm, sm.hist[pass], left);
@@ -131,15 +145,18 @@ select_kernel(const __grid_constant__ Evict p) {
     ties = static_cast<int>(left);  // equals of the threshold that stay
   }
   // numbers of keys above the threshold (or recent) and of equals before each warp's stretch
-  int stay = 0, tie = 0;
-#pragma unroll 4
-  for (int j = j0 + lane; j < j1; j += 32) {
-    const uint32_t r = rank_of(w[j]);
-    stay += j >= cand || (want > 0 && r > thr);
-    tie += j < cand && want > 0 && r == thr;
+  int stay = max(j1 - max(j0, cand), 0), tie = 0;
+  if (want > 0) {
+    int s = 0;
+#pragma unroll 8
+    for (int j = j0 + lane; j < c1; j += 32) {
+      const uint32_t r = rank_at(j);
+      s += r > thr;
+      tie += r == thr;
+    }
+    stay += __reduce_add_sync(0xffffffffu, s);
+    tie = __reduce_add_sync(0xffffffffu, tie);
   }
-  stay = __reduce_add_sync(0xffffffffu, stay);
-  tie = __reduce_add_sync(0xffffffffu, tie);
   if (lane == 0) {
     sm.stay[warp] = stay;
     sm.tie[warp] = tie;
@@ -163,7 +180,7 @@ select_kernel(const __grid_constant__ Evict p) {
     cluster_barrier<C>();  // everything is read: a block may leave
   }
   for (int j = j0 + lane; j - lane < j1; j += 32) {
-    const uint32_t r = j < j1 ? rank_of(w[j]) : 0u;
+    const uint32_t r = j < c1 && want > 0 ? rank_at(j) : 0u;
     const bool equal = j < c1 && want > 0 && r == thr;
     const bool above = j < j1 && (j >= cand || (want > 0 && r > thr));
     const unsigned em = __ballot_sync(0xffffffffu, equal), am = __ballot_sync(0xffffffffu, above), low = (1u << lane) - 1u;
@@ -174,19 +191,22 @@ select_kernel(const __grid_constant__ Evict p) {
   }
 }
 
-// x: segment and column (columns of a row side by side); y: keys, values, weights; z: stretch of rows
-template <typename V, int U>
-__global__ void __launch_bounds__(kMoveThreads)
+// x: segment and column; y: keys and values, or weights; z: stretch of rows. A round: `round` rows, whose places (page and slot, from
+// and to) one thread each looks up; the next round's are looked up while this one's rows are on their way.
+template <typename V>
+__global__ void __launch_bounds__(kMoveThreads, 2)
 move_kernel(const __grid_constant__ Evict p) {
   grid_dep_sync();
-  const int kv = blockIdx.y, tid = threadIdx.x;
-  const int seg = blockIdx.x / p.cols, col = blockIdx.x % p.cols, b = seg / p.Hk, h = seg % p.Hk;
+  constexpr int U = kMovePieces;
+  __shared__ int2 from_s[3][kMoveRows], to_s[3][kMoveRows];
+  const int tid = threadIdx.x, seg = blockIdx.x / p.cols, col = blockIdx.x % p.cols, b = seg / p.Hk, h = seg % p.Hk;
+  const bool pools = blockIdx.y == 0, ordered = pools ? p.pools_in_place : p.weights_in_place;
   const int keep = min(p.rows.length(p.lengths, b), p.budget);
   const int32_t* kept = p.kept + static_cast<int64_t>(seg) * p.budget;
-  if (p.ordered[kv] && blockIdx.z > 0) return;
-  const int first = p.ordered[kv] ? 0 : blockIdx.z * p.chunk, last = p.ordered[kv] ? keep : min(keep, first + p.chunk);
+  if (ordered && blockIdx.z > 0) return;
+  const int first = ordered ? 0 : blockIdx.z * p.chunk, last = ordered ? keep : min(keep, first + p.chunk);
   if (first >= last) return;
-  if (kv == 2) {  // weights: in place they are moved as rows of one column are
+  if (!pools) {  // in place they are moved as rows of one column are
     if (col != 0) return;
     const float* w = p.weights + seg * p.weights_ld;
     float* out = p.weights_out + seg * p.weights_out_ld;
@@ -197,7 +217,7 @@ move_kernel(const __grid_constant__ Evict p) {
         const int i = i0 + k * kMoveThreads + tid;
         if (i < last) x[k] = w[kept[i]];
       }
-      if (p.ordered[2]) __syncthreads();
+      if (ordered) __syncthreads();
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         const int i = i0 + k * kMoveThreads + tid;
@@ -206,30 +226,61 @@ move_kernel(const __grid_constant__ Evict p) {
     }
     return;
   }
-  const int32_t *from = p.rows.table + b * p.rows.table_ld, *to = p.dst_table + b * p.dst_ld;
-  const int row = tid / p.per_col, c = col * p.per_col + tid % p.per_col;  // a thread's row in a round, its piece
-  const int step = kMoveThreads / p.per_col;                              // rows of a round
-  const bool in = row < step && c < p.pieces;
-  for (int r0 = first; r0 < last; r0 += step * U) {
-    V x[U];
-    V* dst[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int r = r0 + k * step + row;
-      dst[k] = nullptr;
-      if (!in || r >= last) continue;
-      const int j = kept[r];
-      if (p.ordered[kv] && j == r) continue;  // it lies where it belongs
-      int64_t page;
-      int slot;
-      if (!p.rows.locate(from, j, page, slot)) continue;
-      x[k] = reinterpret_cast<const V*>(p.pool[kv] + p.rows.offset(kv, page, h, slot))[c];
-      if (p.rows.locate(to, r, page, slot)) dst[k] = reinterpret_cast<V*>(p.pool[kv] + p.rows.offset(kv, page, h, slot)) + c;
+  const int32_t *src = p.rows.table + b * p.rows.table_ld, *dst = p.dst_table + b * p.dst_ld;
+  auto look_up = [&](int r0, int buf) {
+    for (int i = tid; i < p.round && r0 + i < last; i += kMoveThreads) {
+      const int r = r0 + i, j = kept[r];
+      int64_t pf = -1, pt = -1;
+      int sf = 0, st = 0;
+      const bool stays = ordered && j == r;  // it lies where it belongs
+      if (stays || !p.rows.locate(src, j, pf, sf) || !p.rows.locate(dst, r, pt, st)) pf = pt = -1;
+      from_s[buf][i] = make_int2(static_cast<int>(pf), sf);
+      to_s[buf][i] = make_int2(static_cast<int>(pt), st);  // page -1: nothing is moved
     }
-    if (p.ordered[kv]) __syncthreads();
+  };
+  const int row0 = tid / p.per_col, c0 = tid % p.per_col, rows_on = kMoveThreads / p.per_col, c_on = kMoveThreads % p.per_col;
+  look_up(first, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int r0 = first; r0 < last; r0 += p.round) {
+    V x[U], y[U];
+    const int n = min(p.round, last - r0);
+    int row = row0, c = c0;
+    auto on = [&](int k, int2& place, const int2* places) {  // k-th piece of this thread
+      if (k == 0) {
+        row = row0;
+        c = c0;
+      } else {
+        row += rows_on;
+        c += c_on;
+        if (c >= p.per_col) {
+          c -= p.per_col;
+          ++row;
+        }
+      }
+      if (row >= n || col * p.per_col + c >= p.pieces) return false;
+      place = places[row];
+      return place.x >= 0;
+    };
+    int2 at;
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      if (dst[k] != nullptr) *dst[k] = x[k];
+      if (on(k, at, from_s[buf])) {
+        const int piece = col * p.per_col + c;
+        x[k] = reinterpret_cast<const V*>(p.pool[0] + p.rows.offset(0, at.x, h, at.y))[piece];
+        y[k] = reinterpret_cast<const V*>(p.pool[1] + p.rows.offset(1, at.x, h, at.y))[piece];
+      }
+    const int next = buf == 2 ? 0 : buf + 1;  // (a thread may still store to the places of the round before)
+    if (r0 + p.round < last) look_up(r0 + p.round, next);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (on(k, at, to_s[buf])) {
+        const int piece = col * p.per_col + c;
+        reinterpret_cast<V*>(p.pool[0] + p.rows.offset(0, at.x, h, at.y))[piece] = x[k];
+        reinterpret_cast<V*>(p.pool[1] + p.rows.offset(1, at.x, h, at.y))[piece] = y[k];
+      }
+    buf = next;
   }
 }
 
@@ -238,11 +289,12 @@ void launch_select(const Evict& p, int segs, cudaStream_t st) {
   unsigned c = 8;
   while (c > 1 && (static_cast<int64_t>(segs) * c > 2 * kNumSMs || p.rows.capacity < static_cast<int64_t>(c) * 4096)) c /= 2;
   const dim3 grid(static_cast<unsigned>(segs) * c);
+  constexpr size_t smem = sizeof(SelectShared);
   switch (c) {
-    case 8: launch_cluster_k(select_kernel<8>, grid, kSelThreads, 8, st, p); break;
-    case 4: launch_cluster_k(select_kernel<4>, grid, kSelThreads, 4, st, p); break;
-    case 2: launch_cluster_k(select_kernel<2>, grid, kSelThreads, 2, st, p); break;
-    default: launch_k(select_kernel<1>, grid, kSelThreads, 0, st, p);
+    case 8: launch_cluster_k(select_kernel<8>, grid, kSelThreads, 8, smem, st, p); break;
+    case 4: launch_cluster_k(select_kernel<4>, grid, kSelThreads, 4, smem, st, p); break;
+    case 2: launch_cluster_k(select_kernel<2>, grid, kSelThreads, 2, smem, st, p); break;
+    default: launch_k(select_kernel<1>, grid, kSelThreads, smem, st, p);
   }
 }
 
@@ -284,27 +336,25 @@ extern "C" int ptj_kv_evict(const ptj_kv_cache* cache, const int32_t* dst_table,
   const int64_t piece = wide ? 16 : es;
   p.pieces = static_cast<int>(cache->d_head * es / piece);
   const int segs = static_cast<int>(cache->batch * cache->kv_heads);
-  p.ordered[0] = p.ordered[1] = in_place;
-  p.ordered[2] = weights_out == weights;
-  constexpr int U = 8;
-  // In place: columns of 32 bytes. Else whole rows (a block holds at most 256 pieces), in stretches of a few rounds.
+  p.pools_in_place = in_place;
+  p.weights_in_place = weights_out == weights;
+  // In place: columns of 32 bytes. Else whole rows, in stretches of one round each.
   p.per_col = in_place ? static_cast<int>(32 / piece) : p.pieces;
   if (p.per_col > p.pieces) p.per_col = p.pieces;
   p.cols = static_cast<int>(ceil_div(p.pieces, p.per_col));
-  p.chunk = kMoveThreads / p.per_col * U;
+  p.round = kMoveThreads * kMovePieces / p.per_col;
+  if (p.round > kMoveRows) p.round = kMoveRows;
+  p.chunk = p.round;
+  if (ceil_div(most, p.chunk) > 65535) p.chunk = static_cast<int>(ceil_div(ceil_div(most, 65535), p.round)) * p.round;
   p.chunks = static_cast<int>(ceil_div(most, p.chunk));
   const bool one = in_place && (weights_out == weights || !weights_out);
-  if (p.chunks > 65535) {
-    p.chunk = static_cast<int>(ceil_div(most, 65535));
-    p.chunks = static_cast<int>(ceil_div(most, p.chunk));
-  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   launch_select(p, segs, st);
   PTJ_CHECK_LAUNCH();
-  const dim3 grid(static_cast<unsigned>(segs) * p.cols, weights_out ? 3 : 2, one ? 1 : p.chunks);
-  if (wide) launch_k(move_kernel<uint4, U>, grid, kMoveThreads, 0, st, p);
-  else if (es == 2) launch_k(move_kernel<uint16_t, U>, grid, kMoveThreads, 0, st, p);
-  else launch_k(move_kernel<uint32_t, U>, grid, kMoveThreads, 0, st, p);
+  const dim3 grid(static_cast<unsigned>(segs) * p.cols, weights_out ? 2 : 1, one ? 1 : p.chunks);
+  if (wide) launch_k(move_kernel<uint4>, grid, kMoveThreads, 0, st, p);
+  else if (es == 2) launch_k(move_kernel<uint16_t>, grid, kMoveThreads, 0, st, p);
+  else launch_k(move_kernel<uint32_t>, grid, kMoveThreads, 0, st, p);
   PTJ_CHECK_LAUNCH();
   return PTJ_OK;
 }

@@ -13,7 +13,7 @@
 namespace ptj {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 
 struct Verify {
   const void *target, *draft;
@@ -39,6 +39,27 @@ struct Weights {
     double w = Elem<E>::load(row + j);
     if (sub != nullptr) w -= static_cast<double>(Elem<E>::load(sub + j));
     return w > 0.0 && j != skip ? w : 0.0;  // (a NaN has none)
+  }
+  // of every 32nd element from j0 + lane on; a batch of loads is under way at a time, the last one too
+  template <bool SUB>
+  __device__ __forceinline__ double sum(int j0, int j1, int lane) const {
+    constexpr int U = 8;
+    double s[2] = {0.0, 0.0};
+    for (int g = j0 + lane; g < j1; g += 32 * U) {
+      float x[U], y[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int j = g + 32 * i;
+        x[i] = j < j1 && (SUB || j != skip) ? Elem<E>::load(row + j) : 0.f;
+        y[i] = SUB && j < j1 ? Elem<E>::load(sub + j) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const double w = SUB ? static_cast<double>(x[i]) - static_cast<double>(y[i]) : static_cast<double>(x[i]);
+        s[i & 1] += w > 0.0 ? w : 0.0;
+      }
+    }
+    return s[0] + s[1];
   }
 };
 
@@ -88,10 +109,7 @@ verify_kernel(const __grid_constant__ Verify p) {
   // contiguous chunks, one per warp of the cluster
   const int per = (p.V + C * kWarps * 32 - 1) / (C * kWarps * 32) * 32;
   const int j0 = min((rank * kWarps + warp) * per, p.V), j1 = min(j0 + per, p.V);
-  double s = 0.0;
-#pragma unroll 8
-  for (int j = j0 + lane; j < j1; j += 32) s += weight(j);
-  s = warp_sum_f64(s);
+  const double s = warp_sum_f64(weight.sub != nullptr ? weight.template sum<true>(j0, j1, lane) : weight.template sum<false>(j0, j1, lane));
   if (lane == 0) chunk_s[warp] = s;
   __syncthreads();
   if (tid == 0) {
@@ -191,14 +209,14 @@ verify_kernel(const __grid_constant__ Verify p) {
 
 template <typename E>
 void launch_verify(const Verify& p, int64_t batch, cudaStream_t st) {
-  // as many blocks per sequence as leave two for each SM, each with a slice worth a round of its threads
+  // as many blocks per sequence as leave four for each SM, each with a slice worth a few rounds of its threads
   unsigned c = 8;
-  while (c > 1 && (batch * c > 2 * kNumSMs || p.V < static_cast<int64_t>(c) * kThreads)) c /= 2;
+  while (c > 1 && (batch * c > 4 * kNumSMs || p.V < static_cast<int64_t>(c) * kThreads * 2)) c /= 2;
   const dim3 grid(static_cast<unsigned>(batch) * c);
   switch (c) {
-    case 8: launch_cluster_k(verify_kernel<E, 8>, grid, kThreads, 8, st, p); break;
-    case 4: launch_cluster_k(verify_kernel<E, 4>, grid, kThreads, 4, st, p); break;
-    case 2: launch_cluster_k(verify_kernel<E, 2>, grid, kThreads, 2, st, p); break;
+    case 8: launch_cluster_k(verify_kernel<E, 8>, grid, kThreads, 8, 0, st, p); break;
+    case 4: launch_cluster_k(verify_kernel<E, 4>, grid, kThreads, 4, 0, st, p); break;
+    case 2: launch_cluster_k(verify_kernel<E, 2>, grid, kThreads, 2, 0, st, p); break;
     default: launch_k(verify_kernel<E, 1>, grid, kThreads, 0, st, p);
   }
 }

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 import weakref
 
 import torch
@@ -501,72 +502,95 @@ def t_scaled_dot_prod_attn_bkwd3_t(dloss_dx, acts, qkv: torch.Tensor, mask: torc
 
 
 # ---- paged key-value cache ----------------------------------------------------------------------------------------------
+# Descriptors are packed as the bytes of the C structs: a decoding step issues one of these calls per layer, and building ctypes
+# objects field by field took longer than a short kernel.
+_KV_CACHE = struct.Struct("=4Q13qi4x")   # _lib.KvCache
+_NEW_TOKENS = struct.Struct("=5Q14q")    # _lib.NewTokens
+_DECODE_BYTES = {}                       # sizes of a call -> workspace bytes
+
+
 def _on_current_device(*tensors):
     """Launches go to the current device's stream: tensors elsewhere are refused."""
-    dev = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    dev = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise RuntimeError("tensors must live on a CUDA device: there is no CPU implementation")
-        if t.get_device() != dev:
-            raise RuntimeError(f"tensor on cuda:{t.get_device()}, but cuda:{dev} is the current device")
+        if dev is None:
+            dev = torch._C._cuda_getDevice()
+        if at != dev:
+            raise RuntimeError(f"tensor on cuda:{at}, but cuda:{dev} is the current device")
 
 
 def _ints(t, shape, name):
     """An int32 tensor of this shape; rows of a table may be strided."""
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.stride(-1) != 1 and t.shape[-1] > 1:
+    if t.dtype != torch.int32 or t.shape != shape or t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must be an int32 tensor of shape {list(shape)} with contiguous rows")
-    return t
 
 
 def _kv_cache(k_pages, v_pages, page_table, lengths):
-    """The descriptor of a paged cache, after the checks that its tensors allow."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+    """(the bytes of the cache's descriptor, (batch, kv_heads, d_head, page_size, capacity)), after the checks that its tensors
+    allow."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must share one shape [pages, kv_heads, page_size, d_head]")
-    if k_pages.dtype != v_pages.dtype:
+    if v_pages.dtype != dtype:
         raise TypeError("k_pages and v_pages must share a dtype")
-    pages, heads, page_size, d = k_pages.shape
-    sk, sv = k_pages.stride(), v_pages.stride()
-    if d > 1 and (sk[3] != 1 or sv[3] != 1):
+    pages, heads, page_size, d = shape
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if d > 1 and (k3 != 1 or v3 != 1):
         raise ValueError("d_head must be contiguous")
     B, width = page_table.shape
-    _ints(page_table, (B, width), "page_table")
+    if page_table.dtype != torch.int32 or (width > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table must be an int32 tensor [batch, pages of a sequence] with contiguous rows")
     _ints(lengths, (B,), "lengths")
-    return _lib.KvCache(_ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(lengths), B, heads, d, pages, page_size, width,
-                        page_table.stride(0) if B > 1 else width, sk[:3], sv[:3], _dt(k_pages))
+    desc = _KV_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), B, heads, d, pages,
+                          page_size, width, page_table.stride(0) if B > 1 else width, k0, k1, k2, v0, v1, v2, _dt(k_pages))
+    return desc, (B, heads, d, page_size, width * page_size)
 
 
-def _new_tokens(cache, q, k, v, out, counts, dtype):
-    B, Hk, d = cache.batch, cache.kv_heads, cache.d_head
-    some = q if q is not None else k
+def _view(t, shape, dtype, name):
+    """(address, strides of batch, head and token) of a view of new tokens."""
+    if t is None:
+        return 0, 0, 0, 0
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must have the cache's dtype {dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}")
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 and shape[3] > 1:
+        raise ValueError(f"{name} must be {list(shape)} with d_head contiguous")
+    return t.data_ptr(), s0, s1, s2
+
+
+def _new_tokens(sizes, q, k, v, out, counts, dtype):
+    """(the bytes of the new tokens' descriptor, query heads, tokens)."""
+    B, Hk, d = sizes[:3]
+    some = k if q is None else q
     if some.dim() != 4:
         raise ValueError("new tokens must be [batch, heads, tokens, d_head]")
-    T = some.shape[2]
-    views = []
-    for t, heads, name in ((q, None, "q"), (out, None, "out"), (k, Hk, "k"), (v, Hk, "v")):
-        if t is None:
-            views.append((0, (0, 0, 0)))
-            continue
-        if t.dtype != dtype:
-            raise TypeError(f"{name} must have the cache's dtype {dtype}")
-        heads = some.shape[1] if heads is None else heads
-        if tuple(t.shape) != (B, heads, T, d) or (d > 1 and t.stride(3) != 1):
-            raise ValueError(f"{name} must be [{B}, {heads}, {T}, {d}] with d_head contiguous")
-        views.append((t.data_ptr(), t.stride()[:3]))
+    H, T = some.shape[1], some.shape[2]
+    qp, q0, q1, q2 = _view(q, (B, H, T, d), dtype, "q")
+    op, o0, o1, o2 = _view(out, (B, H, T, d), dtype, "out")
+    kp, k0, k1, k2 = _view(k, (B, Hk, T, d), dtype, "k")
+    vp, v0, v1, v2 = _view(v, (B, Hk, T, d), dtype, "v")
     if counts is not None:
         _ints(counts, (B,), "counts")
-    if q is not None and (some.shape[1] % Hk or some.shape[1] < 1):
-        raise ValueError(f"{some.shape[1]} query heads do not share {Hk} key heads evenly")
-    (qp, qs), (op, os), (kp, ks), (vp, vs) = views
-    return _lib.NewTokens(qp, kp, vp, op, _ptr(counts), some.shape[1], T, qs, os, ks, vs)
+    if q is not None and (H % Hk or H < 1):
+        raise ValueError(f"{H} query heads do not share {Hk} key heads evenly")
+    return _NEW_TOKENS.pack(qp, kp, vp, op, 0 if counts is None else counts.data_ptr(), H, T, q0, q1, q2, o0, o1, o2, k0, k1, k2,
+                            v0, v1, v2), H, T
 
 
-def _attended(weights, cache, name):
-    cap = cache.table_width * cache.page_size
+def _attended(weights, sizes, least, name):
+    """Width of a tensor of accumulated weights."""
     if weights.dtype != torch.float32 or weights.dim() != 3 or not weights.is_contiguous() or \
-            tuple(weights.shape[:2]) != (cache.batch, cache.kv_heads) or weights.shape[2] < cap:
-        raise ValueError(f"{name} must be a contiguous float32 tensor [{cache.batch}, {cache.kv_heads}, >= {cap}]")
+            weights.shape[0] != sizes[0] or weights.shape[1] != sizes[1] or weights.shape[2] < least:
+        raise ValueError(f"{name} must be a contiguous float32 tensor [{sizes[0]}, {sizes[1]}, >= {least}]")
+    return weights.shape[2]
 
 
 def kv_append(k, v, k_pages, v_pages, page_table, lengths, counts=None):
@@ -578,11 +602,11 @@ def kv_append(k, v, k_pages, v_pages, page_table, lengths, counts=None):
     says how many of the T rows are tokens. Pages, lengths and counts out of range are skipped or clamped and reported by
     last_kernel_fault."""
     _on_current_device(k, v, k_pages, v_pages, page_table, lengths, counts)
-    cache = _kv_cache(k_pages, v_pages, page_table, lengths)
-    new = _new_tokens(cache, None, k, v, None, counts, k_pages.dtype)
-    if cache.batch == 0 or new.tokens == 0:
+    cache, sizes = _kv_cache(k_pages, v_pages, page_table, lengths)
+    new, _, T = _new_tokens(sizes, None, k, v, None, counts, k_pages.dtype)
+    if sizes[0] == 0 or T == 0:
         return
-    _lib.check(_lib.lib().ptj_kv_append(ctypes.byref(cache), ctypes.byref(new), _stream()), "ptj_kv_append")
+    _lib.check(_lib.lib().ptj_kv_append(cache, new, _stream()), "ptj_kv_append")
 
 
 def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, counts=None, weights=None, weights_out=None,
@@ -596,32 +620,35 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, cou
     the query heads of a key head and the new tokens, into weights_out (default: weights; weights None counts as zeros). What
     weights holds for new keys does not matter. workspace: optional uint8 tensor, see ptj_attn_decode_workspace_bytes."""
     _on_current_device(q, k_pages, v_pages, page_table, lengths, k, v, counts, weights, weights_out, out, workspace)
-    cache = _kv_cache(k_pages, v_pages, page_table, lengths)
+    cache, sizes = _kv_cache(k_pages, v_pages, page_table, lengths)
     if out is None:
         out = torch.empty_like(q)
         if out.dim() == 4 and out.stride(3) != 1:
             out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    new = _new_tokens(cache, q, k, v, out, counts, k_pages.dtype)
-    if cache.batch == 0 or new.tokens == 0:
+    new, H, T = _new_tokens(sizes, q, k, v, out, counts, k_pages.dtype)
+    if sizes[0] == 0 or T == 0:
         return out
     if weights_out is None:
         weights_out = weights
     ld = 0
     if weights_out is not None:
-        _attended(weights_out, cache, "weights_out")
-        ld = weights_out.shape[2]
-        if weights is not None:
-            _attended(weights, cache, "weights")
-            if weights.shape[2] != ld:
-                raise ValueError("weights and weights_out must share one shape")
+        ld = _attended(weights_out, sizes, sizes[4], "weights_out")
+        if weights is not None and _attended(weights, sizes, sizes[4], "weights") != ld:
+            raise ValueError("weights and weights_out must share one shape")
     lib = _lib.lib()
-    need = lib.ptj_attn_decode_workspace_bytes(ctypes.byref(cache), ctypes.byref(new), int(weights_out is not None))
-    if need and workspace is None:
-        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
-    _lib.check(lib.ptj_attn_decode(ctypes.byref(cache), ctypes.byref(new), DROPOUT_RATE if p is None else p, _ptr(weights),
-                                   _ptr(weights_out), ld, _ptr(workspace),
-                                   0 if workspace is None else workspace.numel() * workspace.element_size(), _stream()),
-               "ptj_attn_decode")
+    if workspace is None:
+        key = (sizes, H, T, ld > 0, q.dtype)
+        need = _DECODE_BYTES.get(key)
+        if need is None:
+            if len(_DECODE_BYTES) > 4096:
+                _DECODE_BYTES.clear()
+            need = _DECODE_BYTES[key] = lib.ptj_attn_decode_workspace_bytes(cache, new, int(ld > 0))
+        if need:
+            workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+    rc = lib.ptj_attn_decode(cache, new, DROPOUT_RATE if p is None else p, _ptr(weights), _ptr(weights_out), ld,
+                             _ptr(workspace), 0 if workspace is None else workspace.nbytes, _stream())
+    if rc != 0:
+        _lib.check(rc, "ptj_attn_decode")
     return out
 
 
@@ -632,36 +659,42 @@ def kv_evict(k_pages, v_pages, page_table, lengths, weights, budget, recent=0, *
     int32 [B]). The kept rows become rows 0 .. of the pages of dst_table (default: page_table, in place), which also get
     the sequences that are short enough; their weights become the first ones of weights_out (default: weights)."""
     _on_current_device(k_pages, v_pages, page_table, lengths, weights, dst_table, weights_out)
-    cache = _kv_cache(k_pages, v_pages, page_table, lengths)
-    _attended(weights, cache, "weights")
+    cache, sizes = _kv_cache(k_pages, v_pages, page_table, lengths)
+    B, Hk, _, page_size, capacity = sizes
+    ld = _attended(weights, sizes, capacity, "weights")
     budget, recent = int(budget), int(recent)
     if not 0 <= recent <= budget or budget < 1:
         raise ValueError("kv_evict needs 0 <= recent <= budget and budget >= 1")
-    most = min(budget, cache.table_width * cache.page_size)
+    most = min(budget, capacity)
     weights_out = weights if weights_out is None else weights_out
-    if weights_out.dtype != torch.float32 or weights_out.dim() != 3 or not weights_out.is_contiguous() or \
-            tuple(weights_out.shape[:2]) != (cache.batch, cache.kv_heads) or weights_out.shape[2] < most:
-        raise ValueError(f"weights_out must be a contiguous float32 tensor [{cache.batch}, {cache.kv_heads}, >= {most}]")
-    dst_table = page_table if dst_table is None else dst_table
-    if dst_table.dim() != 2 or dst_table.shape[1] * cache.page_size < most:
+    ld_out = ld if weights_out is weights else _attended(weights_out, sizes, most, "weights_out")
+    if dst_table is None:
+        dst_table = page_table
+    if dst_table.dim() != 2 or dst_table.shape[1] * page_size < most:
         raise ValueError(f"dst_table must list pages for {most} keys of each sequence")
-    _ints(dst_table, (cache.batch, dst_table.shape[1]), "dst_table")
-    kept = torch.empty((cache.batch, cache.kv_heads, budget), device=weights.device, dtype=torch.int32)
+    width = dst_table.shape[1]
+    _ints(dst_table, (B, width), "dst_table")
+    kept = torch.empty((B, Hk, budget), device=weights.device, dtype=torch.int32)
     new_lengths = torch.empty_like(lengths)
-    if cache.batch == 0:
+    if B == 0:
         return kept, new_lengths
-    _lib.check(_lib.lib().ptj_kv_evict(ctypes.byref(cache), _ptr(dst_table), dst_table.shape[1],
-                                       dst_table.stride(0) if cache.batch > 1 else dst_table.shape[1], budget, recent, _ptr(weights),
-                                       weights.shape[2], _ptr(weights_out), weights_out.shape[2], _ptr(kept), _ptr(new_lengths),
-                                       _stream()), "ptj_kv_evict")
+    rc = _lib.lib().ptj_kv_evict(cache, dst_table.data_ptr(), width, dst_table.stride(0) if B > 1 else width, budget, recent,
+                                 weights.data_ptr(), ld, weights_out.data_ptr(), ld_out, kept.data_ptr(), new_lengths.data_ptr(),
+                                 _stream())
+    if rc != 0:
+        _lib.check(rc, "ptj_kv_evict")
     return kept, new_lengths
 
 
 # ---- drafted tokens -----------------------------------------------------------------------------------------------------
+_TWO_STRIDES = struct.Struct("=2q")
+
+
 def _rows_of(probs, name, shape, dtype):
-    if probs.dtype != dtype or tuple(probs.shape) != shape or (shape[2] > 1 and probs.stride(2) != 1):
+    s0, s1, s2 = probs.stride()
+    if probs.dtype != dtype or probs.shape != shape or (shape[2] > 1 and s2 != 1):
         raise ValueError(f"{name} must be a {dtype} tensor {list(shape)} with contiguous rows")
-    return (ctypes.c_int64 * 2)(probs.stride(0), probs.stride(1))
+    return _TWO_STRIDES.pack(s0, s1)
 
 
 def verify_drafts(target_probs, draft_tokens, uniforms, draft_probs=None, counts=None):
@@ -678,23 +711,25 @@ def verify_drafts(target_probs, draft_tokens, uniforms, draft_probs=None, counts
         raise ValueError("target_probs must be [batch, drafts + 1, vocab]")
     B, K, V = target_probs.shape
     K -= 1
-    ts = _rows_of(target_probs, "target_probs", (B, K + 1, V), target_probs.dtype)
-    ds = None if draft_probs is None else _rows_of(draft_probs, "draft_probs", (B, K, V), target_probs.dtype)
-    if draft_tokens.dtype != torch.int32 or tuple(draft_tokens.shape) != (B, K):
+    dtype = target_probs.dtype
+    ts = _rows_of(target_probs, "target_probs", (B, K + 1, V), dtype)
+    ds = None if draft_probs is None else _rows_of(draft_probs, "draft_probs", (B, K, V), dtype)
+    if draft_tokens.dtype != torch.int32 or draft_tokens.shape != (B, K):
         raise ValueError(f"draft_tokens must be an int32 tensor of shape [{B}, {K}]")
-    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != (B, K + 1):
+    if uniforms.dtype != torch.float32 or uniforms.shape != (B, K + 1):
         raise ValueError(f"uniforms must be a float32 tensor of shape [{B}, {K + 1}]")
     if counts is not None:
-        counts = _ints(counts, (B,), "counts").contiguous()
+        _ints(counts, (B,), "counts")
     draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
     tokens = torch.empty((B, K + 1), device=target_probs.device, dtype=torch.int32)
     accepted = torch.empty(B, device=target_probs.device, dtype=torch.int32)
     if B == 0:
         return tokens, accepted
-    _lib.check(_lib.lib().ptj_verify_drafts(_ptr(target_probs), ctypes.byref(ts), _ptr(draft_probs),
-                                            None if ds is None else ctypes.byref(ds), _ptr(draft_tokens), _ptr(counts),
-                                            _ptr(uniforms), _ptr(tokens), _ptr(accepted), B, K, V, _dt(target_probs),
-                                            _stream()), "ptj_verify_drafts")
+    rc = _lib.lib().ptj_verify_drafts(target_probs.data_ptr(), ts, _ptr(draft_probs), ds, draft_tokens.data_ptr(), _ptr(counts),
+                                      uniforms.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), B, K, V, _dt(target_probs),
+                                      _stream())
+    if rc != 0:
+        _lib.check(rc, "ptj_verify_drafts")
     return tokens, accepted
 
 
