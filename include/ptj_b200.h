@@ -402,7 +402,7 @@ int ptj_decode(const float* w_emb, const float* b_head, const float* w_pos, cons
  *
  * One layer's cache: pools of pages [pages, kv_heads, page_size, d_head] (element strides page, head, slot; d_head contiguous)
  * and a page table. Key j of sequence b lies in slot j % page_size of page table[b * table_ld + j / page_size]. lengths[b]
- * counts the sequence's keys, the new tokens of the call among them. Table entries behind the last key are not read.
+ * counts the sequence's keys, the new tokens of the call among them. Table entries behind the last key are not used.
  * The tables and lengths live on the device, where the host cannot check them: a page outside [0, pages) is skipped (its keys
  * count as absent, nothing is written to it) and ptj_last_kernel_fault reports 0x3201; a length outside
  * [0, table_width * page_size] or a count outside [0, tokens] is brought to the nearer bound and reported as 0x3202.

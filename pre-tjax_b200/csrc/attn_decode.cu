@@ -6,9 +6,7 @@ namespace ptj {
 namespace {
 
 constexpr int kMaxRows = 4096;      // query rows of a key head
-constexpr int kDirectKeys = 256;    // a block per segment takes caches up to this length whatever their number
-constexpr int kDirectLong = 2048;   // ... and up to this one where there are no more segments than SMs
-constexpr int kLeastKeys = 64;      // keys that a warp of the list takes at least
+constexpr int kLeastKeys = 64;      // keys that a stretch of the list has at least
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
@@ -23,7 +21,7 @@ DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const Paged
     const int most = pl.dim == 64 ? 32 : 24;
     pl.nrb = static_cast<int>(ceil_div(R, most));
     const int need = static_cast<int>(ceil_div(R, pl.nrb));
-    pl.rows = need <= 8 ? 8 : (need <= 16 ? 16 : most);
+    pl.rows = need <= 4 ? 4 : need <= 8 ? 8 : (need <= 16 ? 16 : most);
   } else {
     const int most = pl.dim == 256 ? 4 : 8;
     pl.nrb = static_cast<int>(ceil_div(R, most));
@@ -33,13 +31,27 @@ DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const Paged
   pl.nrb = static_cast<int>(ceil_div(R, pl.rows));
   pl.prows = R < pl.rows ? R : pl.rows;
   const int64_t segs = c.batch * c.kv_heads * pl.nrb;
-  pl.split = !(rows.capacity <= kDirectKeys || (segs <= kNumSMs && rows.capacity <= kDirectLong)) || (weights && pl.nrb > 1);
+  const int ks = tc ? 16 : 4096 / (pl.dim * pl.es);  // keys of a step
+  const int64_t longest = ceil_div(rows.capacity, ks);
+  // A cluster per segment, of as many blocks as all fit on the GPU at once and have a step for each of their warps (more come in
+  // a second round: 16 x 12 float32 caches of 512 keys 15.5 us with one block each, 22.3 with two; 8 x 12 bf16 caches of 1024 with
+  // 1, 2, 4, 8 blocks: 15.6, 12.9, 10.8, 16.0). The list of stretches takes over where that could leave a warp more than 64 steps,
+  // or more than 16 with SMs idle.
+  const int per_sm = tc ? decode_tc_blocks(pl.dim, pl.rows) : decode_fma_blocks();
+  pl.cluster = 1;
+  while (pl.cluster < 8 && segs * pl.cluster * 2 <= per_sm * kNumSMs && longest > kDecWarps * pl.cluster) pl.cluster *= 2;
+  const int64_t most = ceil_div(longest, kDecWarps * pl.cluster);  // steps of a warp
+  pl.split = most > 64 || (most > 16 && segs * pl.cluster < kNumSMs) || (weights && pl.nrb > 1);
   if (pl.split) {
-    pl.workers = (tc ? decode_tc_blocks(pl.dim, pl.rows) : decode_fma_blocks(pl.dim, pl.rows, pl.es)) * kNumSMs * kDecSplitWarps;
-    pl.part = static_cast<size_t>(pl.workers) * 2 * pl.prows * pl.dim * 4;
-    pl.part_ml = round16(static_cast<size_t>(pl.workers) * 2 * pl.prows * 8);
+    pl.workers = per_sm * kNumSMs * kDecWarps;
+    // small stretches: where sequences may be long enough for 32 steps of a warp, and pieces of a few rows are small beside them
+    const int64_t steps = segs * longest;
+    pl.small = c.batch <= kDecDynamicBatch && pl.prows <= 8 && steps >= 32ll * pl.workers ? pl.workers : 0;
+    const size_t pieces = static_cast<size_t>(pl.workers + pl.small) * 2 * pl.prows;
+    pl.part = pieces * pl.dim * 4;
+    pl.part_ml = round16(pieces * 8);
     if (weights) pl.ml = round16(static_cast<size_t>(segs) * pl.prows * 8);
-    pl.starts = round16(static_cast<size_t>(c.batch + 1) * 8);
+    pl.starts = round16(static_cast<size_t>(c.batch + 2) * 8 + 16);
   }
   if (weights) pl.scores = static_cast<size_t>(c.batch * c.kv_heads * R) * rows.capacity * 4;
   return pl;
@@ -96,12 +108,14 @@ extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* 
   d.part_ml = reinterpret_cast<float*>(ws + pl.part);
   d.ml = reinterpret_cast<float*>(ws + pl.part + pl.part_ml);
   d.starts = reinterpret_cast<int64_t*>(ws + pl.part + pl.part_ml + pl.ml);
+  d.next = reinterpret_cast<unsigned int*>(d.starts + cache->batch + 2);
   d.scores = weights_out == nullptr ? nullptr : reinterpret_cast<float*>(ws + pl.part + pl.part_ml + pl.ml + pl.starts);
   d.scores_ld = d.rows.capacity;
   d.weights = weights;
   d.weights_out = weights_out;
   d.weights_ld = weights_ld;
   d.scale = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(cache->d_head)));
+  d.unscale = 1.f / d.scale;
   d.keep = 1.f - p;
   d.B = static_cast<int>(cache->batch);
   d.Hk = static_cast<int>(Hk);
@@ -112,6 +126,7 @@ extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* 
   d.nrb = pl.nrb;
   d.prows = pl.prows;
   d.workers = pl.workers;
+  d.small = pl.small;
   const bool tc = cache->dtype == PTJ_BF16 && cache->d_head <= 128;
   d.least = kLeastKeys / (tc ? 16 : 4096 / (pl.dim * pl.es));
   d.wide = paged_rows_aligned(*cache);

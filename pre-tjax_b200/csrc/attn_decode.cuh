@@ -6,23 +6,28 @@
 //
 // The keys of a segment (sequence, key head, block of rows) are taken in steps of KS = 4 to 16. Two ways to share them out:
 //
-// * One block per segment, its 8 or 16 warps taking steps in turn and joining their sums in shared memory: one launch, no second
-//   pass, for short caches and for few segments.
-// * All steps of the call form one list in which lengths, known on the device only, no longer matter, and every warp of the GPU
-//   takes an equal stretch of it. A warp that holds all steps of a segment writes its output; pieces of a segment (at most two
-//   per warp) go to the workspace with their reference exponent and sum and are joined, in order, by a second kernel.
+// * A cluster of one to eight blocks per segment, their warps taking steps in turn and joining their sums in shared memory: one launch
+//   and no second pass, unless there are too few segments to fill the GPU that way or sequences are so long that one of them
+//   alone could keep its cluster busy long after the others.
+// * All steps of the call form one list in which lengths, known on the device only, no longer matter. Every warp of the GPU takes
+//   an equal large stretch, three quarters of the list, and then small ones as long as there are some: some SMs get a third less
+//   of the memory's rate than others (with equal stretches alone the average SM was busy for 157 k cycles, the last for 207 k:
+//   128k keys of 8 heads of 128). A segment within one stretch is written by its warp; pieces of others (at most two per stretch)
+//   go to the workspace with their reference exponent and sum and are joined, in order, by a second kernel.
 //
-// Results do not depend on timing. A warp owns a ring of steps in shared memory that cp.async fills ahead of the arithmetic, across
+// Who computes a stretch does not matter to it: results do not depend on timing. A warp owns a ring of steps in shared memory that cp.async fills ahead of the arithmetic, across
 // segments; nothing but the warp itself waits for it. Sums are kept relative to a reference exponent that only moves when a
 // score outgrows it by more than 2^8, so that a step costs one vote instead of a reduction over lanes.
 #pragma once
+#include "cluster.cuh"
 #include "kv_cache.cuh"
 
 namespace ptj {
 
 constexpr int kDecJoinThreads = 256;
 constexpr float kDecLazy = 8.f;
-constexpr int kDecSplitWarps = 4;
+constexpr int kDecWarps = 4;
+constexpr int kDecDynamicBatch = 512;  // small stretches are cut where this many sequences' places fit into shared memory
 
 struct DecodeAttn {
   PagedRows rows;
@@ -33,14 +38,15 @@ struct DecodeAttn {
   const float* weights;
   float* weights_out;
   int64_t weights_ld, scores_ld;
-  float *part, *part_ml;     // pieces: [warps][2][prows][kDim], [..][2] reference exponent and sum
-  float* ml;                 // [segments][prows][2] of segments that one warp did
-  int64_t* starts;           // [B + 1]: place of each sequence's first step in the list; steps of a warp's stretch
+  float *part, *part_ml;     // pieces: [stretches][2][prows][kDim], [..][2] reference exponent and sum
+  float* ml;                 // [segments][prows][2] of segments that lie in one stretch
+  int64_t* starts;           // [B + 2]: place of each sequence's first step in the list; steps of a large and of a small stretch
   float* scores;             // [batch * key heads][R][scores_ld], log2 units; NULL without weights
-  float scale, keep;         // log2(e) / sqrt(d); 1 - p
+  float scale, unscale, keep;  // log2(e) / sqrt(d), its reciprocal; 1 - p
   int B, Hk, G, T, D, R;
   int nrb, prows;            // blocks of rows, rows of a block that exist
-  int workers, least;        // warps that share the list; steps that one takes at least
+  unsigned int* next;        // the next of the small stretches to be taken (zero at the start)
+  int workers, small, least; // warps that share the list; number of small stretches at most; steps of a stretch at least
   int wide, q_wide, out_wide;  // 16-byte accesses are aligned: pools and new rows, queries, output
 };
 
@@ -48,13 +54,14 @@ struct DecodePlan {
   int rows, dim, es;   // of a core: block rows, padded head, bytes of an element
   int nrb, prows;
   bool split;
-  int workers;
+  int cluster;         // blocks per segment
+  int workers, small;
   size_t part, part_ml, ml, starts, scores;  // bytes
   size_t bytes() const { return part + part_ml + ml + starts + scores; }
 };
-// workers of the split form and keys of a step of the core that takes these (0: there is none)
+// blocks that an SM holds of the core that takes these
 int decode_tc_blocks(int dim, int rows);
-int decode_fma_blocks(int dim, int rows, int es);
+int decode_fma_blocks();
 int launch_decode_tc(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st);
 int launch_decode_fma(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st);
 
@@ -65,9 +72,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float base_of(float ref) { return ref == -INFINITY ? 0.f : ref; }
-// factor of sums relative to `ref` when they are taken relative to m; sums without any score above -inf are zero (or NaN)
-__device__ __forceinline__ float rebase(float ref, float m) { return ref == -INFINITY ? 1.f : ex2(ref - m); }
+// Reference exponent before any score above -inf: exponentials of -inf relative to it are zero, and so are such sums.
+constexpr float kNoRef = -3.402823466e38f;
+// factor of sums relative to `ref` when they are taken relative to m
+__device__ __forceinline__ float rebase(float ref, float m) { return ex2(ref - m); }
 
 // What a warp works on: one sequence, key head and block of rows
 struct Segment {
@@ -77,8 +85,7 @@ struct Segment {
   const int32_t* table;
   __device__ __forceinline__ void set_sequence(const DecodeAttn& p, int seq) {
     b = seq;
-    n = p.rows.length(p.lengths, b);
-    count = p.rows.count(p.counts, p.T, b);
+    p.rows.extent(p.lengths, p.counts, p.T, b, n, count);
     first = n - count;
     table = p.rows.table + b * p.rows.table_ld;
   }
@@ -99,9 +106,14 @@ struct Segment {
   }
 };
 
-// n: 16, or 0 to fill the destination with zeros (nothing is read then)
-__device__ __forceinline__ void copy16(uint32_t dst, const char* src, int n) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// on false: the destination is filled with zeros and nothing is read. (A byte count instead of the predicate takes several
+// instructions where it is not a constant.)
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const char* src, bool on) {
+  asm volatile("{\n\t.reg .pred off;\n\tsetp.eq.u32 off, %2, 0;\n\tcp.async.cg.shared.global [%0], [%1], 16, off;\n\t}"
+               ::"r"(dst), "l"(src), "r"(static_cast<uint32_t>(on)) : "memory");
 }
 
 // Place of 16-byte piece c of row r of a step: c ^ swizzle(r). Pieces are swapped so that both ways the tensor-core fragments read a
@@ -115,109 +127,166 @@ template <int KS, int RB>
 __device__ __forceinline__ uint32_t present_keys(const uint8_t* stage) { return *reinterpret_cast<const uint32_t*>(stage + 2 * KS * RB); }
 
 // Copies steps: KS rows of keys, KS rows of values, of RB bytes each, and a word that says which of them exist. Rows the table does
-// not place and keys behind the last one become zeros. New rows are taken from where they are and put into their pages.
+// not place and keys behind the last one become zeros. New rows are taken from where they are; store_new puts them into their
+// pages. Short calls are bound by instruction fetches as much as by anything else: one inlined copy of the common case per kernel,
+// everything else out of line.
 template <int KS, int RB>
 struct Fetcher {
   static constexpr int PIECES = RB / 16, ROWS = PIECES >= 32 ? 1 : 32 / PIECES, COLS = PIECES >= 32 ? PIECES / 32 : 1;
-  int row0, c0;      // this lane's first row and piece
-  uint32_t to;       // its place in a step
-  bool paged, dense; // a step lies in one page; its rows lie one behind the other
+  int row0, c0;   // this lane's first row and piece
+  uint32_t to;    // its place in a step
+  bool dense;     // a step's rows lie one behind the other in one page
+  // Pages of 32 steps to come, one per lane: a look-up in front of every step would be the longest wait of all (800 cycles).
+  int ids, base;  // base: the first of them, counted in steps that this warp takes
+  const char *k, *v;  // this lane's place in slot 0 of page 0 of the key head
+  __device__ __forceinline__ void look_up(const DecodeAttn& p, const int32_t* table, int sub, int stride, int number) {
+    const int page = p.rows.page_of((sub + (threadIdx.x & 31) * stride) * KS);
+    ids = page < p.rows.capacity_pages ? table[page] : -1;
+    base = number;
+  }
   __device__ __forceinline__ void init(const DecodeAttn& p) {
     const int lane = threadIdx.x & 31;
     row0 = PIECES >= 32 ? 0 : lane / PIECES;
     c0 = PIECES >= 32 ? lane : lane % PIECES;
     to = row0 * RB + ((c0 ^ swizzle(row0)) << 4);
-    paged = p.wide && p.rows.page_size % KS == 0;
-    dense = p.rows.slot_stride[0] == RB && p.rows.slot_stride[1] == RB;
+    dense = p.wide && p.rows.page_size % KS == 0 && p.rows.slot_stride[0] == RB && p.rows.slot_stride[1] == RB;
   }
-  // sub: number of the step in its sequence
-  __device__ __forceinline__ void fetch(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage) const {
+  __device__ __forceinline__ void set_head(const DecodeAttn& p, int h) {
+    k = p.k + p.rows.offset(0, 0, h, 0) + (row0 * RB + c0 * 16);
+    v = p.v + p.rows.offset(1, 0, h, 0) + (row0 * RB + c0 * 16);
+  }
+  // Number of a sequence's first steps that are dense and hold no new key.
+  __device__ __forceinline__ int plain_steps(const Segment& sg) const { return dense ? max(sg.first, 0) / KS : 0; }
+  // A plain step. sub: its number in its sequence; number: how many this warp took before it, of those that look_up covers.
+  // false: its page does not exist, the general way has to take it.
+  __device__ __forceinline__ bool plain(const DecodeAttn& p, int sub, int number, uint8_t* stage) const {
+    const int page = __shfl_sync(0xffffffffu, ids, number - base);
+    if (static_cast<unsigned int>(page) >= static_cast<unsigned int>(p.rows.pages)) return false;
     const int j0 = sub * KS;
-    if (!paged || j0 + KS > sg.first) {
-      mixed(p, sg, j0, stage);
-      return;
-    }
-    int64_t page;
-    int slot;
-    const bool on = p.rows.locate(sg.table, j0, page, slot);
-    if ((threadIdx.x & 31) == 0) *present_word<KS, RB>(stage) = on ? (1u << KS) - 1u : 0u;
-    if (!on) page = slot = 0;  // (nothing is read)
-    const char* k = p.k + p.rows.offset(0, page, sg.h, slot);
-    const char* v = p.v + p.rows.offset(1, page, sg.h, slot);
-    if (dense) rows<true>(p, k + (row0 * RB + c0 * 16), v + (row0 * RB + c0 * 16), on, tc::smem_u32(stage));
-    else rows<false>(p, k + row0 * p.rows.slot_stride[0] + c0 * 16, v + row0 * p.rows.slot_stride[1] + c0 * 16, on, tc::smem_u32(stage));
-  }
-  template <bool DENSE>
-  __device__ __forceinline__ void rows(const DecodeAttn& p, const char* k, const char* v, bool on, uint32_t stage) const {
-    const int64_t ks = ROWS * p.rows.slot_stride[0], vs = ROWS * p.rows.slot_stride[1];
+    const int slot = p.rows.page_shift >= 0 ? j0 & (p.rows.page_size - 1) : j0 - p.rows.page_of(j0) * p.rows.page_size;
+    if ((threadIdx.x & 31) == 0) *present_word<KS, RB>(stage) = (1u << KS) - 1u;
+    const char *kr = k + (page * p.rows.page_stride[0] + slot * RB), *vr = v + (page * p.rows.page_stride[1] + slot * RB);
+    const uint32_t at = tc::smem_u32(stage);
 #pragma unroll
     for (int x = 0; x < COLS; ++x) {
-      const int n = on && (c0 + 32 * x) * 16 < p.rows.row_bytes ? 16 : 0;
-      const char *kr = k + 512 * x, *vr = v + 512 * x;
+      if ((c0 + 32 * x) * 16 >= p.rows.row_bytes) continue;  // (zero from the start)
 #pragma unroll
       for (int i = 0; i < KS; i += ROWS) {
-        const uint32_t dst = stage + ((to ^ (swizzle(i) << 4)) + i * RB + 512 * x);
-        copy16(dst, DENSE ? kr + i * RB : kr, n);
-        copy16(dst + KS * RB, DENSE ? vr + i * RB : vr, n);
-        if (!DENSE) {
-          kr += ks;
-          vr += vs;
-        }
+        const uint32_t dst = at + ((to ^ (swizzle(i) << 4)) + i * RB + 512 * x);
+        copy16(dst, kr + i * RB + 512 * x);
+        copy16(dst + KS * RB, vr + i * RB + 512 * x);
+      }
+    }
+    return true;
+  }
+  __device__ __forceinline__ void general(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage) const {
+    if (p.wide) mixed(p, sg, sub * KS, stage);
+    else narrow(p, sg, sub * KS, stage);
+  }
+  // What lies behind narrower rows in a ring is zero: dense steps write their rows only.
+  __device__ __forceinline__ void clear(const DecodeAttn& p, uint8_t* ring, int bytes) const {
+    if (p.rows.row_bytes == RB) return;
+    for (int i = (threadIdx.x & 31) * 16; i < bytes; i += 512) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+  }
+  // Rows here and there: lane r looks row r up, the others get its addresses from it. (Arguments by value: nothing of the caller's
+  // is forced into memory.)
+  static __device__ __noinline__ void mixed(const DecodeAttn& p, const Segment sg, int j0, uint8_t* stage) {
+    const int lane = threadIdx.x & 31, row0 = PIECES >= 32 ? 0 : lane / PIECES, c0 = PIECES >= 32 ? lane : lane % PIECES;
+    const int j = j0 + lane;
+    int64_t page = 0;
+    int slot = 0;
+    const bool on = lane < KS && j < sg.n && p.rows.locate(sg.table, j, page, slot);
+    const char *k = p.k, *v = p.v;
+    if (on) {
+      if (j >= sg.first && p.kn != nullptr) {
+        k = p.kn + sg.b * p.kns[0] + sg.h * p.kns[1] + (j - sg.first) * p.kns[2];
+        v = p.vn + sg.b * p.vns[0] + sg.h * p.vns[1] + (j - sg.first) * p.vns[2];
+      } else {
+        k += p.rows.offset(0, page, sg.h, slot);
+        v += p.rows.offset(1, page, sg.h, slot);
+      }
+    }
+    const uint32_t present = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) *present_word<KS, RB>(stage) = present;
+    const uint32_t at = tc::smem_u32(stage) + row0 * RB;
+#pragma unroll
+    for (int i = 0; i < KS; i += ROWS) {
+      const int r = i + row0;
+      const char* kr = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k), r));
+      const char* vr = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), r));
+#pragma unroll
+      for (int x = 0; x < COLS; ++x) {
+        const int c = c0 + 32 * x;
+        const bool there = (present >> r & 1u) && c * 16 < p.rows.row_bytes;
+        const uint32_t dst = at + i * RB + ((c ^ swizzle(r)) << 4);
+        copy16_or_zero(dst, kr + c * 16, there);
+        copy16_or_zero(dst + KS * RB, vr + c * 16, there);
       }
     }
   }
-  // a step that is not all in one page, or holds new keys or the last one (arguments by value: nothing of the caller's is
-  // forced into memory)
-  static __device__ __noinline__ void mixed(const DecodeAttn& p, const Segment sg, int j0, uint8_t* stage) {
-    const int lane = threadIdx.x & 31, row0 = PIECES >= 32 ? 0 : lane / PIECES, c0 = PIECES >= 32 ? lane : lane % PIECES;
+  // Rows that are not on 16-byte boundaries: by 2 bytes (elements are whole numbers of them), nothing asynchronous.
+  static __device__ __noinline__ void narrow(const DecodeAttn& p, const Segment sg, int j0, uint8_t* stage) {
+    const int lane = threadIdx.x & 31;
     uint32_t present = 0;
-#pragma unroll 1
-    for (int i = 0; i < KS; i += ROWS) {
-      const int r = i + row0, j = j0 + r;
+    for (int r = 0; r < KS; ++r) {
+      const int j = j0 + r;
       int64_t page = 0;
       int slot = 0;
       const bool on = j < sg.n && p.rows.locate(sg.table, j, page, slot);
-      const bool fresh = on && j >= sg.first && p.kn != nullptr;
-      const unsigned lanes = __ballot_sync(0xffffffffu, on);
-#pragma unroll
-      for (int k = 0; k < ROWS; ++k) present |= (lanes >> (k * (PIECES >= 32 ? 0 : PIECES)) & 1u) << (i + k);
-      if (!on) page = slot = 0;
-#pragma unroll
+      if (on) present |= 1u << r;
       for (int kv = 0; kv < 2; ++kv) {
-        char* at = (kv == 0 ? p.k : p.v) + p.rows.offset(kv, page, sg.h, slot);
-        const int64_t* s = kv == 0 ? p.kns : p.vns;
-        const char* src = fresh ? (kv == 0 ? p.kn : p.vn) + sg.b * s[0] + sg.h * s[1] + (j - sg.first) * s[2] : at;
-#pragma unroll
-        for (int x = 0; x < COLS; ++x) {
-          const int c = c0 + 32 * x;
-          const int left = on ? p.rows.row_bytes - c * 16 : 0;  // bytes of the row from this piece on
-          uint8_t* dst = stage + (kv * KS + r) * RB + ((c ^ swizzle(r)) << 4);
-          if (p.wide) {
-            copy16(tc::smem_u32(dst), src + c * 16, left > 0 ? 16 : 0);
-            if (fresh && left > 0 && sg.rb == 0) *reinterpret_cast<uint4*>(at + c * 16) = *reinterpret_cast<const uint4*>(src + c * 16);
-          } else {  // rows that are not on 16-byte boundaries: by 2 bytes (elements are whole numbers of them)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint16_t val = 2 * e < left ? *reinterpret_cast<const uint16_t*>(src + c * 16 + 2 * e) : 0;
-              *reinterpret_cast<uint16_t*>(dst + 2 * e) = val;
-              if (fresh && 2 * e < left && sg.rb == 0) *reinterpret_cast<uint16_t*>(at + c * 16 + 2 * e) = val;
-            }
-          }
+        const char* src = nullptr;
+        if (on) {
+          const int64_t* s = kv == 0 ? p.kns : p.vns;
+          src = j >= sg.first && p.kn != nullptr ? (kv == 0 ? p.kn : p.vn) + sg.b * s[0] + sg.h * s[1] + (j - sg.first) * s[2]
+                                                 : (kv == 0 ? p.k : p.v) + p.rows.offset(kv, page, sg.h, slot);
+        }
+        for (int e = lane * 2; e < RB; e += 64) {
+          const uint16_t val = on && e < p.rows.row_bytes ? *reinterpret_cast<const uint16_t*>(src + e) : 0;
+          *reinterpret_cast<uint16_t*>(stage + (kv * KS + r) * RB + (((e >> 4) ^ swizzle(r)) << 4) + (e & 15)) = val;
         }
       }
     }
-    if ((threadIdx.x & 31) == 0) *present_word<KS, RB>(stage) = present;
+    if (lane == 0) *present_word<KS, RB>(stage) = present;
+  }
+  // Puts the new rows of a step that has arrived into their pages.
+  __device__ __forceinline__ void store_new(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) const {
+    if (p.kn != nullptr && sg.rb == 0 && (sub + 1) * KS > sg.first) write_new(p, sg, sub * KS, stage);
+  }
+  static __device__ __noinline__ void write_new(const DecodeAttn& p, const Segment sg, int j0, const uint8_t* stage) {
+    const int lane = threadIdx.x & 31, r0 = max(sg.first - j0, 0);
+    uint32_t rows = present_keys<KS, RB>(stage) >> r0 << r0;
+    int64_t page = 0;
+    int slot = 0;
+    if (lane < KS && (rows >> lane & 1u)) p.rows.locate(sg.table, j0 + lane, page, slot);  // lane r: row r
+    const unsigned long long at[2] = {reinterpret_cast<unsigned long long>(p.k + p.rows.offset(0, page, sg.h, slot)),
+                                      reinterpret_cast<unsigned long long>(p.v + p.rows.offset(1, page, sg.h, slot))};
+    for (; rows != 0u; rows &= rows - 1u) {
+      const int r = __ffs(rows) - 1;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, at[kv], r));
+        const uint8_t* row = stage + (kv * KS + r) * RB;
+        if (p.wide) {
+          for (int c = lane; c * 16 < p.rows.row_bytes; c += 32)
+            *reinterpret_cast<uint4*>(to + c * 16) = *reinterpret_cast<const uint4*>(row + ((c ^ swizzle(r)) << 4));
+        } else {
+          for (int e = lane * 2; e < p.rows.row_bytes; e += 64)
+            *reinterpret_cast<uint16_t*>(to + e) = *reinterpret_cast<const uint16_t*>(row + (((e >> 4) ^ swizzle(r)) << 4) + (e & 15));
+        }
+      }
+    }
   }
 };
 
 // Sum over the rows of a key of exp2(score - reference) / sum for keys [j0, j1) of a sequence's key head, onto the accumulated
 // weights. row_ml(r): reference exponent and reciprocal sum of row r.
-template <int N, typename F>
+template <int N, int U, typename F>
 __device__ __forceinline__ void add_weights(const DecodeAttn& p, const Segment& sg, int j0, int j1, F&& row_ml) {
   const int64_t bh = static_cast<int64_t>(sg.b) * p.Hk + sg.h;
   const float* in = p.weights == nullptr ? nullptr : p.weights + bh * p.weights_ld;
   float* out = p.weights_out + bh * p.weights_ld;
-  constexpr int U = 4;
   for (int jj = j0 + threadIdx.x; jj < j1; jj += N * U) {
     float w[U];
 #pragma unroll
@@ -228,12 +297,12 @@ __device__ __forceinline__ void add_weights(const DecodeAttn& p, const Segment& 
     for (int r = 0; r < p.R; ++r) {
       if (sg.limit(p, r) < 0) continue;
       const float2 ml = row_ml(r);
-      const float base = base_of(ml.x);
+      const float base = ml.x;
       const float* s = p.scores + (bh * p.R + r) * p.scores_ld;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int j = jj + u * N;
-        if (j < j1) w[u] = fmaf(ex2(s[j] - base), ml.y, w[u]);
+        if (j < j1) w[u] = fmaf(ex2(__ldcg(s + j) - base), ml.y, w[u]);  // (other blocks' writes: not from L1)
       }
     }
 #pragma unroll
@@ -269,45 +338,77 @@ constexpr int ring_bytes() { return Core::kDepth * stage_bytes<Core>(); }
 template <typename Core>
 __device__ __forceinline__ int steps_of(int n) { return (n + Core::KS - 1) / Core::KS; }
 
-// ---- a block per segment -------------------------------------------------------------------------------------------------
+// ---- a cluster of blocks per segment -----------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned cluster_blocks() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float4 peer_float4(const float* p, unsigned rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(tc::mapa_shared(tc::smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 peer_float2(const float* p, unsigned rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(tc::mapa_shared(tc::smem_u32(p), rank)) : "memory");
+  return v;
+}
+
 template <typename E, typename Core>
-__global__ void __launch_bounds__(Core::kDirectWarps * 32, 1)
+__global__ void __launch_bounds__(kDecWarps * 32, Core::kBlocks)
 attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
   grid_dep_sync();
-  constexpr int NW = Core::kDirectWarps, LD = Core::kDim + 4, D = Core::kDepth;
+  constexpr int NW = kDecWarps, LD = Core::kDim + 4, D = Core::kDepth;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float ml[NW][Core::kRows][2], fac[NW][Core::kRows], fin[Core::kRows][2];
+  __shared__ float ml[NW][Core::kRows][2], fac[NW][Core::kRows];
+  __shared__ __align__(8) float top_s[Core::kRows][2];  // of the block: reference exponent, sum
+  __shared__ float fin[Core::kRows][2];                 // of the cluster: reference exponent, reciprocal sum
+  __shared__ float peer_fac[8][Core::kRows];            // factors of the blocks' sums
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int hr = blockIdx.x % (p.Hk * p.nrb);
+  const unsigned C = cluster_blocks(), rank = tc::cluster_ctarank();
+  const int seg = blockIdx.x / C, hr = seg % (p.Hk * p.nrb), b = seg / (p.Hk * p.nrb);
+  const int stride = NW * static_cast<int>(C), s0 = static_cast<int>(rank) * NW + warp;
+  Fetcher<Core::KS, Core::kRowBytes> fetcher;
+  fetcher.look_up(p, p.rows.table + b * p.rows.table_ld, s0, stride, 0);  // (while the length is on its way)
   Segment sg;
-  sg.set_sequence(p, blockIdx.x / (p.Hk * p.nrb));
+  sg.set_sequence(p, b);
   sg.h = hr / p.nrb;
   sg.rb = hr % p.nrb;
   uint8_t* ring = smem + warp * ring_bytes<Core>();
   const int steps = steps_of<Core>(sg.n);
-  Fetcher<Core::KS, Core::kRowBytes> fetcher;
   fetcher.init(p);
-#pragma unroll 1
-  for (int i = 0; i < D - 1; ++i) {
-    if (warp + i * NW < steps) fetcher.fetch(p, sg, warp + i * NW, ring + i * stage_bytes<Core>());
-    cp_async_commit();
-  }
+  fetcher.set_head(p, sg.h);
+  fetcher.clear(p, ring, ring_bytes<Core>());
   Core core;
   core.init(p, sg);
-  int slot = 0, free_slot = D - 1;
-  for (int s = warp; s < steps; s += NW) {
-    cp_async_wait<D - 2>();
-    __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
-    const int ahead = s + (D - 1) * NW;
-    if (ahead < steps) fetcher.fetch(p, sg, ahead, ring + free_slot * stage_bytes<Core>());
+  const int plain = fetcher.plain_steps(sg);
+  int slot = 0, free_slot = 0, number = 0;
+#pragma unroll 1
+  for (int s = s0 - (D - 1) * stride; s < steps; s += stride) {  // (D - 1 rounds ahead: steps to come are fetched only)
+    if (s >= 0) {
+      cp_async_wait<D - 2>();
+      __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
+    }
+    const int ahead = s + (D - 1) * stride;
+    if (ahead < steps) {
+      if (number == fetcher.base + 32) fetcher.look_up(p, sg.table, ahead, stride, number);
+      uint8_t* stage = ring + free_slot * stage_bytes<Core>();
+      if (ahead >= plain || !fetcher.plain(p, ahead, number, stage)) fetcher.general(p, sg, ahead, stage);
+      ++number;
+    }
     cp_async_commit();
-    core.step(p, sg, s, ring + slot * stage_bytes<Core>());
-    slot = slot + 1 == D ? 0 : slot + 1;
     free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
+    if (s < 0) continue;
+    const uint8_t* stage = ring + slot * stage_bytes<Core>();
+    if (s >= plain) fetcher.store_new(p, sg, s, stage);
+    core.step(p, sg, s, stage);
+    slot = slot + 1 == D ? 0 : slot + 1;
   }
   cp_async_wait<0>();
   __syncthreads();
-  // the warps' sums over the rings
+  // the warps' sums over the rings, then the block's over the first warp's
   float* os = reinterpret_cast<float*>(smem);
   core.emit([&](int r, int d, const float4& x, float ref, float sum, bool first) {
     *reinterpret_cast<float4*>(os + (warp * Core::kRows + r) * LD + d) = x;
@@ -317,8 +418,9 @@ attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
     }
   });
   __syncthreads();
-  if (tid < Core::kRows) {
-    float m = -INFINITY, l = 0.f;
+  const int rows = min(Core::kRows, p.R - sg.rb * Core::kRows);
+  if (tid < rows) {
+    float m = kNoRef, l = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w][tid][0]);
 #pragma unroll
@@ -326,66 +428,152 @@ attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
       fac[w][tid] = rebase(ml[w][tid][0], m);
       l = fmaf(fac[w][tid], ml[w][tid][1], l);
     }
+    top_s[tid][0] = m;
+    top_s[tid][1] = l;
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * (Core::kDim / 4); i += NW * 32) {
+    const int r = i / (Core::kDim / 4), d = i % (Core::kDim / 4) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float4 y = *reinterpret_cast<const float4*>(os + (w * Core::kRows + r) * LD + d);
+      const float f = fac[w][r];
+      x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+    }
+    *reinterpret_cast<float4*>(os + r * LD + d) = x;
+  }
+  if (C > 1) tc::cluster_sync_all();
+  else __syncthreads();
+  // (all reads of other blocks are issued before any of them is waited for: one latency, not one per block)
+  if (tid < rows) {
+    float2 v[8];
+#pragma unroll
+    for (unsigned k = 0; k < 8; ++k) v[k] = k < C ? peer_float2(top_s[tid], k) : make_float2(kNoRef, 0.f);
+    float m = kNoRef, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, v[k].x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = rebase(v[k].x, m);
+      peer_fac[k][tid] = f;
+      l = fmaf(f, v[k].y, l);
+    }
     fin[tid][0] = m;
     fin[tid][1] = 1.f / l;
   }
-  __syncthreads();
-  const int rows = min(Core::kRows, p.R - sg.rb * Core::kRows);
-  for (int i = tid; i < rows * (Core::kDim / 4); i += NW * 32) {
-    const int r = i / (Core::kDim / 4), d = i % (Core::kDim / 4) * 4, row = sg.rb * Core::kRows + r;
-    if (d >= p.D) continue;
+  // every block joins its share of the rows' elements
+  const int pieces = rows * (Core::kDim / 4);
+  for (int i0 = static_cast<int>(rank) * NW * 32; i0 < pieces; i0 += NW * 32 * static_cast<int>(C)) {
+    const int i = i0 + tid, r = i / (Core::kDim / 4), d = i % (Core::kDim / 4) * 4, row = sg.rb * Core::kRows + r;
+    const bool on = i < pieces && d < p.D;
+    float4 y[8];
+#pragma unroll
+    for (unsigned k = 0; k < 8; ++k) y[k] = on && k < C ? peer_float4(os + r * LD + d, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i0 == static_cast<int>(rank) * NW * 32) __syncthreads();  // the factors (the first round is every thread's)
+    if (!on) continue;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (sg.limit(p, row) >= 0) {
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float4 y = *reinterpret_cast<const float4*>(os + (w * Core::kRows + r) * LD + d);
-        const float f = fac[w][r];
-        x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+      for (int k = 0; k < 8; ++k) {
+        const float f = k < static_cast<int>(C) ? peer_fac[k][r] : 0.f;
+        x.x = fmaf(f, y[k].x, x.x); x.y = fmaf(f, y[k].y, x.y); x.z = fmaf(f, y[k].z, x.z); x.w = fmaf(f, y[k].w, x.w);
       }
       x = scaled(x, p.keep * fin[r][1]);
     }
     store_out<E>(p, sg, row, d, x);
   }
-  if (p.scores != nullptr)  // (one block of rows: the host sees to it; the scores are this block's)
-    add_weights<NW * 32>(p, sg, 0, sg.n, [&](int r) { return make_float2(fin[r][0], fin[r][1]); });
+  __syncthreads();
+  if (p.scores != nullptr) {  // (one block of rows: the host sees to it; the scores are this cluster's)
+    const int per = (sg.n + static_cast<int>(C) - 1) / static_cast<int>(C), j0 = min(static_cast<int>(rank) * per, sg.n);
+    add_weights<NW * 32, 4>(p, sg, j0, min(j0 + per, sg.n), [&](int r) { return make_float2(fin[r][0], fin[r][1]); });
+  }
+  if (C > 1) tc::cluster_sync_all();  // nobody leaves before its sums are read
 }
 
-// ---- an equal stretch of the list per warp ----------------------------------------------------------------------------------
+// ---- stretches of the list ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {  // (32 bits where they do: a tenth of the time)
   return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
 }
-__device__ __forceinline__ int64_t steps_per_worker(const DecodeAttn& p, int64_t total) {
-  const int64_t q = divide(total * p.Hk * p.nrb + p.workers - 1, p.workers);
-  return q > p.least ? q : p.least;
-}
+// The list of `all` steps: `workers` large stretches of q1 steps, then small ones of q2.
+struct Stretches {
+  int64_t q1, q2, edge;
+  int workers;
+  __device__ __forceinline__ void plan(const DecodeAttn& p, int64_t all) {
+    workers = p.workers;
+    const int64_t share = divide(all, workers);
+    q1 = p.small > 0 ? share - (share >> 2) : share + (share * workers < all);
+    if (q1 < p.least) q1 = p.least;
+    edge = q1 * workers;
+    q2 = 1;
+    if (p.small > 0) {
+      const int64_t rest = all > edge ? all - edge : 0;
+      q2 = divide(rest + p.small - 1, p.small);
+      if (q2 < p.least) q2 = p.least;
+    }
+  }
+  __device__ __forceinline__ void load(const DecodeAttn& p) {
+    workers = p.workers;
+    q1 = p.starts[p.B];
+    q2 = p.starts[p.B + 1];
+    edge = q1 * workers;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t w) const { return w < workers ? w * q1 : edge + (w - workers) * q2; }
+  __device__ __forceinline__ int64_t of(int64_t t) const { return t < edge ? divide(t, q1) : workers + divide(t - edge, q2); }
+};
 
-// A place in the list: the segment and the step in it; `left` steps of the stretch from here on.
+// A place in the list: the segment, the step in it, where this stretch leaves it, and the steps of the stretch behind that.
 template <typename Core>
 struct Cursor {
   Segment sg;
-  int s, steps, left;
-  // one step on; false: the stretch ends. `last` says that the step left was its segment's last in the stretch.
-  __device__ __forceinline__ bool segment_ends() const { return s + 1 == steps || left == 1; }
-  __device__ __forceinline__ void advance(const DecodeAttn& p) {
-    --left;
-    if (++s < steps || left == 0) return;
+  int s, end, steps, left;
+  __device__ __forceinline__ void bound(int n) {  // n steps of the stretch from here on
+    end = min(steps, s + n);
+    left = n - (end - s);
+  }
+  // to the stretch's next segment (left > 0)
+  __device__ __forceinline__ void next_segment(const DecodeAttn& p) {
     s = 0;
-    if (++sg.rb < p.nrb) return;
-    sg.rb = 0;
-    if (++sg.h < p.Hk) return;
-    sg.h = 0;
-    do sg.set_sequence(p, sg.b + 1); while (sg.n == 0);  // (steps are left: a sequence that has some follows)
+    if (++sg.rb == p.nrb) {
+      sg.rb = 0;
+      if (++sg.h == p.Hk) {
+        sg.h = 0;
+        do sg.set_sequence(p, sg.b + 1); while (sg.n == 0);  // (steps are left: a sequence that has some follows)
+        steps = steps_of<Core>(sg.n);
+      }
+    }
+    bound(left);
+  }
+  // place `at` of the list, which lies in sequence b whose first step is at place `start`; n steps from there on
+  __device__ __forceinline__ void set(const DecodeAttn& p, int b, int64_t start, int64_t at, int64_t n) {
+    sg.set_sequence(p, b);
     steps = steps_of<Core>(sg.n);
+    const int64_t hr = divide(at - start, steps);
+    s = static_cast<int>(at - start - hr * steps);
+    sg.h = static_cast<int>(hr) / p.nrb;
+    sg.rb = static_cast<int>(hr) - sg.h * p.nrb;
+    bound(static_cast<int>(n));
   }
 };
 
+// the last sequence that starts at or before a place (empty ones start where the next does)
+__device__ __forceinline__ int sequence_at(const int64_t* first, int n, int64_t at) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first[mid] <= at) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
 template <typename E, typename Core>
-__global__ void __launch_bounds__(kDecSplitWarps * 32, Core::kBlocks)
+__global__ void __launch_bounds__(kDecWarps * 32, Core::kBlocks)
 attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
   grid_dep_sync();
-  constexpr int NW = kDecSplitWarps, N = NW * 32, D = Core::kDepth;
+  constexpr int NW = kDecWarps, N = NW * 32, D = Core::kDepth;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t tot[NW], start_s[NW][2];
+  __shared__ int64_t tot[NW], start_s[NW], first_s[kDecDynamicBatch];
+  __shared__ int seq_s[NW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // steps of all sequences, and of those before each thread's stretch of sequences
   const int per = (p.B + N - 1) / N, b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
@@ -406,69 +594,108 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
     total += tot[w];
   }
   const int64_t heads = static_cast<int64_t>(p.Hk) * p.nrb, all = total * heads;
-  const int64_t q = steps_per_worker(p, total);
+  Stretches st;
+  st.plan(p, all);
   // the thread whose sequences hold the first step of a warp's stretch looks for its sequence
-  int64_t acc = before;
+  int64_t acc = before * heads;
   for (int b = b0; b < b1; ++b) {
-    const int64_t t = steps_of<Core>(p.rows.length(p.lengths, b));
-    if (blockIdx.x == 0) p.starts[b] = acc * heads;
+    const int64_t t = steps_of<Core>(p.rows.length(p.lengths, b)) * heads;
+    if (blockIdx.x == 0) p.starts[b] = acc;
+    if (p.small > 0) first_s[b] = acc;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const int64_t at = (static_cast<int64_t>(blockIdx.x) * NW + w) * q;
-      if (at >= acc * heads && at < (acc + t) * heads) {
-        start_s[w][0] = b;
-        start_s[w][1] = acc * heads;
+      const int64_t at = (static_cast<int64_t>(blockIdx.x) * NW + w) * st.q1;
+      if (at >= acc && at < acc + t) {
+        seq_s[w] = b;
+        start_s[w] = acc;
       }
     }
     acc += t;
   }
-  if (blockIdx.x == 0 && tid == 0) p.starts[p.B] = q;
+  if (blockIdx.x == 0 && tid == 0) {
+    p.starts[p.B] = st.q1;
+    p.starts[p.B + 1] = st.q2;
+  }
   __syncthreads();
-  const int64_t worker = static_cast<int64_t>(blockIdx.x) * NW + warp, range0 = worker * q;
+  int64_t stretch = static_cast<int64_t>(blockIdx.x) * NW + warp;
+  if (st.begin(stretch) >= all) return;
   Cursor<Core> cur;
-  cur.left = static_cast<int>(min(q, all - range0));
-  if (range0 >= all) return;
-  cur.sg.set_sequence(p, static_cast<int>(start_s[warp][0]));
-  cur.steps = steps_of<Core>(cur.sg.n);
-  const int64_t in_seq = range0 - start_s[warp][1], hr = divide(in_seq, cur.steps);
-  cur.s = static_cast<int>(in_seq - hr * cur.steps);
-  cur.sg.h = static_cast<int>(hr) / p.nrb;
-  cur.sg.rb = static_cast<int>(hr) - cur.sg.h * p.nrb;
+  cur.set(p, seq_s[warp], start_s[warp], st.begin(stretch), min(st.q1, all - st.begin(stretch)));
   uint8_t* ring = smem + warp * ring_bytes<Core>();
   Fetcher<Core::KS, Core::kRowBytes> fetcher;
   fetcher.init(p);
+  fetcher.clear(p, ring, ring_bytes<Core>());
   Cursor<Core> ahead = cur;
-#pragma unroll 1
-  for (int i = 0; i < D - 1; ++i) {
-    if (ahead.left > 0) {
-      fetcher.fetch(p, ahead.sg, ahead.s, ring + i * stage_bytes<Core>());
-      ahead.advance(p);
+  unsigned int ticket = 0;  // lane 0: the small stretch that was taken
+  int64_t following = -1;   // the stretch that `ahead` is in, when that is not `cur`'s
+  bool asked = p.small == 0, over = asked;
+  const int32_t* looked_up = nullptr;  // the sequence whose pages the lanes hold
+  int fast = 0;  // steps of `ahead` below this one are plain, covered by look_up and nothing is to be done about what follows them
+  // Fetches the step at `ahead` and moves it on, into the next small stretch where its own ends. That one is asked for two steps
+  // before: the answer is there in time, and few stretches wait at a slow SM.
+  auto fetch_ahead = [&](uint8_t* stage) {
+    if (ahead.s < fast && fetcher.plain(p, ahead.s, ahead.s, stage)) {
+      ++ahead.s;
+      return;
     }
-    cp_async_commit();
-  }
-  int slot = 0, free_slot = D - 1;
+    if (ahead.s == ahead.end) {
+      if (ahead.left > 0) {
+        ahead.next_segment(p);
+      } else {
+        if (over) return;
+        const int64_t w = st.workers + static_cast<int64_t>(__shfl_sync(0xffffffffu, ticket, 0)), at = st.begin(w);
+        if (at >= all) {
+          over = true;
+          return;
+        }
+        following = w;
+        const int b = sequence_at(first_s, p.B, at);
+        ahead.set(p, b, first_s[b], at, min(st.q2, all - at));
+        asked = false;
+      }
+      looked_up = nullptr;
+    }
+    if (looked_up == nullptr || ahead.s >= fetcher.base + 32) {
+      looked_up = ahead.sg.table;
+      fetcher.look_up(p, looked_up, ahead.s, 1, ahead.s);
+      fetcher.set_head(p, ahead.sg.h);
+    }
+    if (!asked && ahead.left == 0 && ahead.s + 2 >= ahead.end) {
+      if (lane == 0) ticket = atomicAdd(p.next, 1u);
+      asked = true;
+    }
+    const int plain = fetcher.plain_steps(ahead.sg);
+    if (ahead.s >= plain || !fetcher.plain(p, ahead.s, ahead.s, stage)) fetcher.general(p, ahead.sg, ahead.s, stage);
+    ++ahead.s;
+    fast = min(min(plain, fetcher.base + 32), !asked && ahead.left == 0 ? ahead.end - 2 : ahead.end);
+  };
+  int slot = 0, free_slot = 0, lead = D - 1;  // lead: steps to fetch before the first one is computed
   bool first_piece = true;
   for (;;) {  // segments
-    const int s_first = cur.s;
+    const int s_first = cur.s, cur_plain = fetcher.plain_steps(cur.sg);
     Core core;
     core.init(p, cur.sg);
+#pragma unroll 1
     for (;;) {
-      cp_async_wait<D - 2>();
-      __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
-      if (ahead.left > 0) {
-        fetcher.fetch(p, ahead.sg, ahead.s, ring + free_slot * stage_bytes<Core>());
-        ahead.advance(p);
+      if (lead == 0) {
+        cp_async_wait<D - 2>();
+        __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
       }
+      fetch_ahead(ring + free_slot * stage_bytes<Core>());
       cp_async_commit();
-      core.step(p, cur.sg, cur.s, ring + slot * stage_bytes<Core>());
-      slot = slot + 1 == D ? 0 : slot + 1;
       free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
-      if (cur.segment_ends()) break;
-      ++cur.s;
-      --cur.left;
+      if (lead > 0) {
+        --lead;
+        continue;
+      }
+      const uint8_t* stage = ring + slot * stage_bytes<Core>();
+      if (cur.s >= cur_plain) fetcher.store_new(p, cur.sg, cur.s, stage);
+      core.step(p, cur.sg, cur.s, stage);
+      slot = slot + 1 == D ? 0 : slot + 1;
+      if (++cur.s == cur.end) break;
     }
-    const bool whole = s_first == 0 && cur.s + 1 == cur.steps;
-    const int64_t piece = worker * 2 + (first_piece ? 0 : 1);
+    const bool whole = s_first == 0 && cur.s == cur.steps;
+    const int64_t piece = stretch * 2 + (first_piece ? 0 : 1);
     const int row0 = cur.sg.rb * Core::kRows;
     core.emit([&](int r, int d, const float4& x, float ref, float sum, bool first) {
       const int row = row0 + r;
@@ -480,137 +707,155 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
       }
       if (first && (!whole || p.scores != nullptr)) {
         float* to = whole ? p.ml + (cur.sg.index(p) * p.prows + r) * 2 : p.part_ml + (piece * p.prows + r) * 2;
-        to[0] = ref;
-        to[1] = sum;
+        *reinterpret_cast<float2*>(to) = make_float2(ref, sum);
       }
     });
     first_piece = false;
-    if (cur.left == 1) break;
-    cur.advance(p);
+    if (cur.left > 0) {
+      cur.next_segment(p);
+      continue;
+    }
+    // A stretch ends. `ahead` is in the next one by now, if there is one: no stretch but the list's last is shorter than the ring.
+    if (following < 0) break;
+    stretch = following;
+    following = -1;
+    first_piece = true;
+    const int64_t at = st.begin(stretch);
+    const int b = sequence_at(first_s, p.B, at);
+    cur.set(p, b, first_s[b], at, min(st.q2, all - at));
   }
   cp_async_wait<0>();
 }
 
-// Pieces of a segment: which warps hold some, and where.
+// Pieces of a segment: which stretches hold some, and where.
 struct Pieces {
-  int64_t w0, w1, t0, q;
+  int64_t w0, w1;
+  int second;  // its piece of stretch w0 is that stretch's second
   __device__ __forceinline__ Pieces(const DecodeAttn& p, const Segment& sg, int rb, int steps) {
-    q = p.starts[p.B];
-    t0 = p.starts[sg.b] + (static_cast<int64_t>(sg.h) * p.nrb + rb) * steps;
-    w0 = divide(t0, q);
-    w1 = divide(t0 + steps - 1, q);
+    Stretches st;
+    st.load(p);
+    const int64_t t0 = p.starts[sg.b] + (static_cast<int64_t>(sg.h) * p.nrb + rb) * steps;
+    w0 = st.of(t0);
+    w1 = st.of(t0 + steps - 1);
+    // a segment that starts where a stretch starts is its first piece, as is one that started before
+    second = t0 > st.begin(w0);
   }
-  // a segment that starts where a warp's stretch starts is its first piece, as is one that started before
   __device__ __forceinline__ int64_t row(const DecodeAttn& p, int64_t w, int rr) const {
-    return (w * 2 + (t0 <= w * q ? 0 : 1)) * p.prows + rr;
+    return (w * 2 + (w == w0 ? second : 0)) * p.prows + rr;
   }
 };
 
-// Blocks [0, rows_blocks): WPR warps per query row, joined where several warps hold pieces of it, zero where there is nothing to
-// attend. The others: the weights of a stretch of one sequence's and key head's keys.
+// WPR warps per query row, joined where several stretches hold pieces of it, zero where there is nothing to attend.
 template <typename E, typename Core, int WPR>
-__global__ void __launch_bounds__(kDecJoinThreads)
-attn_decode_join_kernel(const __grid_constant__ DecodeAttn p, int rows_blocks, int chunk, int chunks) {
+__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : kDecJoinThreads)
+attn_decode_join_kernel(const __grid_constant__ DecodeAttn p) {
   grid_dep_sync();
-  constexpr int N = kDecJoinThreads, PER = N / 32 / WPR;            // rows of a block
-  constexpr int kVecs = Core::kDim / 4, kGroups = WPR * 32 / kVecs > 0 ? WPR * 32 / kVecs : 1, kReach = kVecs > WPR * 32 ? kVecs / (WPR * 32) : 1;
+  constexpr int PER = (WPR > 8 ? WPR : kDecJoinThreads / 32) / WPR, VL = Core::kDim / 32;  // rows of a block, elements of a lane
   const int tid = threadIdx.x, lane = tid & 31;
   Segment sg;
-  if (blockIdx.x < rows_blocks) {
-    __shared__ float2 sums[PER][kGroups];
-    __shared__ float4 part_s[PER][kGroups][kVecs];
-    const int slot = tid / (WPR * 32), t = tid % (WPR * 32);
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * PER + slot;  // row of all
-    const bool there = id < static_cast<int64_t>(p.B) * p.Hk * p.R;
-    const int bh = there ? static_cast<int>(id / p.R) : 0, r = there ? static_cast<int>(id % p.R) : 0;
-    sg.set_sequence(p, bh / p.Hk);
-    sg.h = bh % p.Hk;
-    sg.rb = r / Core::kRows;
-    const int rr = r % Core::kRows, grp = t / kVecs, steps = steps_of<Core>(sg.n);
-    const bool some = there && sg.limit(p, r) >= 0 && steps > 0;
-    const Pieces pc(p, sg, sg.rb, steps > 0 ? steps : 1);
-    const bool split = some && pc.w0 != pc.w1;
-    float m = -INFINITY, l = 0.f;
-    float4 x[kReach];
+  __shared__ float2 ml_s[PER][WPR];
+  __shared__ float part_s[PER][WPR][WPR > 1 ? Core::kDim : 1];
+  const int slot = tid / (WPR * 32), wr = tid / 32 % WPR;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * PER + slot;  // row of all
+  const bool there = id < static_cast<int64_t>(p.B) * p.Hk * p.R;
+  const int bh = there ? static_cast<int>(id / p.R) : 0, r = there ? static_cast<int>(id % p.R) : 0;
+  sg.set_sequence(p, bh / p.Hk);
+  sg.h = bh % p.Hk;
+  sg.rb = r / Core::kRows;
+  const int rr = r % Core::kRows, steps = steps_of<Core>(sg.n), d = lane * VL;
+  const bool some = there && sg.limit(p, r) >= 0 && steps > 0;
+  const Pieces pc(p, sg, sg.rb, steps > 0 ? steps : 1);
+  const bool split = some && pc.w0 != pc.w1;
+  float m = kNoRef, l = 0.f;
+  float x[VL];
 #pragma unroll
-    for (int k = 0; k < kReach; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (split) {
-      // every group of lanes takes every kGroups-th piece, relative to a maximum of its own
-#pragma unroll 4
-      for (int64_t w = pc.w0 + grp; w <= pc.w1; w += kGroups) m = fmaxf(m, p.part_ml[pc.row(p, w, rr) * 2]);
-#pragma unroll 4
-      for (int64_t w = pc.w0 + grp; w <= pc.w1; w += kGroups) {
-        const int64_t s = pc.row(p, w, rr);
-        const float f = rebase(p.part_ml[s * 2], m);
-        l = fmaf(f, p.part_ml[s * 2 + 1], l);
+  for (int k = 0; k < VL; ++k) x[k] = 0.f;
+  if (split) {
+    for (int64_t base = pc.w0 + wr; base <= pc.w1; base += 32 * WPR) {
+      const int64_t w = base + lane * WPR;  // this lane's piece
+      float2 ml = make_float2(kNoRef, 0.f);
+      if (w <= pc.w1) ml = *reinterpret_cast<const float2*>(p.part_ml + pc.row(p, w, rr) * 2);
+      const float top = fmaxf(warp_max(ml.x), m), old = rebase(m, top), f = w <= pc.w1 ? rebase(ml.x, top) : 0.f;
+      m = top;
+      l = fmaf(l, old, warp_sum(f * ml.y));
 #pragma unroll
-        for (int k = 0; k < kReach; ++k) {
-          const int d = (t % kVecs + k * WPR * 32) * 4;
-          if (d < p.D) {
-            const float4 y = *reinterpret_cast<const float4*>(p.part + s * Core::kDim + d);
-            x[k].x = fmaf(f, y.x, x[k].x); x[k].y = fmaf(f, y.y, x[k].y); x[k].z = fmaf(f, y.z, x[k].z); x[k].w = fmaf(f, y.w, x[k].w);
+      for (int k = 0; k < VL; ++k) x[k] *= old;
+      const int n = static_cast<int>(min(static_cast<int64_t>(32), (pc.w1 - base) / WPR + 1));
+      constexpr int U = VL <= 4 ? 16 : 8;  // pieces that are read at a time
+      for (int i0 = 0; i0 < n; i0 += U) {
+        float y[U][VL];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float* at = p.part + pc.row(p, base + min(i0 + u, n - 1) * WPR, rr) * Core::kDim + d;
+          if constexpr (VL == 2) {
+            *reinterpret_cast<float2*>(y[u]) = *reinterpret_cast<const float2*>(at);
+          } else {
+#pragma unroll
+            for (int k = 0; k < VL; k += 4) *reinterpret_cast<float4*>(y[u] + k) = *reinterpret_cast<const float4*>(at + k);
           }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float fi = __shfl_sync(0xffffffffu, f, min(i0 + u, 31));
+          if (i0 + u >= n) continue;
+#pragma unroll
+          for (int k = 0; k < VL; ++k) x[k] = fmaf(fi, y[u][k], x[k]);
         }
       }
     }
-    if constexpr (kGroups > 1) {
-      part_s[slot][grp][t % kVecs] = x[0];
-      if (t % kVecs == 0) sums[slot][grp] = make_float2(m, l);
-      if constexpr (WPR > 1) __syncthreads();
-      else __syncwarp();
-      if (grp > 0) return;
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) m = fmaxf(m, sums[slot][k].x);
-      l = 0.f;
-      x[0] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        const float f = rebase(sums[slot][k].x, m);
-        const float4 y = part_s[slot][k][t % kVecs];
-        l = fmaf(f, sums[slot][k].y, l);
-        x[0].x = fmaf(f, y.x, x[0].x); x[0].y = fmaf(f, y.y, x[0].y); x[0].z = fmaf(f, y.z, x[0].z); x[0].w = fmaf(f, y.w, x[0].w);
-      }
-    }
-    if (!there || (some && !split)) return;
-#pragma unroll
-    for (int k = 0; k < kReach; ++k) {
-      const int d = (t % kVecs + k * WPR * 32) * 4;
-      if (d < p.D) store_out<E>(p, sg, r, d, some ? scaled(x[k], p.keep / l) : make_float4(0.f, 0.f, 0.f, 0.f));
-    }
-    return;
   }
-  const int id = (blockIdx.x - rows_blocks) / chunks;
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int k = 0; k < VL; ++k) part_s[slot][wr][d + k] = x[k];
+    if (lane == 0) ml_s[slot][wr] = make_float2(m, l);
+    __syncthreads();
+    if (wr > 0) return;
+#pragma unroll
+    for (int k = 0; k < WPR; ++k) m = fmaxf(m, ml_s[slot][k].x);
+    l = 0.f;
+#pragma unroll
+    for (int k = 0; k < VL; ++k) x[k] = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < WPR; ++k) {
+      const float f = rebase(ml_s[slot][k].x, m);
+      l = fmaf(f, ml_s[slot][k].y, l);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) x[e] = fmaf(f, part_s[slot][k][d + e], x[e]);
+    }
+  }
+  if (!there || (some && !split)) return;
+  if (split && p.scores != nullptr && lane == 0)
+    *reinterpret_cast<float2*>(p.ml + (sg.index(p) * p.prows + rr) * 2) = make_float2(m, l);
+  const float f = p.keep / l;
+  char* row = p.out + sg.b * p.os[0] + (sg.h * p.G + r / p.T) * p.os[1] + (r % p.T) * p.os[2];
+#pragma unroll
+  for (int k = 0; k < VL; ++k)
+    if (d + k < p.D) Elem<E>::store(reinterpret_cast<E*>(row) + d + k, some ? x[k] * f : 0.f);
+}
+
+// The weights of kWeightsChunk of one sequence's and key head's keys, from the rows' statistics that the join left.
+constexpr int kWeightsChunk = 1024;
+
+__global__ void __launch_bounds__(kDecJoinThreads)
+attn_decode_weights_kernel(const __grid_constant__ DecodeAttn p, int rows_of_block, int chunks) {
+  grid_dep_sync();
+  extern __shared__ float2 row_ml[];  // [R]
+  const int tid = threadIdx.x, id = blockIdx.x / chunks;
+  const float* ml = p.ml + static_cast<int64_t>(id) * p.nrb * p.prows * 2;
+  for (int r = tid; r < p.R; r += kDecJoinThreads) {
+    const float2 x = *reinterpret_cast<const float2*>(ml + (r / rows_of_block * p.prows + r % rows_of_block) * 2);
+    row_ml[r] = make_float2(x.x, 1.f / x.y);
+  }
+  Segment sg;
   sg.set_sequence(p, id / p.Hk);
   sg.h = id % p.Hk;
-  const int j0 = (blockIdx.x - rows_blocks) % chunks * chunk, steps = steps_of<Core>(sg.n);
-  if (j0 >= sg.n) return;
-  extern __shared__ float2 row_ml[];  // [R]
-  for (int r = tid >> 5; r < p.R; r += N / 32) {  // a warp per row
-    const int rb = r / Core::kRows, rr = r % Core::kRows;
-    const Pieces pc(p, sg, rb, steps);
-    float m = -INFINITY, l = 0.f;
-    if (pc.w0 == pc.w1) {
-      const float* s = p.ml + ((static_cast<int64_t>(id) * p.nrb + rb) * p.prows + rr) * 2;
-      m = s[0];
-      l = s[1];
-    } else {
-      for (int64_t w = pc.w0 + lane; w <= pc.w1; w += 32) m = fmaxf(m, p.part_ml[pc.row(p, w, rr) * 2]);
-      m = warp_max(m);
-      for (int64_t w = pc.w0 + lane; w <= pc.w1; w += 32) {
-        const float* s = p.part_ml + pc.row(p, w, rr) * 2;
-        l = fmaf(rebase(s[0], m), s[1], l);
-      }
-      l = warp_sum(l);
-    }
-    if (lane == 0) row_ml[r] = make_float2(m, 1.f / l);
-  }
   __syncthreads();
-  add_weights<N>(p, sg, j0, min(j0 + chunk, sg.n), [&](int r) { return row_ml[r]; });
+  const int j0 = blockIdx.x % chunks * kWeightsChunk;
+  if (j0 < sg.n)
+    add_weights<kDecJoinThreads, kWeightsChunk / kDecJoinThreads>(p, sg, j0, min(j0 + kWeightsChunk, sg.n), [&](int r) { return row_ml[r]; });
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
-constexpr int kWeightsChunk = 1024;
-
 template <typename K>
 bool set_smem(K kernel, int bytes) {
   if (bytes <= 48 * 1024) return true;
@@ -620,29 +865,35 @@ bool set_smem(K kernel, int bytes) {
 }
 
 template <typename E, typename Core>
-int launch_decode(const DecodeAttn& d, bool split, cudaStream_t st) {
-  if (!split) {
-    constexpr int ring = Core::kDirectWarps * ring_bytes<Core>(), sums = Core::kDirectWarps * Core::kRows * (Core::kDim + 4) * 4;
+int launch_decode(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
+  constexpr int ring = kDecWarps * ring_bytes<Core>(), sums = kDecWarps * Core::kRows * (Core::kDim + 4) * 4;
+  if (!pl.split) {
     constexpr int smem = ring > sums ? ring : sums;
     if (!set_smem(attn_decode_direct_kernel<E, Core>, smem)) return PTJ_ERR_LAUNCH;
-    launch_k(attn_decode_direct_kernel<E, Core>, d.B * d.Hk * d.nrb, Core::kDirectWarps * 32, smem, st, d);
+    launch_cluster_k(attn_decode_direct_kernel<E, Core>, dim3(static_cast<unsigned>(d.B * d.Hk * d.nrb * pl.cluster)), kDecWarps * 32,
+                     pl.cluster, smem, st, d);
     PTJ_CHECK_LAUNCH();
     return PTJ_OK;
   }
-  constexpr int smem = kDecSplitWarps * ring_bytes<Core>();
-  // rows that many warps hold pieces of are joined by a block each: where there are few rows
-  const int64_t rows = static_cast<int64_t>(d.B) * d.Hk * d.R;
-  const bool few = rows <= 2 * kNumSMs;
-  const int64_t row_blocks = few ? rows : ceil_div(rows, kDecJoinThreads / 32);
-  const int64_t chunks = d.scores == nullptr ? 1 : ceil_div(d.rows.capacity, kWeightsChunk);
-  const int64_t blocks = row_blocks + (d.scores == nullptr ? 0 : static_cast<int64_t>(d.B) * d.Hk * chunks);
+  // warps that join a row: by the pieces to be expected of a segment
+  const int64_t rows = static_cast<int64_t>(d.B) * d.Hk * d.R, pieces = (d.workers + d.small) / (static_cast<int64_t>(d.B) * d.Hk * d.nrb);
+  const int wpr = pieces <= 3 ? 1 : (pieces <= 32 ? 4 : 16), threads = wpr == 16 ? 512 : kDecJoinThreads;
+  const int64_t blocks = ceil_div(rows * wpr * 32, threads);
   if (blocks > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
-  if (!set_smem(attn_decode_split_kernel<E, Core>, smem)) return PTJ_ERR_LAUNCH;
-  launch_k(attn_decode_split_kernel<E, Core>, d.workers / kDecSplitWarps, kDecSplitWarps * 32, smem, st, d);
+  if (d.small > 0 && cudaMemsetAsync(d.next, 0, 4, st) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return PTJ_ERR_LAUNCH;
+  }
+  if (!set_smem(attn_decode_split_kernel<E, Core>, ring)) return PTJ_ERR_LAUNCH;
+  launch_k(attn_decode_split_kernel<E, Core>, d.workers / kDecWarps, kDecWarps * 32, ring, st, d);
   PTJ_CHECK_LAUNCH();
-  const auto join = few ? attn_decode_join_kernel<E, Core, kDecJoinThreads / 32> : attn_decode_join_kernel<E, Core, 1>;
-  launch_k(join, static_cast<int>(blocks), kDecJoinThreads, d.scores == nullptr ? 0 : d.R * 8, st, d, static_cast<int>(row_blocks),
-           kWeightsChunk, static_cast<int>(chunks));
+  const auto join = wpr == 1 ? attn_decode_join_kernel<E, Core, 1> : (wpr == 4 ? attn_decode_join_kernel<E, Core, 4> : attn_decode_join_kernel<E, Core, 16>);
+  launch_k(join, static_cast<int>(blocks), threads, 0, st, d);
+  PTJ_CHECK_LAUNCH();
+  if (d.scores == nullptr) return PTJ_OK;
+  const int64_t chunks = ceil_div(d.rows.capacity, kWeightsChunk);
+  if (chunks * d.B * d.Hk > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
+  launch_k(attn_decode_weights_kernel, static_cast<int>(chunks * d.B * d.Hk), kDecJoinThreads, d.R * 8, st, d, pl.rows, static_cast<int>(chunks));
   PTJ_CHECK_LAUNCH();
   return PTJ_OK;
 }

@@ -13,9 +13,10 @@ struct CoreFma {
   static constexpr int LPK = DP / VEC < 32 ? DP / VEC : 32, NV = DP / (VEC * LPK), KPW = 32 / LPK, W = VEC * NV;
   static constexpr int KS = 4096 / kRowBytes, KB = KS / KPW;  // keys of a step, of a lane
   static constexpr int kDepth = 3;
-  static constexpr int kBlocks = 2, kDirectWarps = 8;
+  static constexpr int kBlocks = 2;
   float q[RB][W], o[RB][W];
-  float ref[RB], sum[RB];
+  float ref[RB], sum[RB], over[RB];  // over: scores beyond it (not scaled) move the reference
+  int limit[RB];  // last keys that the rows attend
   int sub_lane, grp;
 
   __device__ __forceinline__ int elem(int i) const { return (i * LPK + sub_lane) * VEC; }
@@ -26,12 +27,14 @@ struct CoreFma {
     grp = lane / LPK;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      ref[r] = -INFINITY;
+      ref[r] = kNoRef;
+      over[r] = -INFINITY;
       sum[r] = 0.f;
 #pragma unroll
       for (int i = 0; i < W; ++i) q[r][i] = o[r][i] = 0.f;
       const int row = sg.rb * kRows + r;
-      if (sg.limit(p, row) < 0) continue;
+      limit[r] = sg.limit(p, row);
+      if (limit[r] < 0) continue;
       const E* src = reinterpret_cast<const E*>(sg.q_row(p, row));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -57,11 +60,7 @@ struct CoreFma {
   __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) {
     const int j0 = sub * KS;
     const uint32_t present = present_keys<KS, kRowBytes>(stage);
-    if (j0 + KS > sg.first + 1 || present != (1u << KS) - 1u) step_of<true>(p, sg, j0, stage, present);
-    else step_of<false>(p, sg, j0, stage, present);
-  }
-  template <bool EDGE>
-  __device__ __forceinline__ void step_of(const DecodeAttn& p, const Segment& sg, int j0, const uint8_t* stage, uint32_t present) {
+    const bool edge = j0 + KS > sg.first + 1 || present != (1u << KS) - 1u;  // some rows do not attend all of its keys
     float k[KB][W], v[KB][W];
 #pragma unroll
     for (int e = 0; e < KB; ++e) read(stage, e * KPW + grp, k[e]);
@@ -71,7 +70,6 @@ struct CoreFma {
     for (int r = 0; r < RB; ++r) {
       const int row = sg.rb * kRows + r;
       if (RB > 1 && row >= p.R) break;
-      const int limit = EDGE ? sg.limit(p, row) : 0;
       float s[KB];
 #pragma unroll
       for (int e = 0; e < KB; ++e) {
@@ -83,35 +81,49 @@ struct CoreFma {
       for (int x = LPK / 2; x > 0; x >>= 1)
 #pragma unroll
         for (int e = 0; e < KB; ++e) s[e] += __shfl_xor_sync(0xffffffffu, s[e], x);
-      bool over = false;
+      if (edge) {
 #pragma unroll
-      for (int e = 0; e < KB; ++e) {
-        const int i = e * KPW + grp;
-        s[e] *= p.scale;
-        if (EDGE && (!((present >> i) & 1u) || j0 + i > limit)) s[e] = -INFINITY;
-        over |= s[e] > ref[r] + kDecLazy;
-        if (p.scores != nullptr && sub_lane == 0 && j0 + i < sg.n)
-          p.scores[((static_cast<int64_t>(sg.b) * p.Hk + sg.h) * p.R + row) * p.scores_ld + j0 + i] = s[e];
+        for (int e = 0; e < KB; ++e)
+          if (!((present >> (e * KPW + grp)) & 1u) || j0 + e * KPW + grp > limit[r]) s[e] = -INFINITY;
       }
-      if (__any_sync(0xffffffffu, over)) {
+      bool moves = false;
+#pragma unroll
+      for (int e = 0; e < KB; ++e) moves |= s[e] > over[r];
+      if (p.scores != nullptr && sub_lane == 0) {
+        float* to = sg.score_row(p, row) + j0 + grp;
+#pragma unroll
+        for (int e = 0; e < KB; ++e)
+          if (j0 + e * KPW + grp < sg.n) to[e * KPW] = s[e] * p.scale;
+      }
+      if (__any_sync(0xffffffffu, moves)) {
         float m = s[0];
 #pragma unroll
         for (int e = 1; e < KB; ++e) m = fmaxf(m, s[e]);
-        m = fmaxf(warp_max(m), ref[r]);
+        m = fmaxf(warp_max(m) * p.scale, ref[r]);
         const float f = rebase(ref[r], m);
         ref[r] = m;
+        over[r] = (m + kDecLazy) * p.unscale;
         sum[r] *= f;
 #pragma unroll
         for (int i = 0; i < W; ++i) o[r][i] *= f;
       }
-      const float base = base_of(ref[r]);
 #pragma unroll
       for (int e = 0; e < KB; ++e) {
-        const float x = ex2(s[e] - base);
-        sum[r] += x;
-        const bool on = !EDGE || j0 + e * KPW + grp <= limit;  // zero times what is not finite is not zero
+        s[e] = ex2(fmaf(s[e], p.scale, -ref[r]));
+        sum[r] += s[e];
+      }
+      if (edge) {  // zero times what is not finite is not zero
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[r][i] = fmaf(x, on ? v[e][i] : 0.f, o[r][i]);
+        for (int e = 0; e < KB; ++e) {
+          if (j0 + e * KPW + grp > limit[r]) continue;
+#pragma unroll
+          for (int i = 0; i < W; ++i) o[r][i] = fmaf(s[e], v[e][i], o[r][i]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < KB; ++e)
+#pragma unroll
+          for (int i = 0; i < W; ++i) o[r][i] = fmaf(s[e], v[e][i], o[r][i]);
       }
     }
   }
@@ -138,24 +150,21 @@ struct CoreFma {
 
 }  // namespace
 
-int decode_fma_blocks(int dim, int rows, int es) {
-  if (es == 2) return dim == 256 && (rows == 1 || rows == 4) ? 2 : 0;
-  return (dim == 64 || dim == 128) && (rows == 1 || rows == 4 || rows == 8) || dim == 256 && (rows == 1 || rows == 4) ? 2 : 0;
-}
+int decode_fma_blocks() { return CoreFma<float, 64, 1>::kBlocks; }
 
 int launch_decode_fma(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
   using B = __nv_bfloat16;
   if (pl.es == 2)
-    return pl.rows == 1 ? launch_decode<B, CoreFma<B, 256, 1>>(d, pl.split, st) : launch_decode<B, CoreFma<B, 256, 4>>(d, pl.split, st);
+    return pl.rows == 1 ? launch_decode<B, CoreFma<B, 256, 1>>(d, pl, st) : launch_decode<B, CoreFma<B, 256, 4>>(d, pl, st);
   switch (pl.dim + pl.rows) {
-    case 64 + 1: return launch_decode<float, CoreFma<float, 64, 1>>(d, pl.split, st);
-    case 64 + 4: return launch_decode<float, CoreFma<float, 64, 4>>(d, pl.split, st);
-    case 64 + 8: return launch_decode<float, CoreFma<float, 64, 8>>(d, pl.split, st);
-    case 128 + 1: return launch_decode<float, CoreFma<float, 128, 1>>(d, pl.split, st);
-    case 128 + 4: return launch_decode<float, CoreFma<float, 128, 4>>(d, pl.split, st);
-    case 128 + 8: return launch_decode<float, CoreFma<float, 128, 8>>(d, pl.split, st);
-    case 256 + 1: return launch_decode<float, CoreFma<float, 256, 1>>(d, pl.split, st);
-    default: return launch_decode<float, CoreFma<float, 256, 4>>(d, pl.split, st);
+    case 64 + 1: return launch_decode<float, CoreFma<float, 64, 1>>(d, pl, st);
+    case 64 + 4: return launch_decode<float, CoreFma<float, 64, 4>>(d, pl, st);
+    case 64 + 8: return launch_decode<float, CoreFma<float, 64, 8>>(d, pl, st);
+    case 128 + 1: return launch_decode<float, CoreFma<float, 128, 1>>(d, pl, st);
+    case 128 + 4: return launch_decode<float, CoreFma<float, 128, 4>>(d, pl, st);
+    case 128 + 8: return launch_decode<float, CoreFma<float, 128, 8>>(d, pl, st);
+    case 256 + 1: return launch_decode<float, CoreFma<float, 256, 1>>(d, pl, st);
+    default: return launch_decode<float, CoreFma<float, 256, 4>>(d, pl, st);
   }
 }
 

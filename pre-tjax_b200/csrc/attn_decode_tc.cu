@@ -5,25 +5,28 @@
 // is free as long as Q and K agree, so a lane's 16 bytes of a key are its operands of two products, and its 16 bytes of four
 // values turn into operands of four products by picking halves of pairs (the transposition that V needs). P^T comes from S^T by
 // transposing 8 x 8 blocks in registers. Probabilities are multiplied in two bf16 parts (16 bits): rounding them to one would
-// cost as much accuracy as rounding the output does. The products of the fourth-generation form suffice: 12 per step of 16 keys
-// at 64 elements, 2 % of their rate at full memory speed.
+// cost as much accuracy as rounding the output does. Up to four rows take four columns with their first parts and the other four
+// with their second ones, so the second part costs nothing; more rows take a second product. A product takes 32 cycles of an SM's
+// quarter here (the form with operands in registers; 24 of them a step of 16 keys of 128 elements kept its pipe busy half of
+// the time), which is what bounds many rows.
 #include "attn_decode.cuh"
 
 namespace ptj {
 namespace {
 
-template <int DP, int NR>
+template <int DP, int NR, bool HALF = false>
 struct CoreTc {
-  static constexpr int KS = 16, kRows = 8 * NR, kDim = DP, kRowBytes = 2 * DP, KU = DP / 32, VW = DP / 64;
+  static_assert(!HALF || NR == 1, "");
+  static constexpr int KS = 16, kRows = HALF ? 4 : 8 * NR, kDim = DP, kRowBytes = 2 * DP, KU = DP / 32, VW = DP / 64;
   static constexpr int kDepth = DP == 64 ? (NR == 1 ? 3 : 4) : 3;
   static constexpr int kBlocks = DP == 64 ? (NR == 1 ? 4 : 3) : 2;  // resident per SM
-  static constexpr int kDirectWarps = DP == 64 && NR == 1 ? 16 : 8;
   uint4 q[NR][KU];
   float o[NR][DP / 16][4];
-  float ref[NR][2], sum[NR][2];
+  float ref[NR][2], sum[NR][2], over[NR][2];  // over: scores beyond it (not scaled) move the reference
   int g, c;
   uint32_t key_at, value_at[2];  // this lane's pieces in a step
-  float* score_at;               // scores of its first row, at the first of its keys of step 0
+  float* score_at;               // scores of its first column's row, at the first of its keys of step 0; NULL: not wanted
+  int limit[NR][2];              // last keys that its columns' rows attend
 
   __device__ __forceinline__ void init(const DecodeAttn& p, const Segment& sg) {
     const int lane = threadIdx.x & 31;
@@ -32,10 +35,10 @@ struct CoreTc {
     key_at = g * kRowBytes + ((c ^ swizzle(g)) << 4);
 #pragma unroll
     for (int i = 0; i < 2; ++i) value_at[i] = (KS + 2 * c + i) * kRowBytes + ((g ^ swizzle(2 * c + i)) << 4);
-    score_at = p.scores == nullptr ? nullptr : sg.score_row(p, sg.rb * kRows + 2 * c) + g;
+    score_at = p.scores == nullptr || (HALF && c >= 2) ? nullptr : sg.score_row(p, sg.rb * kRows + 2 * c) + g;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-      const int r = sg.rb * kRows + i * 8 + g;
+      const int r = sg.rb * kRows + (HALF ? g & 3 : i * 8 + g);
       const bool on = sg.limit(p, r) >= 0;
       const char* row = on ? sg.q_row(p, r) : nullptr;
 #pragma unroll
@@ -53,8 +56,11 @@ struct CoreTc {
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        ref[i][e] = -INFINITY;
+        ref[i][e] = kNoRef;
+        over[i][e] = -INFINITY;
         sum[i][e] = 0.f;
+        const int row = sg.rb * kRows + row_of(i, e);
+        limit[i][e] = sg.limit(p, row);
       }
 #pragma unroll
       for (int j = 0; j < DP / 16; ++j)
@@ -63,6 +69,8 @@ struct CoreTc {
     }
   }
 
+  // row of the block that column 2 c + e of a product belongs to
+  __device__ __forceinline__ int row_of(int i, int e) const { return HALF ? 2 * (c & 1) + e : i * 8 + 2 * c + e; }
   // rows of S^T (keys of a step) and k of O^T's products that this lane holds
   __device__ __forceinline__ int key_of(int i) const { return g + 8 * i; }
   __device__ __forceinline__ int value_of(int i) const { return 2 * c + (i & 1) + 8 * (i >> 1); }
@@ -93,7 +101,7 @@ struct CoreTc {
     const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
     const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
     mma(acc, a0, a1, a2, a3, ph[0], ph[1]);
-    mma(acc, a0, a1, a2, a3, pl[0], pl[1]);
+    if constexpr (!HALF) mma(acc, a0, a1, a2, a3, pl[0], pl[1]);
   }
 
   __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) {
@@ -102,21 +110,23 @@ struct CoreTc {
     float s[NR][4];
 #pragma unroll
     for (int i = 0; i < NR; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    float s2[NR][4];  // a second chain of products where there is one column of them
+#pragma unroll
+    for (int i = 0; i < NR; ++i) s2[i][0] = s2[i][1] = s2[i][2] = s2[i][3] = 0.f;
 #pragma unroll
     for (int u = 0; u < KU; ++u) {
       const uint4 k0 = key(stage, 0, u), k1 = key(stage, 1, u);
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
         mma(s[i], k0.x, k1.x, k0.y, k1.y, q[i][u].x, q[i][u].y);
-        mma(s[i], k0.z, k1.z, k0.w, k1.w, q[i][u].z, q[i][u].w);
+        mma(NR == 1 ? s2[i] : s[i], k0.z, k1.z, k0.w, k1.w, q[i][u].z, q[i][u].w);
       }
     }
+    if constexpr (NR == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][e] += s2[0][e];
+    }
     const uint32_t present = present_keys<KS, kRowBytes>(stage);
-    bool over = false;
-#pragma unroll
-    for (int i = 0; i < NR; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] *= p.scale;
     if (edge || present != 0xffffu) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -126,25 +136,26 @@ struct CoreTc {
         for (int i = 0; i < NR; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (!there || j > sg.limit(p, sg.rb * kRows + i * 8 + 2 * c + e)) s[i][2 * x + e] = -INFINITY;
+            if (!there || j > limit[i][e]) s[i][2 * x + e] = -INFINITY;
       }
     }
+    bool moves = false;
 #pragma unroll
     for (int i = 0; i < NR; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) over |= s[i][e] > ref[i][e & 1] + kDecLazy;
+      for (int e = 0; e < 4; ++e) moves |= s[i][e] > over[i][e & 1];
     if (score_at != nullptr) {
 #pragma unroll
       for (int i = 0; i < NR; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (sg.rb * kRows + i * 8 + 2 * c + e < p.R) {
+          if (sg.rb * kRows + row_of(i, e) < p.R) {
             float* to = score_at + (i * 8 + e) * p.scores_ld + j0;
-            if (j0 + g < sg.n) to[0] = s[i][e];
-            if (j0 + g + 8 < sg.n) to[8] = s[i][e + 2];
+            if (j0 + g < sg.n) to[0] = s[i][e] * p.scale;
+            if (j0 + g + 8 < sg.n) to[8] = s[i][e + 2] * p.scale;
           }
     }
-    if (__any_sync(0xffffffffu, over)) {
+    if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
       for (int i = 0; i < NR; ++i)
 #pragma unroll
@@ -152,9 +163,10 @@ struct CoreTc {
           float m = fmaxf(s[i][e], s[i][e + 2]);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-          m = fmaxf(m, ref[i][e]);
+          m = fmaxf(m * p.scale, ref[i][e]);
           const float f = rebase(ref[i][e], m);
           ref[i][e] = m;
+          over[i][e] = (m + kDecLazy) * p.unscale;
           sum[i][e] *= f;
 #pragma unroll
           for (int j = 0; j < DP / 16; ++j) {
@@ -168,13 +180,17 @@ struct CoreTc {
     for (int i = 0; i < NR; ++i)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const float x0 = ex2(s[i][2 * k] - base_of(ref[i][0])), x1 = ex2(s[i][2 * k + 1] - base_of(ref[i][1]));
+        const float x0 = ex2(fmaf(s[i][2 * k], p.scale, -ref[i][0])), x1 = ex2(fmaf(s[i][2 * k + 1], p.scale, -ref[i][1]));
         sum[i][0] += x0;
         sum[i][1] += x1;
         const uint32_t hi = pack(x0, x1);
         const uint32_t lo = pack(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
-        ph[i][k] = transpose8(hi);
-        pl[i][k] = transpose8(lo);
+        if constexpr (HALF) {
+          ph[i][k] = transpose8(c < 2 ? hi : lo);
+        } else {
+          ph[i][k] = transpose8(hi);
+          pl[i][k] = transpose8(lo);
+        }
       }
     // a value that some rows of the step attend and others do not must be finite to be multiplied by the others' zeros
     if (edge && not_finite(stage)) {
@@ -226,7 +242,7 @@ struct CoreTc {
             values(acc, v, j, ph[i], pl[i]);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if ((sg.rb * kRows + i * 8 + 2 * c + e) % p.T == tok) {
+              if (limit[i][e] == sg.first + tok) {
                 o[i][w * 4 + j][e] += acc[e];
                 o[i][w * 4 + j][e + 2] += acc[e + 2];
               }
@@ -244,33 +260,45 @@ struct CoreTc {
         float l = sum[i][e];
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        if constexpr (HALF) {  // the parts of a row meet; its two lanes share the elements
 #pragma unroll
-        for (int w = 0; w < VW; ++w)
+          for (int j = 0; j < DP / 16; ++j) {
+            o[i][j][e] += __shfl_xor_sync(0xffffffffu, o[i][j][e], 2);
+            o[i][j][e + 2] += __shfl_xor_sync(0xffffffffu, o[i][j][e + 2], 2);
+          }
+        }
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-            f(i * 8 + 2 * c + e, 64 * w + 8 * g + 4 * hf,
-              make_float4(o[i][w * 4 + 2 * hf][e], o[i][w * 4 + 2 * hf][e + 2], o[i][w * 4 + 2 * hf + 1][e], o[i][w * 4 + 2 * hf + 1][e + 2]),
-              ref[i][e], l, w == 0 && hf == 0 && g == 0);
+        for (int w = 0; w < VW; ++w) {
+          const float (&x)[4] = o[i][4 * w], (&y)[4] = o[i][4 * w + 1], (&z)[4] = o[i][4 * w + 2], (&u)[4] = o[i][4 * w + 3];
+          if constexpr (HALF) {
+            const bool up = c >= 2;
+            f(row_of(i, e), 64 * w + 8 * g + (up ? 4 : 0),
+              make_float4(up ? z[e] : x[e], up ? z[e + 2] : x[e + 2], up ? u[e] : y[e], up ? u[e + 2] : y[e + 2]), ref[i][e], l,
+              w == 0 && g == 0 && !up);
+          } else {
+            f(row_of(i, e), 64 * w + 8 * g, make_float4(x[e], x[e + 2], y[e], y[e + 2]), ref[i][e], l, w == 0 && g == 0);
+            f(row_of(i, e), 64 * w + 8 * g + 4, make_float4(z[e], z[e + 2], u[e], u[e + 2]), ref[i][e], l, false);
+          }
+        }
       }
   }
 };
 
 }  // namespace
 
-int decode_tc_blocks(int dim, int rows) {
-  if (dim == 64) return rows == 8 || rows == 16 || rows == 32 ? CoreTc<64, 1>::kBlocks : 0;
-  return dim == 128 && (rows == 8 || rows == 16 || rows == 24) ? CoreTc<128, 1>::kBlocks : 0;
-}
+int decode_tc_blocks(int dim, int rows) { return dim == 128 ? CoreTc<128, 1>::kBlocks : (rows <= 8 ? CoreTc<64, 1>::kBlocks : CoreTc<64, 2>::kBlocks); }
 
 int launch_decode_tc(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
   using E = __nv_bfloat16;
   switch (pl.dim + pl.rows) {
-    case 64 + 8: return launch_decode<E, CoreTc<64, 1>>(d, pl.split, st);
-    case 64 + 16: return launch_decode<E, CoreTc<64, 2>>(d, pl.split, st);
-    case 64 + 32: return launch_decode<E, CoreTc<64, 4>>(d, pl.split, st);
-    case 128 + 8: return launch_decode<E, CoreTc<128, 1>>(d, pl.split, st);
-    case 128 + 16: return launch_decode<E, CoreTc<128, 2>>(d, pl.split, st);
-    default: return launch_decode<E, CoreTc<128, 3>>(d, pl.split, st);
+    case 64 + 4: return launch_decode<E, CoreTc<64, 1, true>>(d, pl, st);
+    case 64 + 8: return launch_decode<E, CoreTc<64, 1>>(d, pl, st);
+    case 64 + 16: return launch_decode<E, CoreTc<64, 2>>(d, pl, st);
+    case 64 + 32: return launch_decode<E, CoreTc<64, 4>>(d, pl, st);
+    case 128 + 4: return launch_decode<E, CoreTc<128, 1, true>>(d, pl, st);
+    case 128 + 8: return launch_decode<E, CoreTc<128, 1>>(d, pl, st);
+    case 128 + 16: return launch_decode<E, CoreTc<128, 2>>(d, pl, st);
+    default: return launch_decode<E, CoreTc<128, 3>>(d, pl, st);
   }
 }
 

@@ -31,6 +31,7 @@ int make_paged_rows(const ptj_kv_cache* c, PagedRows& out) {
   for (int i = 0; i < 25; ++i)
     if (c->page_size == (1ll << i)) out.page_shift = i;
   out.capacity = static_cast<int>(c->table_width * c->page_size);
+  out.capacity_pages = static_cast<int>(c->table_width);
   out.row_bytes = static_cast<int>(c->d_head * es);
   return PTJ_OK;
 }

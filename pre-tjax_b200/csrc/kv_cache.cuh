@@ -16,23 +16,23 @@ struct PagedRows {
   int64_t page_stride[2], head_stride[2], slot_stride[2];  // of the keys' and the values' pool
   unsigned int* fault;
   int pages, page_size, page_shift;  // page_shift: log2 of the page size, -1 where it is no power of two
-  int capacity;                      // keys that a row of the table holds
+  int capacity, capacity_pages;      // keys that a row of the table holds, its pages
   int row_bytes;                     // of a key or a value
-  // page and slot of key j; false: the table names no page of the pool
-  __device__ __forceinline__ bool locate(const int32_t* row, int j, int64_t& page, int& slot) const {
-    int i;
-    if (page_shift >= 0) {
-      i = j >> page_shift;
-      slot = j & (page_size - 1);
-    } else {
-      i = static_cast<int>(static_cast<unsigned int>(j) / static_cast<unsigned int>(page_size));
-      slot = j - i * page_size;
-    }
-    const int p = row[i];
-    page = p;
-    if (static_cast<unsigned int>(p) < static_cast<unsigned int>(pages)) return true;
+  // place of key j's page in the table
+  __device__ __forceinline__ int page_of(int j) const {
+    return page_shift >= 0 ? j >> page_shift : static_cast<int>(static_cast<unsigned int>(j) / static_cast<unsigned int>(page_size));
+  }
+  __device__ __forceinline__ bool check(int page) const {
+    if (static_cast<unsigned int>(page) < static_cast<unsigned int>(pages)) return true;
     tc::record_fault(fault, kFaultPage);
     return false;
+  }
+  // page and slot of key j; false: the table names no page of the pool
+  __device__ __forceinline__ bool locate(const int32_t* row, int j, int64_t& page, int& slot) const {
+    const int i = page_of(j), p = row[i];
+    slot = j - i * page_size;
+    page = p;
+    return check(p);
   }
   __device__ __forceinline__ int64_t offset(int kv, int64_t page, int h, int slot) const {  // kv: 0 keys, 1 values
     return page * page_stride[kv] + h * head_stride[kv] + slot * slot_stride[kv];
@@ -42,6 +42,16 @@ struct PagedRows {
     if (n >= 0 && n <= capacity) return n;
     tc::record_fault(fault, kFaultLength);
     return n < 0 ? 0 : capacity;
+  }
+  // length and count at once: one wait for both
+  __device__ __forceinline__ void extent(const int32_t* lengths, const int32_t* counts, int tokens, int b, int& n, int& c) const {
+    n = lengths[b];
+    c = counts == nullptr ? tokens : counts[b];
+    if (n < 0 || n > capacity || c < 0 || c > tokens) {
+      tc::record_fault(fault, kFaultLength);
+      n = min(max(n, 0), capacity);
+      c = min(max(c, 0), tokens);
+    }
   }
   __device__ __forceinline__ int count(const int32_t* counts, int tokens, int b) const {
     if (counts == nullptr) return tokens;

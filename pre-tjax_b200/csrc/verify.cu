@@ -4,16 +4,17 @@
 // max(p - q, 0) leaves the target's distribution p unchanged: q(x) min(1, p/q) + (sum of rejections) max(p - q, 0) / total = p(x).
 //
 // Of all the probabilities only one row per sequence (two with a draft's distribution) is read whole: the one the next token is
-// drawn from. A cluster of C blocks shares it. Each block sums its slice, the sums meet through distributed shared memory, and
-// the block in whose slice the running sum passes the mark looks for the place: a warp's chunk, 256 elements of it, 32, one.
-// Sums are float64, products of two float32 in float64 are exact: decisions then agree with a sum in any other order except for
-// marks within 1e-13 or so of a border.
+// drawn from. A cluster of C blocks shares it, every warp takes a contiguous chunk and keeps the sums of up to 32 groups of it. The
+// blocks' sums meet through distributed shared memory; the group in which the running sum passes the mark is found from sums, and
+// only its elements (256 of a vocabulary below 500 000) are read again. Bound by the chain of dependent loads, not by bytes: the
+// drafts, their probabilities, the row in four or five batches, the group. Sums are float64, products of two float32 in float64 are
+// exact: decisions then agree with a sum in any other order except for marks within 1e-13 or so of a border.
 #include "cluster.cuh"
 
 namespace ptj {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kGroups = 32, kBatch = 8, kGroup = 32 * kBatch;
 
 struct Verify {
   const void *target, *draft;
@@ -40,34 +41,54 @@ struct Weights {
     if (sub != nullptr) w -= static_cast<double>(Elem<E>::load(sub + j));
     return w > 0.0 && j != skip ? w : 0.0;  // (a NaN has none)
   }
-  // of every 32nd element from j0 + lane on; a batch of loads is under way at a time, the last one too
+  // this lane's elements of the kGroup from g on
   template <bool SUB>
-  __device__ __forceinline__ double sum(int j0, int j1, int lane) const {
-    constexpr int U = 8;
-    double s[2] = {0.0, 0.0};
-    for (int g = j0 + lane; g < j1; g += 32 * U) {
-      float x[U], y[U];
+  __device__ __forceinline__ void load(int g, int j1, float (&x)[kBatch], float (&y)[kBatch]) const {
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int j = g + 32 * i;
-        x[i] = j < j1 && (SUB || j != skip) ? Elem<E>::load(row + j) : 0.f;
-        y[i] = SUB && j < j1 ? Elem<E>::load(sub + j) : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const double w = SUB ? static_cast<double>(x[i]) - static_cast<double>(y[i]) : static_cast<double>(x[i]);
-        s[i & 1] += w > 0.0 ? w : 0.0;
-      }
+    for (int i = 0; i < kBatch; ++i) {
+      const int j = g + 32 * i + (threadIdx.x & 31);
+      x[i] = j < j1 && (SUB || j != skip) ? Elem<E>::load(row + j) : 0.f;
+      y[i] = SUB && j < j1 ? Elem<E>::load(sub + j) : 0.f;
     }
-    return s[0] + s[1];
+  }
+  // sums of the groups of [j0, j1), `size` elements each (a multiple of kGroup); a batch of loads is ahead of the arithmetic
+  template <bool SUB>
+  __device__ __forceinline__ void sums(int j0, int j1, int size, double* out) const {
+    float x[2][kBatch], y[2][kBatch];
+    load<SUB>(j0, j1, x[0], y[0]);
+    double s = 0.0;
+    int group = 0, end = j0 + size;
+    auto add = [&](int k, int g) {
+      double a[2] = {0.0, 0.0};
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const double w = SUB ? static_cast<double>(x[k][i]) - static_cast<double>(y[k][i]) : static_cast<double>(x[k][i]);
+        a[i & 1] += w > 0.0 ? w : 0.0;
+      }
+      s += a[0] + a[1];
+      if (g + kGroup >= end || g + kGroup >= j1) {
+        s = warp_sum_f64(s);
+        if ((threadIdx.x & 31) == 0) out[group] = s;
+        ++group;
+        end += size;
+        s = 0.0;
+      }
+    };
+    for (int g = j0; g < j1; g += 2 * kGroup) {
+      load<SUB>(g + kGroup, j1, x[1], y[1]);
+      add(0, g);
+      if (g + kGroup >= j1) break;
+      load<SUB>(g + 2 * kGroup, j1, x[0], y[0]);
+      add(1, g + kGroup);
+    }
   }
 };
 
 template <typename E, int C>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 verify_kernel(const __grid_constant__ Verify p) {
   grid_dep_sync();
-  __shared__ double chunk_s[kWarps], total_s;
+  __shared__ double group_s[kWarps][kGroups], chunk_s[kWarps], total_s;
   __shared__ int n_s;
   __shared__ float best_s[kWarps];
   __shared__ int arg_s[kWarps];
@@ -106,14 +127,21 @@ verify_kernel(const __grid_constant__ Verify p) {
   const bool rejected = n < count;
   Weights<E> weight{target + n * p.ts[1], rejected && draft != nullptr ? draft + n * p.ds[1] : nullptr,
                     rejected && draft == nullptr ? tokens[n] : -1};
-  // contiguous chunks, one per warp of the cluster
-  const int per = (p.V + C * kWarps * 32 - 1) / (C * kWarps * 32) * 32;
-  const int j0 = min((rank * kWarps + warp) * per, p.V), j1 = min(j0 + per, p.V);
-  const double s = warp_sum_f64(weight.sub != nullptr ? weight.template sum<true>(j0, j1, lane) : weight.template sum<false>(j0, j1, lane));
+  // contiguous chunks, one per warp of the cluster, of at most kGroups groups
+  const int groups_all = (p.V + kGroup - 1) / kGroup;  // of kGroup elements
+  const int per_groups = (groups_all + C * kWarps - 1) / (C * kWarps), size = (per_groups + kGroups - 1) / kGroups * kGroup;
+  const int per = per_groups * kGroup;
+  const int j0 = static_cast<int>(min(static_cast<int64_t>(rank * kWarps + warp) * per, static_cast<int64_t>(p.V)));
+  const int j1 = static_cast<int>(min(static_cast<int64_t>(j0) + per, static_cast<int64_t>(p.V))), groups = (j1 - j0 + size - 1) / size;
+  if (weight.sub != nullptr) weight.template sums<true>(j0, j1, size, group_s[warp]);
+  else weight.template sums<false>(j0, j1, size, group_s[warp]);
+  __syncwarp();
+  const double s = warp_sum_f64(lane < groups ? group_s[warp][lane] : 0.0);
   if (lane == 0) chunk_s[warp] = s;
   __syncthreads();
   if (tid == 0) {
     double t = 0.0;
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) t += chunk_s[w];
     total_s = t;
   }
@@ -147,35 +175,33 @@ verify_kernel(const __grid_constant__ Verify p) {
     // (a mark that rounding puts behind all sums belongs to the last chunk that has any weight)
     while (w > 0 && !(chunk_s[w] > 0.0)) at -= chunk_s[--w];
     if (warp != w) return;
+    int k = 0;
+    for (; k < groups - 1 && !(at + group_s[w][k] > mark); ++k) at += group_s[w][k];
+    while (k > 0 && !(group_s[w][k] > 0.0)) at -= group_s[w][--k];
     int pick = -1, last = -1;  // last: the last element with weight so far
-    for (int g = j0; g < j1; g += 256) {
-      double x[8], sum = 0.0;
+    const int g1 = min(j0 + (k + 1) * size, j1);
+    for (int g = j0 + k * size; g < g1 && pick < 0; g += kGroup) {
+      double x[kBatch];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kBatch; ++i) {
         const int j = g + i * 32 + lane;
-        x[i] = j < j1 ? weight(j) : 0.0;
-        sum += x[i];
+        x[i] = j < g1 ? weight(j) : 0.0;
       }
-      sum = warp_sum_f64(sum);
-      const bool here = at + sum > mark;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kBatch; ++i) {
         const unsigned some = __ballot_sync(0xffffffffu, x[i] > 0.0);
-        if (some != 0u && pick < 0) last = g + i * 32 + 31 - __clz(some);
-        if (here && pick < 0) {
-          double c = x[i];
+        if (pick >= 0 || some == 0u) continue;
+        last = g + i * 32 + 31 - __clz(some);
+        double c = x[i];
 #pragma unroll
-          for (int k = 1; k < 32; k <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, c, k);
-            if (lane >= k) c += y;
-          }
-          const unsigned over = __ballot_sync(0xffffffffu, at + c > mark && x[i] > 0.0);
-          if (over != 0u) pick = g + i * 32 + __ffs(over) - 1;
-          at += __shfl_sync(0xffffffffu, c, 31);
+        for (int d = 1; d < 32; d <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, c, d);
+          if (lane >= d) c += y;
         }
+        const unsigned over = __ballot_sync(0xffffffffu, at + c > mark && x[i] > 0.0);
+        if (over != 0u) pick = g + i * 32 + __ffs(over) - 1;
+        at += __shfl_sync(0xffffffffu, c, 31);
       }
-      if (pick >= 0 || here) break;
-      at += sum;
     }
     if (lane == 0) out[n] = pick >= 0 ? pick : max(last, 0);
     return;
@@ -209,9 +235,9 @@ verify_kernel(const __grid_constant__ Verify p) {
 
 template <typename E>
 void launch_verify(const Verify& p, int64_t batch, cudaStream_t st) {
-  // as many blocks per sequence as leave four for each SM, each with a slice worth a few rounds of its threads
+  // as many blocks per sequence as leave about seven for each SM, each with a slice worth a round of its warps
   unsigned c = 8;
-  while (c > 1 && (batch * c > 4 * kNumSMs || p.V < static_cast<int64_t>(c) * kThreads * 2)) c /= 2;
+  while (c > 1 && (batch * c > 7 * kNumSMs || p.V < static_cast<int64_t>(c) * kWarps * kGroup)) c /= 2;
   const dim3 grid(static_cast<unsigned>(batch) * c);
   switch (c) {
     case 8: launch_cluster_k(verify_kernel<E, 8>, grid, kThreads, 8, 0, st, p); break;
