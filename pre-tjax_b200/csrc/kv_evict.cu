@@ -338,14 +338,17 @@ extern "C" int ptj_kv_evict(const ptj_kv_cache* cache, const int32_t* dst_table,
   const int segs = static_cast<int>(cache->batch * cache->kv_heads);
   p.pools_in_place = in_place;
   p.weights_in_place = weights_out == weights;
-  // In place: columns of 32 bytes. Else whole rows, in stretches of one round each.
+  // In place: columns of 32 bytes. Else whole rows, in stretches of a few rounds.
   p.per_col = in_place ? static_cast<int>(32 / piece) : p.pieces;
   if (p.per_col > p.pieces) p.per_col = p.pieces;
   p.cols = static_cast<int>(ceil_div(p.pieces, p.per_col));
   p.round = kMoveThreads * kMovePieces / p.per_col;
   if (p.round > kMoveRows) p.round = kMoveRows;
-  p.chunk = p.round;
-  if (ceil_div(most, p.chunk) > 65535) p.chunk = static_cast<int>(ceil_div(ceil_div(most, 65535), p.round)) * p.round;
+  // rounds of a block: so many that all blocks are resident (two per SM) where the rows are that many
+  const int64_t rounds = ceil_div(most, p.round), least = ceil_div(rounds, 65535);
+  int64_t each = ceil_div(rounds * segs, 2 * kNumSMs);
+  each = each < 1 ? 1 : (each > 16 ? 16 : each);
+  p.chunk = static_cast<int>((each > least ? each : least) * p.round);
   p.chunks = static_cast<int>(ceil_div(most, p.chunk));
   const bool one = in_place && (weights_out == weights || !weights_out);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -235,9 +235,9 @@ verify_kernel(const __grid_constant__ Verify p) {
 
 template <typename E>
 void launch_verify(const Verify& p, int64_t batch, cudaStream_t st) {
-  // as many blocks per sequence as leave about seven for each SM, each with a slice worth a round of its warps
+  // as many blocks per sequence as are resident at once (four per SM), each with a slice worth a round of its warps
   unsigned c = 8;
-  while (c > 1 && (batch * c > 7 * kNumSMs || p.V < static_cast<int64_t>(c) * kWarps * kGroup)) c /= 2;
+  while (c > 1 && (batch * c > 4 * kNumSMs || p.V < static_cast<int64_t>(c) * kWarps * kGroup)) c /= 2;
   const dim3 grid(static_cast<unsigned>(batch) * c);
   switch (c) {
     case 8: launch_cluster_k(verify_kernel<E, 8>, grid, kThreads, 8, 0, st, p); break;
