@@ -190,3 +190,33 @@ def test_library_refuses_on_its_own():
         assert verify(**kw) == -1, kw
     assert verify(dt=9) == -3
     assert lib.ptj_launch_count() == before
+
+
+def test_cache_and_speculation_refusals():
+    """What serving refuses before it touches a device."""
+    sv, gpt2 = pkg("serving"), pkg("gpt2")
+    cfg = gpt2.GPT2Config(vocab=10, dim=8, layers=1, heads=2, ffn=16, seq=32)
+    for kw in (dict(batch=0), dict(batch=1, capacity=0), dict(batch=1, page_size=0)):
+        with pytest.raises(ValueError):
+            sv.PagedCache(cfg, device="cpu", **kw)
+    c = sv.PagedCache(cfg, 2, capacity=20, page_size=16, device="cpu")
+    assert tuple(c.page_table.shape) == (2, 2) and c.k.shape == (1, 4, 2, 16, 4)
+    with pytest.raises(RuntimeError, match="track_weights"):
+        c.evict(4, 2)
+    with pytest.raises(ValueError, match="sequences for a cache"):
+        sv.decode_step((cfg, None), torch.zeros(3, 1, dtype=I32), c)
+    with pytest.raises(ValueError, match="another model"):
+        sv.decode_step((gpt2.GPT2Config(vocab=10, dim=16, layers=1, heads=2, ffn=16, seq=32), None), torch.zeros(2, 1, dtype=I32), c)
+
+
+@pytest.mark.parametrize("change", [dict(drafts=0), dict(uniforms=torch.zeros(4, 2, 4)), dict(uniforms=torch.zeros(4, 3, 10)),
+                                    dict(new_tokens=40), dict(budget=3, recent=4)])
+def test_speculation_refusals(change, monkeypatch):
+    sv, gpt2 = pkg("serving"), pkg("gpt2")
+    cfg = gpt2.GPT2Config(vocab=10, dim=8, layers=1, heads=2, ffn=16, seq=32)
+    monkeypatch.setattr(sv, "_weights", lambda params, dtype, p=None: (cfg, None))
+    args = dict(params=[[torch.zeros(1)]], draft_params=[[torch.zeros(1)]], prompt=torch.zeros(2, 5, dtype=I32), new_tokens=8,
+                uniforms=torch.zeros(4, 2, 10), drafts=4)
+    args.update(change)
+    with pytest.raises(ValueError):
+        sv.speculate(**args)
