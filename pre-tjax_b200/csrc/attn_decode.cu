@@ -7,6 +7,7 @@ namespace {
 
 constexpr int kMaxRows = 4096;      // query rows of a key head
 constexpr int kLeastKeys = 64;      // keys that a stretch of the list has at least
+constexpr int kMostPieces = 1024;   // pieces of a sequence of the capacity's length, about
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
@@ -128,7 +129,9 @@ extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* 
   d.workers = pl.workers;
   d.small = pl.small;
   const bool tc = cache->dtype == PTJ_BF16 && cache->d_head <= 128;
-  d.least = kLeastKeys / (tc ? 16 : 4096 / (pl.dim * pl.es));
+  const int ks = tc ? 16 : 4096 / (pl.dim * pl.es);
+  const int64_t share = ceil_div(ceil_div(d.rows.capacity, ks), kMostPieces);  // (few segments: a row is not joined from thousands of pieces)
+  d.least = static_cast<int>(share > kLeastKeys / ks ? share : kLeastKeys / ks);
   d.wide = paged_rows_aligned(*cache);
   if (d.kn && d.wide && !(view_aligned(tokens->k, tokens->k_strides, *cache, Hk, T) && view_aligned(tokens->v, tokens->v_strides, *cache, Hk, T))) {
     const int rc2 = ptj_kv_append(cache, tokens, stream);  // new rows that cannot be read 16 bytes at a time

@@ -135,10 +135,10 @@ struct Fetcher {
   static constexpr int PIECES = RB / 16, ROWS = PIECES >= 32 ? 1 : 32 / PIECES, COLS = PIECES >= 32 ? PIECES / 32 : 1;
   int row0, c0;   // this lane's first row and piece
   uint32_t to;    // its place in a step
-  bool dense;     // a step's rows lie one behind the other in one page
+  bool dense;     // a step's rows lie in one page
   // Pages of 32 steps to come, one per lane: a look-up in front of every step would be the longest wait of all (800 cycles).
   int ids, base;  // base: the first of them, counted in steps that this warp takes
-  const char *k, *v;  // this lane's place in slot 0 of page 0 of the key head
+  const char *k, *v;  // this lane's place in slot row0 of page 0 of the key head
   __device__ __forceinline__ void look_up(const DecodeAttn& p, const int32_t* table, int sub, int stride, int number) {
     const int page = p.rows.page_of((sub + (threadIdx.x & 31) * stride) * KS);
     ids = page < p.rows.capacity_pages ? table[page] : -1;
@@ -149,11 +149,11 @@ struct Fetcher {
     row0 = PIECES >= 32 ? 0 : lane / PIECES;
     c0 = PIECES >= 32 ? lane : lane % PIECES;
     to = row0 * RB + ((c0 ^ swizzle(row0)) << 4);
-    dense = p.wide && p.rows.page_size % KS == 0 && p.rows.slot_stride[0] == RB && p.rows.slot_stride[1] == RB;
+    dense = p.wide && p.rows.page_size % KS == 0;
   }
   __device__ __forceinline__ void set_head(const DecodeAttn& p, int h) {
-    k = p.k + p.rows.offset(0, 0, h, 0) + (row0 * RB + c0 * 16);
-    v = p.v + p.rows.offset(1, 0, h, 0) + (row0 * RB + c0 * 16);
+    k = p.k + p.rows.offset(0, 0, h, row0) + c0 * 16;
+    v = p.v + p.rows.offset(1, 0, h, row0) + c0 * 16;
   }
   // Number of a sequence's first steps that are dense and hold no new key.
   __device__ __forceinline__ int plain_steps(const Segment& sg) const { return dense ? max(sg.first, 0) / KS : 0; }
@@ -165,17 +165,21 @@ struct Fetcher {
     const int j0 = sub * KS;
     const int slot = p.rows.page_shift >= 0 ? j0 & (p.rows.page_size - 1) : j0 - p.rows.page_of(j0) * p.rows.page_size;
     if ((threadIdx.x & 31) == 0) *present_word<KS, RB>(stage) = (1u << KS) - 1u;
-    const char *kr = k + (page * p.rows.page_stride[0] + slot * RB), *vr = v + (page * p.rows.page_stride[1] + slot * RB);
+    const char *kr = k + (page * p.rows.page_stride[0] + slot * p.rows.slot_stride[0]);
+    const char *vr = v + (page * p.rows.page_stride[1] + slot * p.rows.slot_stride[1]);
+    const int64_t ks = ROWS * p.rows.slot_stride[0], vs = ROWS * p.rows.slot_stride[1];
     const uint32_t at = tc::smem_u32(stage);
 #pragma unroll
-    for (int x = 0; x < COLS; ++x) {
-      if ((c0 + 32 * x) * 16 >= p.rows.row_bytes) continue;  // (zero from the start)
+    for (int i = 0; i < KS; i += ROWS) {
 #pragma unroll
-      for (int i = 0; i < KS; i += ROWS) {
+      for (int x = 0; x < COLS; ++x) {
+        if ((c0 + 32 * x) * 16 >= p.rows.row_bytes) continue;  // (zero from the start)
         const uint32_t dst = at + ((to ^ (swizzle(i) << 4)) + i * RB + 512 * x);
-        copy16(dst, kr + i * RB + 512 * x);
-        copy16(dst + KS * RB, vr + i * RB + 512 * x);
+        copy16(dst, kr + 512 * x);
+        copy16(dst + KS * RB, vr + 512 * x);
       }
+      kr += ks;
+      vr += vs;
     }
     return true;
   }

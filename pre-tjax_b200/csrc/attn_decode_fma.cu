@@ -1,7 +1,9 @@
 // Attention of new tokens over a paged cache on CUDA cores, float32 arithmetic: float32 caches and bf16 heads beyond 128.
 //
-// LPK lanes share a key, 16 bytes of the row each, NV times; 32 / LPK keys stand side by side. A row of queries costs a product per
-// element and key twice and log2(LPK) shuffles per key; up to eight rows stay under what memory delivers (4 bytes an element).
+// LPK lanes share a key, 16 bytes of the row each, NV times; 32 / LPK keys stand side by side, KB one behind the other. The lanes'
+// parts of KB scores are added with every lane giving half of what it holds away at each exchange: KB - 1 + log2(LPK / KB) shuffles
+// for KB scores, after which a lane has one of them, its exponential costs one instruction for all, and KB broadcasts bring them
+// back for the products with the values.
 #include "attn_decode.cuh"
 
 namespace ptj {
@@ -12,6 +14,7 @@ struct CoreFma {
   static constexpr int VEC = 16 / static_cast<int>(sizeof(E)), kDim = DP, kRowBytes = DP * static_cast<int>(sizeof(E)), kRows = RB;
   static constexpr int LPK = DP / VEC < 32 ? DP / VEC : 32, NV = DP / (VEC * LPK), KPW = 32 / LPK, W = VEC * NV;
   static constexpr int KS = 4096 / kRowBytes, KB = KS / KPW;  // keys of a step, of a lane
+  static constexpr int REP = LPK / KB;                        // lanes that end with the same score
   static constexpr int kDepth = 3;
   static constexpr int kBlocks = 2;
   float q[RB][W], o[RB][W];
@@ -77,29 +80,26 @@ struct CoreFma {
 #pragma unroll
         for (int i = 0; i < W; ++i) s[e] = fmaf(q[r][i], k[e][i], s[e]);
       }
+      // to one score per lane: that of key `own`
 #pragma unroll
-      for (int x = LPK / 2; x > 0; x >>= 1)
+      for (int n = KB / 2, x = LPK / 2; x > 0; n /= 2, x /= 2) {
+        if (n > 0) {
+          const bool up = sub_lane & x;
 #pragma unroll
-        for (int e = 0; e < KB; ++e) s[e] += __shfl_xor_sync(0xffffffffu, s[e], x);
-      if (edge) {
-#pragma unroll
-        for (int e = 0; e < KB; ++e)
-          if (!((present >> (e * KPW + grp)) & 1u) || j0 + e * KPW + grp > limit[r]) s[e] = -INFINITY;
+          for (int e = 0; e < n; ++e) {
+            const float give = up ? s[e] : s[e + n], stay = up ? s[e + n] : s[e];
+            s[e] = stay + __shfl_xor_sync(0xffffffffu, give, x);
+          }
+        } else {
+          s[0] += __shfl_xor_sync(0xffffffffu, s[0], x);
+        }
       }
-      bool moves = false;
-#pragma unroll
-      for (int e = 0; e < KB; ++e) moves |= s[e] > over[r];
-      if (p.scores != nullptr && sub_lane == 0) {
-        float* to = sg.score_row(p, row) + j0 + grp;
-#pragma unroll
-        for (int e = 0; e < KB; ++e)
-          if (j0 + e * KPW + grp < sg.n) to[e * KPW] = s[e] * p.scale;
-      }
-      if (__any_sync(0xffffffffu, moves)) {
-        float m = s[0];
-#pragma unroll
-        for (int e = 1; e < KB; ++e) m = fmaxf(m, s[e]);
-        m = fmaxf(warp_max(m) * p.scale, ref[r]);
+      const int own = sub_lane / REP * KPW + grp;  // place in the step
+      float mine = s[0];
+      if (edge && (!((present >> own) & 1u) || j0 + own > limit[r])) mine = -INFINITY;
+      if (p.scores != nullptr && sub_lane % REP == 0 && j0 + own < sg.n) sg.score_row(p, row)[j0 + own] = mine * p.scale;
+      if (__any_sync(0xffffffffu, mine > over[r])) {
+        const float m = fmaxf(warp_max(mine) * p.scale, ref[r]);
         const float f = rebase(ref[r], m);
         ref[r] = m;
         over[r] = (m + kDecLazy) * p.unscale;
@@ -107,11 +107,10 @@ struct CoreFma {
 #pragma unroll
         for (int i = 0; i < W; ++i) o[r][i] *= f;
       }
+      mine = ex2(fmaf(mine, p.scale, -ref[r]));
+      sum[r] += mine;
 #pragma unroll
-      for (int e = 0; e < KB; ++e) {
-        s[e] = ex2(fmaf(s[e], p.scale, -ref[r]));
-        sum[r] += s[e];
-      }
+      for (int e = 0; e < KB; ++e) s[e] = __shfl_sync(0xffffffffu, mine, e * REP, LPK);
       if (edge) {  // zero times what is not finite is not zero
 #pragma unroll
         for (int e = 0; e < KB; ++e) {
@@ -133,10 +132,9 @@ struct CoreFma {
   __device__ __forceinline__ void emit(F&& f) {
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      float l = sum[r];
+      const float l = warp_sum(sum[r]) * (1.f / REP);
 #pragma unroll
       for (int x = LPK; x < 32; x <<= 1) {
-        l += __shfl_xor_sync(0xffffffffu, l, x);
 #pragma unroll
         for (int i = 0; i < W; ++i) o[r][i] += __shfl_xor_sync(0xffffffffu, o[r][i], x);
       }
