@@ -421,7 +421,8 @@ typedef struct {
   const void *q, *k, *v;                       /* k, v: NULL where the cache holds the new rows already */
   void* out;
   const int32_t* counts;
-  int64_t heads, tokens;                       /* heads: a multiple of kv_heads; query head i reads key head i / (heads / kv_heads) */
+  int64_t heads, tokens;                       /* heads: a multiple of kv_heads; query head i reads key head i / (heads / kv_heads);
+                                                  at most 4096 query rows (heads / kv_heads * tokens) per key head */
   int64_t q_strides[3], o_strides[3], k_strides[3], v_strides[3];
 } ptj_new_tokens;
 /* Writes the rows k, v of the new tokens into their pages; positions below 0 (a count above the length) are left out. */
@@ -429,7 +430,7 @@ int ptj_kv_append(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, void*
 /* Attention of the new tokens over the cache, evaluation semantics (the output is multiplied by 1 - p):
  *   out = (1 - p) softmax(q K^T / sqrt(d_head)) V over keys 0 .. position of the token.
  * With tokens->k and ->v the new rows are written to their pages as by ptj_kv_append and attended to. A token behind counts[b]
- * or below position 0 attends nothing: a zero row. Rows read only the keys they attend: what lies in other slots, an infinity
+ * or below position 0 attends nothing: a zero row. out overlaps no input. Rows read only the keys they attend: what lies in other slots, an infinity
  * or a NaN included, reaches no output. Softmax statistics and sums are float32.
  * weights_out (optional, float[batch, kv_heads, weights_ld], weights_ld >= table_width * page_size): the attention that each
  * key received, summed over the query heads of its key head and the new tokens, plus weights (same layout; NULL = 0; may be
@@ -442,7 +443,8 @@ int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, flo
  * (recent <= budget) and of the others those with the largest weights (float[batch, kv_heads, weights_ld], weights_ld >=
  * table_width * page_size), the lowest positions among equals; a NaN ranks below everything. Keys stay in order: key kept[i]
  * becomes key i of dst_table (rows of dst_ld entries; dst_table == cache->table: in place). Other sequences are only copied
- * to dst_table. Destination pages of different sequences differ, and unless in place they are no source pages.
+ * to dst_table. Destination pages of different sequences differ. In place is what the address says: a copy of cache->table, or
+ * any other table that names a source page, is an error that is not noticed, since rows then move in no order.
  *   kept         int32[batch, kv_heads, budget]: positions that stay, -1 behind them
  *   new_lengths  int32[batch]: min(lengths, budget); not the array `lengths`
  *   weights_out  float[batch, kv_heads, weights_out_ld]: weights of the kept keys (may be weights itself, with its leading

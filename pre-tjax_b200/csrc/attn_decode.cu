@@ -85,11 +85,11 @@ extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* 
   const DecodePlan pl = make_plan(*cache, *tokens, d.rows, weights_out != nullptr);
   const int64_t Hk = cache->kv_heads, T = tokens->tokens, R = tokens->heads / Hk * T;
   if (cache->batch * Hk * R > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
-  if (ptj_device_check() != PTJ_OK || (d.rows.fault = tc::fault_word()) == nullptr) return PTJ_ERR_DEVICE;
   if (pl.bytes() > 0) {
     if (!workspace || workspace_bytes < pl.bytes()) return PTJ_ERR_WORKSPACE;
     if (!aligned16(workspace)) return PTJ_ERR_MISALIGNED;
   }
+  if (ptj_device_check() != PTJ_OK || (d.rows.fault = tc::fault_word()) == nullptr) return PTJ_ERR_DEVICE;
   d.lengths = cache->lengths;
   d.counts = tokens->counts;
   d.q = static_cast<const char*>(tokens->q);

@@ -17,7 +17,8 @@ struct CoreFma {
   static constexpr int REP = LPK / KB;                        // lanes that end with the same score
   static constexpr int kDepth = 3;
   static constexpr int kBlocks = 2;
-  float q[RB][W], o[RB][W];
+  static constexpr int P = W / 2;  // pairs of elements: products run two elements wide
+  uint64_t q[RB][P], o[RB][P];
   float ref[RB], sum[RB], over[RB];  // over: scores beyond it (not scaled) move the reference
   int limit[RB];  // last keys that the rows attend
   int sub_lane, grp;
@@ -34,7 +35,7 @@ struct CoreFma {
       over[r] = -INFINITY;
       sum[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) q[r][i] = o[r][i] = 0.f;
+      for (int i = 0; i < P; ++i) q[r][i] = o[r][i] = 0ull;  // (two zeros)
       const int row = sg.rb * kRows + r;
       limit[r] = sg.limit(p, row);
       if (limit[r] < 0) continue;
@@ -42,20 +43,22 @@ struct CoreFma {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (elem(i) + e < p.D) q[r][i * VEC + e] = Elem<E>::load(src + elem(i) + e);
+        for (int e = 0; e < VEC; e += 2) {
+          const int d = elem(i) + e;
+          q[r][(i * VEC + e) / 2] = f2_pack(d < p.D ? Elem<E>::load(src + d) : 0.f, d + 1 < p.D ? Elem<E>::load(src + d + 1) : 0.f);
+        }
     }
   }
 
-  __device__ __forceinline__ void read(const uint8_t* stage, int r, float (&out)[W]) const {
+  __device__ __forceinline__ void read(const uint8_t* stage, int r, uint64_t (&out)[P]) const {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const uint4 x = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + (((i * LPK + sub_lane) ^ swizzle(r % KS)) << 4));
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if constexpr (sizeof(E) == 4) out[i * VEC + e] = __uint_as_float(w[e]);
-        else out[i * VEC + e] = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+      for (int e = 0; e < VEC / 2; ++e) {
+        if constexpr (sizeof(E) == 4) out[i * VEC / 2 + e] = f2_pack(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+        else out[i * VEC / 2 + e] = f2_pack(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
       }
     }
   }
@@ -64,7 +67,7 @@ struct CoreFma {
     const int j0 = sub * KS;
     const uint32_t present = present_keys<KS, kRowBytes>(stage);
     const bool edge = j0 + KS > sg.first + 1 || present != (1u << KS) - 1u;  // some rows do not attend all of its keys
-    float k[KB][W], v[KB][W];
+    uint64_t k[KB][P], v[KB][P];
 #pragma unroll
     for (int e = 0; e < KB; ++e) read(stage, e * KPW + grp, k[e]);
 #pragma unroll
@@ -76,9 +79,12 @@ struct CoreFma {
       float s[KB];
 #pragma unroll
       for (int e = 0; e < KB; ++e) {
-        s[e] = 0.f;
+        uint64_t d = f2_mul(q[r][0], k[e][0]);
 #pragma unroll
-        for (int i = 0; i < W; ++i) s[e] = fmaf(q[r][i], k[e][i], s[e]);
+        for (int i = 1; i < P; ++i) d = f2_fma(q[r][i], k[e][i], d);
+        float lo, hi;
+        f2_unpack(d, lo, hi);
+        s[e] = lo + hi;
       }
       // to one score per lane: that of key `own`
 #pragma unroll
@@ -105,7 +111,7 @@ struct CoreFma {
         over[r] = (m + kDecLazy) * p.unscale;
         sum[r] *= f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[r][i] *= f;
+        for (int i = 0; i < P; ++i) o[r][i] = f2_mul(o[r][i], f2_pack(f, f));
       }
       mine = ex2(fmaf(mine, p.scale, -ref[r]));
       sum[r] += mine;
@@ -116,13 +122,13 @@ struct CoreFma {
         for (int e = 0; e < KB; ++e) {
           if (j0 + e * KPW + grp > limit[r]) continue;
 #pragma unroll
-          for (int i = 0; i < W; ++i) o[r][i] = fmaf(s[e], v[e][i], o[r][i]);
+          for (int i = 0; i < P; ++i) o[r][i] = f2_fma(f2_pack(s[e], s[e]), v[e][i], o[r][i]);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < KB; ++e)
 #pragma unroll
-          for (int i = 0; i < W; ++i) o[r][i] = fmaf(s[e], v[e][i], o[r][i]);
+          for (int i = 0; i < P; ++i) o[r][i] = f2_fma(f2_pack(s[e], s[e]), v[e][i], o[r][i]);
       }
     }
   }
@@ -134,14 +140,17 @@ struct CoreFma {
     for (int r = 0; r < RB; ++r) {
       const float l = warp_sum(sum[r]) * (1.f / REP);
 #pragma unroll
-      for (int x = LPK; x < 32; x <<= 1) {
+      for (int x = LPK; x < 32; x <<= 1)
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[r][i] += __shfl_xor_sync(0xffffffffu, o[r][i], x);
-      }
+        for (int i = 0; i < P; ++i) o[r][i] = f2_add(o[r][i], __shfl_xor_sync(0xffffffffu, o[r][i], x));
       if (grp == 0)
 #pragma unroll
-        for (int i = 0; i < W; i += 4)
-          f(r, elem(i / VEC) + i % VEC, make_float4(o[r][i], o[r][i + 1], o[r][i + 2], o[r][i + 3]), ref[r], l, sub_lane == 0 && i == 0);
+        for (int i = 0; i < W; i += 4) {
+          float4 x;
+          f2_unpack(o[r][i / 2], x.x, x.y);
+          f2_unpack(o[r][i / 2 + 1], x.z, x.w);
+          f(r, elem(i / VEC) + i % VEC, x, ref[r], l, sub_lane == 0 && i == 0);
+        }
     }
   }
 };

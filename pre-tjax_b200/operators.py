@@ -618,7 +618,8 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, cou
     i reads key head i // (H / kv_heads). The output is multiplied by 1 - p (default DROPOUT_RATE), as everywhere in evaluation.
     weights float32 [B, kv_heads, capacity]: the attention that every key received so far; the call adds its own, summed over
     the query heads of a key head and the new tokens, into weights_out (default: weights; weights None counts as zeros). What
-    weights holds for new keys does not matter. workspace: optional uint8 tensor, see ptj_attn_decode_workspace_bytes."""
+    weights holds for new keys does not matter. out overlaps no input; H / kv_heads * T <= 4096. workspace: optional uint8 tensor,
+    see ptj_attn_decode_workspace_bytes."""
     _on_current_device(q, k_pages, v_pages, page_table, lengths, k, v, counts, weights, weights_out, out, workspace)
     cache, sizes = _kv_cache(k_pages, v_pages, page_table, lengths)
     if out is None:
@@ -657,7 +658,8 @@ def kv_evict(k_pages, v_pages, page_table, lengths, weights, budget, recent=0, *
     the others those with the largest accumulated weights (attn_decode), the lowest positions among equals (a NaN ranks below
     everything). Returns (kept int32 [B, kv_heads, budget]: positions that stayed, in order, -1 behind them; new lengths
     int32 [B]). The kept rows become rows 0 .. of the pages of dst_table (default: page_table, in place), which also get
-    the sequences that are short enough; their weights become the first ones of weights_out (default: weights)."""
+    the sequences that are short enough; their weights become the first ones of weights_out (default: weights). Another table than
+    page_table itself names none of its pages: rows then move in no order."""
     _on_current_device(k_pages, v_pages, page_table, lengths, weights, dst_table, weights_out)
     cache, sizes = _kv_cache(k_pages, v_pages, page_table, lengths)
     B, Hk, _, page_size, capacity = sizes

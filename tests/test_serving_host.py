@@ -176,6 +176,13 @@ def test_library_refuses_on_its_own():
         assert call(good(), new(**kw)) == -1, kw
     assert call(good(), new(), p=1.1) == -1 and call(good(), new(), w=16, wo=None) == -1
     assert call(good(), new(), wo=16, ld=31) == -1
+    long = dict(table_width=4096, table_ld=4096, batch=1, kv_heads=1)
+    need = lib.ptj_attn_decode_workspace_bytes(ctypes.byref(good(**long)), ctypes.byref(new(heads=1)), 0)
+    assert need > 0 and call(good(**long), new(heads=1)) == -5
+    assert lib.ptj_attn_decode(ctypes.byref(good(**long)), ctypes.byref(new(heads=1)), 0.1, None, None, 0, 16, need - 1, None) == -5
+    assert lib.ptj_attn_decode(ctypes.byref(good(**long)), ctypes.byref(new(heads=1)), 0.1, None, None, 0, 24, need, None) == -2
+    assert lib.ptj_attn_decode_workspace_bytes(None, None, 0) == 0
+    assert call(good(kv_heads=1), new(heads=4097)) == -1  # query rows of a key head
     assert lib.ptj_kv_append(ctypes.byref(good()), ctypes.byref(new()), None) == -1
     evict = lambda dst=16, width=1, ld=1, budget=8, recent=0, w=16, wld=32, wo=16, wold=32, kept=16, nl=32: lib.ptj_kv_evict(
         ctypes.byref(good()), dst, width, ld, budget, recent, w, wld, wo, wold, kept, nl, None)
