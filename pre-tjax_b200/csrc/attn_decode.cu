@@ -9,14 +9,22 @@ constexpr int kMaxRows = 4096;      // query rows of a key head
 constexpr int kLeastKeys = 64;      // keys that a stretch of the list has at least
 constexpr int kMostPieces = 1024;   // pieces of a sequence of the capacity's length, about
 
+constexpr int kManyRows = 16;       // query rows of a key head beyond which the tcgen05 kernel takes over
+
+bool new_rows_aligned(const ptj_kv_cache& c, const ptj_new_tokens& t) {
+  return !t.k || (view_aligned(t.k, t.k_strides, c, c.kv_heads, t.tokens) && view_aligned(t.v, t.v_strides, c, c.kv_heads, t.tokens));
+}
+
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
-DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const PagedRows& rows, bool weights) {
+// aligned: rows of pools and new tokens are whole 16-byte pieces on 16-byte boundaries
+DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const PagedRows& rows, bool weights, bool aligned) {
   DecodePlan pl = {};
   const int R = static_cast<int>(t.heads / c.kv_heads * t.tokens);
   pl.es = static_cast<int>(dtype_size(c.dtype));
   const bool tc = c.dtype == PTJ_BF16 && c.d_head <= 128;
   pl.dim = c.d_head <= 64 && (tc || pl.es == 4) ? 64 : (c.d_head <= 128 && (tc || pl.es == 4) ? 128 : 256);
+  pl.wide = tc && R > kManyRows && aligned;
   // the core with the fewest blocks of rows (each reads the keys and values again, mostly from L2), of those the smallest
   if (tc) {
     const int most = pl.dim == 64 ? 32 : 24;
@@ -29,10 +37,11 @@ DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const Paged
     const int need = static_cast<int>(ceil_div(R, pl.nrb));
     pl.rows = need <= 1 ? 1 : (need <= 4 ? 4 : most);
   }
+  if (pl.wide) pl.rows = 32;
   pl.nrb = static_cast<int>(ceil_div(R, pl.rows));
   pl.prows = R < pl.rows ? R : pl.rows;
   const int64_t segs = c.batch * c.kv_heads * pl.nrb;
-  const int ks = tc ? 16 : 4096 / (pl.dim * pl.es);  // keys of a step
+  const int ks = pl.wide ? 128 : (tc ? 16 : 4096 / (pl.dim * pl.es));  // keys of a step
   const int64_t longest = ceil_div(rows.capacity, ks);
   // A cluster per segment, of as many blocks as all fit on the GPU at once and have a step for each of their warps (more come in
   // a second round: 16 x 12 float32 caches of 512 keys 15.5 us with one block each, 22.3 with two; 8 x 12 bf16 caches of 1024 with
@@ -42,12 +51,12 @@ DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const Paged
   pl.cluster = 1;
   while (pl.cluster < 8 && segs * pl.cluster * 2 <= per_sm * kNumSMs && longest > kDecWarps * pl.cluster) pl.cluster *= 2;
   const int64_t most = ceil_div(longest, kDecWarps * pl.cluster);  // steps of a warp
-  pl.split = most > 64 || (most > 16 && segs * pl.cluster < kNumSMs) || (weights && pl.nrb > 1);
+  pl.split = pl.wide || most > 64 || (most > 16 && segs * pl.cluster < kNumSMs) || (weights && pl.nrb > 1);
   if (pl.split) {
-    pl.workers = per_sm * kNumSMs * kDecWarps;
+    pl.workers = pl.wide ? decode_wide_blocks() * kNumSMs : per_sm * kNumSMs * kDecWarps;
     // small stretches: where sequences may be long enough for 32 steps of a warp, and pieces of a few rows are small beside them
     const int64_t steps = segs * longest;
-    pl.small = c.batch <= kDecDynamicBatch && pl.prows <= 8 && steps >= 32ll * pl.workers ? pl.workers : 0;
+    pl.small = !pl.wide && c.batch <= kDecDynamicBatch && pl.prows <= 8 && steps >= 32ll * pl.workers ? pl.workers : 0;
     const size_t pieces = static_cast<size_t>(pl.workers + pl.small) * 2 * pl.prows;
     pl.part = pieces * pl.dim * 4;
     pl.part_ml = round16(pieces * 8);
@@ -73,7 +82,10 @@ using namespace ptj;
 extern "C" size_t ptj_attn_decode_workspace_bytes(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, int with_weights) {
   PagedRows rows;
   if (check_decode(cache, tokens, rows) != PTJ_OK) return 0;
-  return make_plan(*cache, *tokens, rows, with_weights != 0).bytes();
+  // (the size goes by sizes alone, so that a caller can keep it)
+  const size_t a = make_plan(*cache, *tokens, rows, with_weights != 0, true).bytes();
+  const size_t b = make_plan(*cache, *tokens, rows, with_weights != 0, false).bytes();
+  return a > b ? a : b;
 }
 
 extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, float p, const float* weights,
@@ -82,7 +94,7 @@ extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* 
   const int rc = check_decode(cache, tokens, d.rows);
   if (rc != PTJ_OK) return rc;
   if (!(p >= 0.f && p <= 1.f) || (weights && !weights_out) || (weights_out && weights_ld < d.rows.capacity)) return PTJ_ERR_BAD_SHAPE;
-  const DecodePlan pl = make_plan(*cache, *tokens, d.rows, weights_out != nullptr);
+  const DecodePlan pl = make_plan(*cache, *tokens, d.rows, weights_out != nullptr, paged_rows_aligned(*cache) && new_rows_aligned(*cache, *tokens));
   const int64_t Hk = cache->kv_heads, T = tokens->tokens, R = tokens->heads / Hk * T;
   if (cache->batch * Hk * R > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
   if (pl.bytes() > 0) {
@@ -129,11 +141,11 @@ extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* 
   d.workers = pl.workers;
   d.small = pl.small;
   const bool tc = cache->dtype == PTJ_BF16 && cache->d_head <= 128;
-  const int ks = tc ? 16 : 4096 / (pl.dim * pl.es);
+  const int ks = pl.wide ? 128 : (tc ? 16 : 4096 / (pl.dim * pl.es));
   const int64_t share = ceil_div(ceil_div(d.rows.capacity, ks), kMostPieces);  // (few segments: a row is not joined from thousands of pieces)
-  d.least = static_cast<int>(share > kLeastKeys / ks ? share : kLeastKeys / ks);
+  d.least = static_cast<int>(share > kLeastKeys / ks ? share : (kLeastKeys / ks > 1 ? kLeastKeys / ks : 1));
   d.wide = paged_rows_aligned(*cache);
-  if (d.kn && d.wide && !(view_aligned(tokens->k, tokens->k_strides, *cache, Hk, T) && view_aligned(tokens->v, tokens->v_strides, *cache, Hk, T))) {
+  if (d.kn && d.wide && !new_rows_aligned(*cache, *tokens)) {
     const int rc2 = ptj_kv_append(cache, tokens, stream);  // new rows that cannot be read 16 bytes at a time
     if (rc2 != PTJ_OK) return rc2;
     d.kn = d.vn = nullptr;
@@ -141,5 +153,6 @@ extern "C" int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* 
   d.q_wide = view_aligned(tokens->q, tokens->q_strides, *cache, tokens->heads, T);
   d.out_wide = cache->d_head % 4 == 0 && view_aligned(tokens->out, tokens->o_strides, *cache, tokens->heads, T);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (pl.wide) return launch_decode_wide(d, pl, st);
   return tc ? launch_decode_tc(d, pl, st) : launch_decode_fma(d, pl, st);
 }

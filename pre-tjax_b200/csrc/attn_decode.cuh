@@ -53,7 +53,7 @@ struct DecodeAttn {
 struct DecodePlan {
   int rows, dim, es;   // of a core: block rows, padded head, bytes of an element
   int nrb, prows;
-  bool split;
+  bool split, wide;    // wide: many rows, attn_decode_wide.cu
   int cluster;         // blocks per segment
   int workers, small;
   size_t part, part_ml, ml, starts, scores;  // bytes
@@ -62,8 +62,10 @@ struct DecodePlan {
 // blocks that an SM holds of the core that takes these
 int decode_tc_blocks(int dim, int rows);
 int decode_fma_blocks();
+int decode_wide_blocks();
 int launch_decode_tc(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st);
 int launch_decode_fma(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st);
+int launch_decode_wide(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st);
 
 namespace {
 
@@ -868,6 +870,25 @@ bool set_smem(K kernel, int bytes) {
   return false;
 }
 
+// Joins the pieces that the stretches left and, where they are wanted, forms the weights.
+template <typename E, typename Core>
+int launch_join(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
+  // warps that join a row: by the pieces to be expected of a segment
+  const int64_t rows = static_cast<int64_t>(d.B) * d.Hk * d.R, pieces = (d.workers + d.small) / (static_cast<int64_t>(d.B) * d.Hk * d.nrb);
+  const int wpr = pieces <= 3 ? 1 : (pieces <= 32 ? 4 : 16), threads = wpr == 16 ? 512 : kDecJoinThreads;
+  const int64_t blocks = ceil_div(rows * wpr * 32, threads);
+  if (blocks > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
+  const auto join = wpr == 1 ? attn_decode_join_kernel<E, Core, 1> : (wpr == 4 ? attn_decode_join_kernel<E, Core, 4> : attn_decode_join_kernel<E, Core, 16>);
+  launch_k(join, static_cast<int>(blocks), threads, 0, st, d);
+  PTJ_CHECK_LAUNCH();
+  if (d.scores == nullptr) return PTJ_OK;
+  const int64_t chunks = ceil_div(d.rows.capacity, kWeightsChunk);
+  if (chunks * d.B * d.Hk > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
+  launch_k(attn_decode_weights_kernel, static_cast<int>(chunks * d.B * d.Hk), kDecJoinThreads, d.R * 8, st, d, pl.rows, static_cast<int>(chunks));
+  PTJ_CHECK_LAUNCH();
+  return PTJ_OK;
+}
+
 template <typename E, typename Core>
 int launch_decode(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
   constexpr int ring = kDecWarps * ring_bytes<Core>(), sums = kDecWarps * Core::kRows * (Core::kDim + 4) * 4;
@@ -879,11 +900,6 @@ int launch_decode(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
     PTJ_CHECK_LAUNCH();
     return PTJ_OK;
   }
-  // warps that join a row: by the pieces to be expected of a segment
-  const int64_t rows = static_cast<int64_t>(d.B) * d.Hk * d.R, pieces = (d.workers + d.small) / (static_cast<int64_t>(d.B) * d.Hk * d.nrb);
-  const int wpr = pieces <= 3 ? 1 : (pieces <= 32 ? 4 : 16), threads = wpr == 16 ? 512 : kDecJoinThreads;
-  const int64_t blocks = ceil_div(rows * wpr * 32, threads);
-  if (blocks > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
   if (d.small > 0 && cudaMemsetAsync(d.next, 0, 4, st) != cudaSuccess) {
     (void)cudaGetLastError();
     return PTJ_ERR_LAUNCH;
@@ -891,15 +907,7 @@ int launch_decode(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
   if (!set_smem(attn_decode_split_kernel<E, Core>, ring)) return PTJ_ERR_LAUNCH;
   launch_k(attn_decode_split_kernel<E, Core>, d.workers / kDecWarps, kDecWarps * 32, ring, st, d);
   PTJ_CHECK_LAUNCH();
-  const auto join = wpr == 1 ? attn_decode_join_kernel<E, Core, 1> : (wpr == 4 ? attn_decode_join_kernel<E, Core, 4> : attn_decode_join_kernel<E, Core, 16>);
-  launch_k(join, static_cast<int>(blocks), threads, 0, st, d);
-  PTJ_CHECK_LAUNCH();
-  if (d.scores == nullptr) return PTJ_OK;
-  const int64_t chunks = ceil_div(d.rows.capacity, kWeightsChunk);
-  if (chunks * d.B * d.Hk > 0x7fffffff) return PTJ_ERR_BAD_SHAPE;
-  launch_k(attn_decode_weights_kernel, static_cast<int>(chunks * d.B * d.Hk), kDecJoinThreads, d.R * 8, st, d, pl.rows, static_cast<int>(chunks));
-  PTJ_CHECK_LAUNCH();
-  return PTJ_OK;
+  return launch_join<E, Core>(d, pl, st);
 }
 
 }  // namespace

@@ -1,0 +1,397 @@
+// Attention of new tokens over a paged cache, bf16, many query rows per key head (drafted tokens of shared heads): tcgen05.
+//
+// The kernels with operands in registers are bound by their products from 16 rows on (attn_decode_tc.cu). Here a block takes 128 keys
+// at a time: S^T = K Q^T (128 keys x 32 rows) and O^T += V^T P^T (128 elements x 64 columns: 32 rows' first bf16 parts of the
+// probabilities and their second ones) run from shared memory into tensor memory, so that a thread of the 128 owns one key:
+// its 32 scores, exponentials and parts, one row of the product's operand. Keys stand in the 128-byte-swizzled layout with the head
+// elements contiguous, which is K-major for the first product and MN-major for the second; cp.async writes it row by row, since
+// rows lie in pages. Heads of 64 elements fill half of the second product's rows, what the other half multiplies is not read.
+//
+// Bound by the chain of a tile (keys arrive, product, scores, parts, product); two blocks per SM run theirs against each other, the
+// next tile's keys are on their way from the first product on and its values from the second. 4 x 8 caches of 30k keys of 128,
+// 32 rows: 198 us with operands in registers (in two passes), now 112, floor 75.
+#include "attn_decode.cuh"
+#include "tc_runtime.h"
+
+namespace ptj {
+namespace {
+
+using namespace tc;
+
+constexpr int kWideThreads = 128, kWideBlocks = 2;
+constexpr uint32_t kWideTmem = 128, kColO = 32;  // columns: 32 of scores, 64 of outputs
+
+template <int DP>
+struct CoreWide {
+  static constexpr int KS = 128, kRows = 32, kDim = DP;
+  static constexpr int DB = DP / 64;  // blocks of 64 elements
+  static constexpr int kK = 0, kV = kK + DB * 16384, kP = kV + DB * 16384, kQ = kP + 16384, kX = kQ + DB * 4096;
+  static constexpr int kSmem = kX + kRows * DP * 4 + 1024;  // (rounded up to 1024 bytes at run time)
+};
+
+// 16-byte piece c of row r of an operand with rows of DP elements in blocks of 64 (`block` bytes each)
+__device__ __forceinline__ int place(int r, int c, int block) { return (c >> 3) * block + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
+
+template <int DP>
+__global__ void __launch_bounds__(kWideThreads, kWideBlocks)
+attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
+  using Core = CoreWide<DP>;
+  constexpr int N = kWideThreads, NW = N / 32, R = Core::kRows, CH = DP / 8, RPI = 32 / CH;  // pieces of a row, rows of a warp's copy
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  __shared__ uint64_t bars[2];  // scores, outputs
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ __align__(16) float over_s[R], ref_s[R], fac_s[R], red[NW][R];
+  __shared__ int limit_s[R];
+  __shared__ int64_t tot[NW], start_s;
+  __shared__ int seq_s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == 0) {
+    tmem_alloc(&tmem_slot, kWideTmem);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    mbar_init(&bars[0], 1);
+    mbar_init(&bars[1], 1);
+    fence_barrier_init();
+    abort_flag = 0;
+  }
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot, lanes = static_cast<uint32_t>(warp) * 32u << 16;
+  const AbortCtx ctx{&abort_flag, p.rows.fault};
+  grid_dep_sync();  // nothing above touches global memory
+
+  // steps of all sequences, and of those before each thread's
+  const int per = (p.B + N - 1) / N, b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += steps_of<Core>(p.rows.length(p.lengths, b));
+  int64_t incl = mine;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, x);
+    if (lane >= x) incl += y;
+  }
+  if (lane == 31) tot[warp] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) before += tot[w];
+    total += tot[w];
+  }
+  const int64_t heads = static_cast<int64_t>(p.Hk) * p.nrb, all = total * heads;
+  Stretches st;
+  st.plan(p, all);
+  const int64_t worker = blockIdx.x, range0 = st.begin(worker);
+  int64_t acc = before * heads;
+  for (int b = b0; b < b1; ++b) {
+    const int64_t t = steps_of<Core>(p.rows.length(p.lengths, b)) * heads;
+    if (blockIdx.x == 0) p.starts[b] = acc;
+    if (range0 >= acc && range0 < acc + t) {
+      seq_s = b;
+      start_s = acc;
+    }
+    acc += t;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    p.starts[p.B] = st.q1;
+    p.starts[p.B + 1] = st.q2;
+  }
+  __syncthreads();
+
+  uint32_t scores_done = 0, outputs_done = 0;  // parities
+  if (range0 < all) {
+    Cursor<Core> cur;
+    cur.set(p, seq_s, start_s, range0, min(st.q1, all - range0));
+    bool first_piece = true;
+    for (;;) {  // segments
+      const Segment& sg = cur.sg;
+      // the rows' queries
+      {
+        const int r = tid >> 2, row = sg.rb * R + r, limit = sg.limit(p, row);
+        const char* q = limit >= 0 ? sg.q_row(p, row) : nullptr;
+#pragma unroll
+        for (int c = tid & 3; c < CH; c += 4) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (q != nullptr && p.q_wide && c * 8 + 8 <= p.D) {
+            x = *reinterpret_cast<const uint4*>(q + c * 16);
+          } else if (q != nullptr) {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(q);
+            auto at = [&](int d) { return d < p.D ? static_cast<uint32_t>(e[d]) : 0u; };
+            x = make_uint4(at(8 * c) | at(8 * c + 1) << 16, at(8 * c + 2) | at(8 * c + 3) << 16, at(8 * c + 4) | at(8 * c + 5) << 16,
+                           at(8 * c + 6) | at(8 * c + 7) << 16);
+          }
+          *reinterpret_cast<uint4*>(smem + Core::kQ + place(r, c, 4096)) = x;
+        }
+        if ((tid & 3) == 0) {
+          limit_s[r] = limit;
+          over_s[r] = -INFINITY;
+          ref_s[r] = kNoRef;
+        }
+      }
+      float sum[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum[r] = 0.f;
+      bool extra = false;  // products with values that are not finite wait in shared memory
+
+      // this thread's key of a tile
+      const char *kr = nullptr, *vr = nullptr;  // NULL: absent
+      auto page_at = [&](int j) { return j < sg.n ? sg.table[p.rows.page_of(j)] : 0; };
+      auto locate = [&](int j, int page) {
+        kr = vr = nullptr;
+        if (j >= sg.n || !p.rows.check(page)) return;
+        if (j >= sg.first && p.kn != nullptr) {
+          kr = p.kn + sg.b * p.kns[0] + sg.h * p.kns[1] + (j - sg.first) * p.kns[2];
+          vr = p.vn + sg.b * p.vns[0] + sg.h * p.vns[1] + (j - sg.first) * p.vns[2];
+        } else {
+          const int slot = j - p.rows.page_of(j) * p.rows.page_size;
+          kr = p.k + p.rows.offset(0, page, sg.h, slot);
+          vr = p.v + p.rows.offset(1, page, sg.h, slot);
+        }
+      };
+      auto copy_rows = [&](const char* mine_at, int where) {  // a warp copies its 32 lanes' rows
+        const uint32_t to = smem_u32(smem + where);
+#pragma unroll
+        for (int i = 0; i < 32; i += RPI) {
+          const int r = i + lane / CH, c = lane % CH;
+          const char* row = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), r));
+          copy16_or_zero(to + place(warp * 32 + r, c, 16384), row == nullptr ? p.k : row + c * 16, row != nullptr && c * 16 < p.rows.row_bytes);
+        }
+        cp_async_commit();
+      };
+      auto store_new = [&](int kv, int j, int page, int where) {  // this thread's row, if it is new, to its page
+        if (j < sg.first || j >= sg.n || p.kn == nullptr || sg.rb != 0 || !p.rows.check(page)) return;
+        char* at = (kv == 0 ? p.k : p.v) + p.rows.offset(kv, page, sg.h, j - p.rows.page_of(j) * p.rows.page_size);
+        for (int c = 0; c * 16 < p.rows.row_bytes; ++c)
+          *reinterpret_cast<uint4*>(at + c * 16) = *reinterpret_cast<const uint4*>(smem + where + place(tid, c, 16384));
+      };
+
+      const int s_first = cur.s;
+      int page = page_at(s_first * 128 + tid), page_next = s_first + 1 < cur.end ? page_at(s_first * 128 + 128 + tid) : 0;
+      locate(s_first * 128 + tid, page);
+      copy_rows(kr, Core::kK);
+#pragma unroll 1
+      for (; cur.s < cur.end; ++cur.s) {
+        const int j0 = cur.s * 128, j = j0 + tid;
+        const bool edge = j0 + 128 > sg.first + 1, there = kr != nullptr, news = p.kn != nullptr && j0 + 128 > sg.first;
+        if (cur.s > s_first) {  // the values' and parts' places are free
+          mbar_wait(&bars[1], outputs_done & 1, ctx, 0x3301u);
+          ++outputs_done;
+        }
+        copy_rows(vr, Core::kV);
+        cp_async_wait<1>();  // the keys
+        fence_proxy_async_smem();
+        __syncthreads();
+        if (news) {
+          store_new(0, j, page, Core::kK);
+          __syncthreads();  // (the next keys overwrite what is read here)
+        }
+        if (warp == 0) {
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            mma_bf16_ss_elect(tmem, smem_desc_sw128(smem_u32(smem + Core::kK) + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
+                              smem_desc_sw128(smem_u32(smem + Core::kQ) + (k >> 2) * 4096 + (k & 3) * 32, 16, 1024),
+                              idesc_bf16_f32(128, R, false, false), k > 0);
+          mma_commit_elect(&bars[0]);
+        }
+        const int page_now = page;
+        if (cur.s + 1 < cur.end) {  // (looked up a tile ahead)
+          page = page_next;
+          page_next = cur.s + 2 < cur.end ? page_at(j + 256) : 0;
+        }
+        mbar_wait(&bars[0], scores_done & 1, ctx, 0x3302u);
+        ++scores_done;
+        tc_fence_after_sync();
+        if (cur.s + 1 < cur.end) {
+          locate(j + 128, page);
+          copy_rows(kr, Core::kK);
+        } else {
+          cp_async_commit();
+        }
+        float s[R];
+        tmem_ld_32x32f(tmem + lanes, s);
+        tmem_ld_wait();
+        if (edge) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (!there || j > limit_s[r]) s[r] = -INFINITY;
+        } else if (!there) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) s[r] = -INFINITY;
+        }
+        if (p.scores != nullptr && j < sg.n) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (sg.rb * R + r < p.R) sg.score_row(p, sg.rb * R + r)[j] = s[r] * p.scale;
+        }
+        bool moves = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) moves |= s[r] > over_s[r];
+        if (__syncthreads_or(moves)) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float m = warp_max(s[r]);
+            if (lane == 0) red[warp][r] = m;
+          }
+          __syncthreads();
+          if (tid < R) {
+            float m = red[0][tid];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) m = fmaxf(m, red[w][tid]);
+            m = fmaxf(m * p.scale, ref_s[tid]);
+            fac_s[tid] = rebase(ref_s[tid], m);
+            ref_s[tid] = m;
+            over_s[tid] = (m + kDecLazy) * p.unscale;
+          }
+          __syncthreads();
+#pragma unroll
+          for (int r = 0; r < R; ++r) sum[r] *= fac_s[r];
+          if (cur.s > s_first) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              uint32_t o[32];
+              tmem_ld_32x32(tmem + lanes + kColO + part * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int r = 0; r < R; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * fac_s[r]);
+              tmem_st_32x32(tmem + lanes + kColO + part * 32, o);
+              tmem_st_wait();
+            }
+          }
+        }
+        // exponentials, their sums, and their parts: a row of the operand, first parts in its first 64 bytes
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = c * 8 + 2 * e;
+            const float x0 = ex2(fmaf(s[r], p.scale, -ref_s[r])), x1 = ex2(fmaf(s[r + 1], p.scale, -ref_s[r + 1]));
+            sum[r] += x0;
+            sum[r + 1] += x1;
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x0, x1);
+            hi[e] = *reinterpret_cast<const uint32_t*>(&h);
+            const __nv_bfloat162 l = __floats2bfloat162_rn(x0 - __uint_as_float(hi[e] << 16), x1 - __uint_as_float(hi[e] & 0xffff0000u));
+            lo[e] = *reinterpret_cast<const uint32_t*>(&l);
+          }
+          *reinterpret_cast<uint4*>(smem + Core::kP + place(tid, c, 0)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(smem + Core::kP + place(tid, c + 4, 0)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        cp_async_wait<1>();  // the values
+        if (edge) {
+          // a value that some rows attend and others do not must be finite to be multiplied by the others' zeros
+          __syncthreads();
+          if (news) store_new(1, j, page_now, Core::kV);
+          bool bad = false;
+          if (there)
+            for (int c = 0; c < CH; ++c) {
+              const uint4 x = *reinterpret_cast<const uint4*>(smem + Core::kV + place(tid, c, 16384));
+              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+            }
+          if (__syncthreads_or(bad)) {
+            float* x = reinterpret_cast<float*>(smem + Core::kX);  // [R][DP]
+            if (!extra)
+              for (int i = tid; i < R * DP; i += N) x[i] = 0.f;
+            extra = true;
+            __syncthreads();
+            if (tid < DP)  // a thread per element: this one's column of x, and of the values
+              for (int key = 0; key < 128; ++key) {
+                uint16_t* v = reinterpret_cast<uint16_t*>(smem + Core::kV + place(key, tid >> 3, 16384)) + (tid & 7);
+                if ((*v & 0x7f80u) != 0x7f80u) continue;
+                const float val = __uint_as_float(static_cast<uint32_t>(*v) << 16);
+                for (int r = 0; r < R; ++r)
+                  if (j0 + key <= limit_s[r]) {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(smem + Core::kP + place(key, r >> 3, 0)) + (r & 7);
+                    const float pr = __uint_as_float(static_cast<uint32_t>(*h) << 16);
+                    x[r * DP + tid] += pr * val;
+                  }
+                *v = 0;
+              }
+            __syncthreads();
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        __syncthreads();
+        if (warp == 0) {
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_bf16_ss_elect(tmem + kColO, smem_desc_sw128(smem_u32(smem + Core::kV) + k * 2048, 16384, 1024),
+                              smem_desc_sw128(smem_u32(smem + Core::kP) + k * 2048, 16384, 1024), idesc_bf16_f32(128, 64, true, true),
+                              cur.s > s_first || k > 0);
+          mma_commit_elect(&bars[1]);
+        }
+      }
+      cp_async_wait<0>();
+      mbar_wait(&bars[1], outputs_done & 1, ctx, 0x3303u);
+      ++outputs_done;
+      tc_fence_after_sync();
+      // sums over the keys, then every thread has an element of all rows
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float l = warp_sum(sum[r]);
+        if (lane == 0) red[warp][r] = l;
+      }
+      float hi[R], lo[R];
+      tmem_ld_32x32f(tmem + lanes + kColO, hi);
+      tmem_ld_32x32f(tmem + lanes + kColO + 32, lo);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      __syncthreads();
+      const bool whole = s_first == 0 && cur.s == cur.steps;
+      const int64_t piece = worker * 2 + (first_piece ? 0 : 1);
+      if (tid < p.D) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int row = sg.rb * R + r;
+          if (row >= p.R) continue;
+          const float l = (red[0][r] + red[1][r]) + (red[2][r] + red[3][r]);
+          float o = hi[r] + lo[r];
+          if (extra) o += reinterpret_cast<const float*>(smem + Core::kX)[r * DP + tid];
+          if (whole) {
+            char* to = p.out + sg.b * p.os[0] + (sg.h * p.G + row / p.T) * p.os[1] + (row % p.T) * p.os[2];
+            reinterpret_cast<__nv_bfloat16*>(to)[tid] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * (p.keep / l) : 0.f);
+          } else {
+            p.part[(piece * p.prows + r) * Core::kDim + tid] = o;
+          }
+          if (tid == 0 && (!whole || p.scores != nullptr)) {
+            float* to = whole ? p.ml + (sg.index(p) * p.prows + r) * 2 : p.part_ml + (piece * p.prows + r) * 2;
+            *reinterpret_cast<float2*>(to) = make_float2(ref_s[r], l);
+          }
+        }
+      }
+      first_piece = false;
+      __syncthreads();  // what the next segment overwrites has been read
+      if (cur.left == 0) break;
+      cur.next_segment(p);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 0) tmem_dealloc(tmem, kWideTmem);
+}
+
+template <int DP>
+int launch_wide(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
+  using Core = CoreWide<DP>;
+  if (!set_smem(attn_decode_wide_kernel<DP>, Core::kSmem)) return PTJ_ERR_LAUNCH;
+  launch_k(attn_decode_wide_kernel<DP>, d.workers, kWideThreads, Core::kSmem, st, d);
+  PTJ_CHECK_LAUNCH();
+  return launch_join<__nv_bfloat16, Core>(d, pl, st);
+}
+
+}  // namespace
+
+int decode_wide_blocks() { return kWideBlocks; }
+int launch_decode_wide(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
+  return pl.dim == 64 ? launch_wide<64>(d, pl, st) : launch_wide<128>(d, pl, st);
+}
+
+}  // namespace ptj

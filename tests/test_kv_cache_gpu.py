@@ -44,6 +44,10 @@ CASES = [
     (BF16, 8, 2, 64, 5, 16, [5, 7, 3, 0, 333]),
     (BF16, 16, 2, 128, 4, 64, [4, 1000]),
     (BF16, 2, 1, 64, 40, 16, [40, 333]),
+    (BF16, 8, 1, 128, 4, 16, [4, 127, 128, 129, 3, 0, 700]),   # 32 query rows per key head
+    (BF16, 10, 2, 64, 7, 7, [7, 300]),
+    (BF16, 6, 2, 96, 13, 48, [13, 1, 500]),
+    (BF16, 8, 1, 72, 9, 24, [9, 260]),
     (BF16, 2, 2, 8, 1, 1, [1, 5, 40]),
     (BF16, 2, 2, 16, 3, 5, [3, 41]),
     (BF16, 2, 2, 256, 1, 16, [1, 99]),
@@ -166,6 +170,53 @@ def test_append_and_attend(dtype, D, T):
     ops.kv_append(dk, dv, kp2, vp2, table.cuda(), lens.cuda(), counts.cuda())
     assert same(kp2, k_want) and same(vp2, v_want)
     again = ops.attn_decode(dq, kp2, vp2, table.cuda(), lens.cuda(), counts=counts.cuda(), p=0.1)
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_many_rows_read_only_what_they_attend(D, bad):
+    """24 query rows per key head: later tokens' keys and values that are not finite, across the border of two tiles of 128."""
+    T = 12
+    kp, vp, table, lens = ref.paged([262, 12, 300], 1, D, 16, BF16)
+    q = torch.randn((3, 2, T, D), generator=torch.Generator().manual_seed(20)).to(BF16)
+    counts = torch.full((3,), T, dtype=torch.int32)
+    want, _, spread = ref.attend(q, kp, vp, table, lens, counts, p=0.0)
+    for b, n in enumerate((262, 12)):
+        for pool, at in ((vp, n - 1), (kp, n - 2), (vp, n - 3)):
+            pool[int(table[b, at // 16]), :, at % 16, 5:9] = bad
+    out, _, _, _ = run(q, kp, vp, table, lens, counts, p=0.0)
+    check_out(out[:2, :, :T - 3], want[:2, :, :T - 3], spread[:2, :, :T - 3], BF16)
+    check_out(out[2], want[2], spread[2], BF16)
+    assert not out[:2, :, T - 3, 5:9].isfinite().any() and out[:2, :, T - 3, 9:].isfinite().all()
+    assert not out[:2, :, T - 1].isfinite().all()
+
+
+def test_many_rows_append_split_and_replay():
+    """24 rows, long and short sequences: new rows are written, the pieces of a sequence joined, twice the same bits."""
+    ops = pkg("operators")
+    lengths, Hk, H, T, D, page = [20000, 6, 0, 1500], 2, 8, 6, 128, 32
+    kp, vp, table, lens = ref.paged(lengths, Hk, D, page, BF16)
+    counts = torch.clamp(lens, max=T)
+    new = torch.randn((4, T, H + 2 * Hk, D), generator=torch.Generator().manual_seed(21)).to(BF16)
+    q, k, v = (x.transpose(1, 2) for x in (new[:, :, :H], new[:, :, H:H + Hk], new[:, :, H + Hk:]))
+    k_want, v_want = kp.clone(), vp.clone()
+    for b, n in enumerate(lengths):
+        for t in range(int(counts[b])):
+            at = n - int(counts[b]) + t
+            for pool, x in ((k_want, k), (v_want, v)):
+                pool[int(table[b, at // page]), :, at % page] = x[b, :, t]
+    dnew = new.cuda()
+    dq, dk, dv = (x.transpose(1, 2) for x in (dnew[:, :, :H], dnew[:, :, H:H + Hk], dnew[:, :, H + Hk:]))
+    w = torch.zeros((4, Hk, table.shape[1] * page))
+    out, k_got, v_got, got = run(dq, kp, vp, table, lens, counts, w, k=dk, v=dv)
+    same = lambda a, b: torch.equal(a.cpu().nan_to_num(7.0), b.nan_to_num(7.0))
+    assert same(k_got, k_want) and same(v_got, v_want)
+    want, w_want, spread = ref.attend(q, k_want, v_want, table, lens, counts, w, p=0.1)
+    check_out(out, want, spread, BF16)
+    rel = ref.attention_error(6.0 * D**0.5, 20000, D) + (H // Hk * T + 2) * 2.0**-23
+    assert bool(((got.double().cpu() - w_want).abs() <= rel * w_want + 1e-30).all())
+    again = ops.attn_decode(dq, k_got, v_got, table.cuda(), lens.cuda(), counts=counts.cuda(), p=0.1)
     assert torch.equal(out, again)
 
 
