@@ -2,8 +2,9 @@
 //
 // The kernels with operands in registers are bound by their products from 16 rows on (attn_decode_tc.cu). Here a block takes 128 keys
 // at a time: S^T = K Q^T (128 keys x 32 rows) and O^T += V^T P^T (128 elements x 64 columns: 32 rows' first bf16 parts of the
-// probabilities and their second ones) run from shared memory into tensor memory, so that a thread of the 128 owns one key:
-// its 32 scores, exponentials and parts, one row of the product's operand. Keys stand in the 128-byte-swizzled layout with the head
+// probabilities and their second ones) run from shared memory into tensor memory, so that two threads share a key: each has 16 of
+// its scores, exponentials and parts, half a row of the product's operand. (One thread with all 32 was a third slower: four warps
+// do not hide the chain of a tile.) Keys stand in the 128-byte-swizzled layout with the head
 // elements contiguous, which is K-major for the first product and MN-major for the second; cp.async writes it row by row, since
 // rows lie in pages. Heads of 64 elements fill half of the second product's rows, what the other half multiplies is not read.
 //
@@ -18,7 +19,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kWideThreads = 128, kWideBlocks = 2;
+constexpr int kWideThreads = 256, kWideBlocks = 2;
 constexpr uint32_t kWideTmem = 128, kColO = 32;  // columns: 32 of scores, 64 of outputs
 
 template <int DP>
@@ -36,13 +37,14 @@ template <int DP>
 __global__ void __launch_bounds__(kWideThreads, kWideBlocks)
 attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
   using Core = CoreWide<DP>;
-  constexpr int N = kWideThreads, NW = N / 32, R = Core::kRows, CH = DP / 8, RPI = 32 / CH;  // pieces of a row, rows of a warp's copy
+  constexpr int N = kWideThreads, NW = N / 32, R = Core::kRows, RH = R / 2, CH = DP / 8, RPI = 32 / CH;  // pieces of a row, rows of a copy
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   __shared__ uint64_t bars[2];  // scores, outputs
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ __align__(16) float over_s[R], ref_s[R], fac_s[R], red[NW][R];
+  __shared__ __align__(16) float over_s[R], ref_s[R], fac_s[R], red[NW][RH];
+  __shared__ uint8_t there_s[2][128];
   __shared__ int limit_s[R];
   __shared__ int64_t tot[NW], start_s;
   __shared__ int seq_s;
@@ -59,7 +61,8 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
   }
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = tmem_slot, lanes = static_cast<uint32_t>(warp) * 32u << 16;
+  const uint32_t tmem = tmem_slot, lanes = static_cast<uint32_t>(warp & 3) * 32u << 16;
+  const int key = (warp & 3) * 32 + lane, r0 = (warp >> 2) * RH;  // this thread's key of a tile (and element of outputs), its rows
   const AbortCtx ctx{&abort_flag, p.rows.fault};
   grid_dep_sync();  // nothing above touches global memory
 
@@ -110,10 +113,10 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
       const Segment& sg = cur.sg;
       // the rows' queries
       {
-        const int r = tid >> 2, row = sg.rb * R + r, limit = sg.limit(p, row);
+        const int r = tid >> 3, row = sg.rb * R + r, limit = sg.limit(p, row);
         const char* q = limit >= 0 ? sg.q_row(p, row) : nullptr;
 #pragma unroll
-        for (int c = tid & 3; c < CH; c += 4) {
+        for (int c = tid & 7; c < CH; c += 8) {
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
           if (q != nullptr && p.q_wide && c * 8 + 8 <= p.D) {
             x = *reinterpret_cast<const uint4*>(q + c * 16);
@@ -125,67 +128,69 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
           }
           *reinterpret_cast<uint4*>(smem + Core::kQ + place(r, c, 4096)) = x;
         }
-        if ((tid & 3) == 0) {
+        if ((tid & 7) == 0) {
           limit_s[r] = limit;
           over_s[r] = -INFINITY;
           ref_s[r] = kNoRef;
         }
       }
-      float sum[R];
+      float sum[RH];
 #pragma unroll
-      for (int r = 0; r < R; ++r) sum[r] = 0.f;
+      for (int i = 0; i < RH; ++i) sum[i] = 0.f;
       bool extra = false;  // products with values that are not finite wait in shared memory
 
-      // this thread's key of a tile
-      const char *kr = nullptr, *vr = nullptr;  // NULL: absent
+      // A warp copies 16 keys; lane i < 16 has the address of the i-th key's row, lane 16 + i that of its value's. NULL: absent.
+      const int mine16 = warp * 16 + (lane & 15), kv = lane >> 4;
+      const char* at = nullptr;
       auto page_at = [&](int j) { return j < sg.n ? sg.table[p.rows.page_of(j)] : 0; };
-      auto locate = [&](int j, int page) {
-        kr = vr = nullptr;
-        if (j >= sg.n || !p.rows.check(page)) return;
-        if (j >= sg.first && p.kn != nullptr) {
-          kr = p.kn + sg.b * p.kns[0] + sg.h * p.kns[1] + (j - sg.first) * p.kns[2];
-          vr = p.vn + sg.b * p.vns[0] + sg.h * p.vns[1] + (j - sg.first) * p.vns[2];
-        } else {
-          const int slot = j - p.rows.page_of(j) * p.rows.page_size;
-          kr = p.k + p.rows.offset(0, page, sg.h, slot);
-          vr = p.v + p.rows.offset(1, page, sg.h, slot);
-        }
+      auto slot_at = [&](int j, int page) {  // in the pages
+        return (kv == 0 ? p.k : p.v) + p.rows.offset(kv, page, sg.h, j - p.rows.page_of(j) * p.rows.page_size);
       };
-      auto copy_rows = [&](const char* mine_at, int where) {  // a warp copies its 32 lanes' rows
+      auto locate = [&](int tile, int page) {
+        const int j = tile * 128 + mine16;
+        at = nullptr;
+        if (j < sg.n && p.rows.check(page)) {
+          const int64_t* st = kv == 0 ? p.kns : p.vns;
+          at = j >= sg.first && p.kn != nullptr ? (kv == 0 ? p.kn : p.vn) + sg.b * st[0] + sg.h * st[1] + (j - sg.first) * st[2]
+                                                : slot_at(j, page);
+        }
+        if (kv == 0) there_s[tile & 1][mine16] = at != nullptr;
+      };
+      auto copy_rows = [&](int which, int where) {
         const uint32_t to = smem_u32(smem + where);
 #pragma unroll
-        for (int i = 0; i < 32; i += RPI) {
+        for (int i = 0; i < 16; i += RPI) {
           const int r = i + lane / CH, c = lane % CH;
-          const char* row = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine_at), r));
-          copy16_or_zero(to + place(warp * 32 + r, c, 16384), row == nullptr ? p.k : row + c * 16, row != nullptr && c * 16 < p.rows.row_bytes);
+          const char* row = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), which * 16 + r));
+          copy16_or_zero(to + place(warp * 16 + r, c, 16384), row + c * 16, row != nullptr && c * 16 < p.rows.row_bytes);
         }
         cp_async_commit();
       };
-      auto store_new = [&](int kv, int j, int page, int where) {  // this thread's row, if it is new, to its page
-        if (j < sg.first || j >= sg.n || p.kn == nullptr || sg.rb != 0 || !p.rows.check(page)) return;
-        char* at = (kv == 0 ? p.k : p.v) + p.rows.offset(kv, page, sg.h, j - p.rows.page_of(j) * p.rows.page_size);
+      auto store_new = [&](int which, int j, int page, int where) {  // this lane's row, if it is new, to its page
+        if (kv != which || j < sg.first || j >= sg.n || p.kn == nullptr || sg.rb != 0 || !p.rows.check(page)) return;
+        char* to = slot_at(j, page);
         for (int c = 0; c * 16 < p.rows.row_bytes; ++c)
-          *reinterpret_cast<uint4*>(at + c * 16) = *reinterpret_cast<const uint4*>(smem + where + place(tid, c, 16384));
+          *reinterpret_cast<uint4*>(to + c * 16) = *reinterpret_cast<const uint4*>(smem + where + place(mine16, c, 16384));
       };
 
       const int s_first = cur.s;
-      int page = page_at(s_first * 128 + tid), page_next = s_first + 1 < cur.end ? page_at(s_first * 128 + 128 + tid) : 0;
-      locate(s_first * 128 + tid, page);
-      copy_rows(kr, Core::kK);
+      int page = page_at(s_first * 128 + mine16), page_next = s_first + 1 < cur.end ? page_at(s_first * 128 + 128 + mine16) : 0;
+      locate(s_first, page);
+      copy_rows(0, Core::kK);
 #pragma unroll 1
       for (; cur.s < cur.end; ++cur.s) {
-        const int j0 = cur.s * 128, j = j0 + tid;
-        const bool edge = j0 + 128 > sg.first + 1, there = kr != nullptr, news = p.kn != nullptr && j0 + 128 > sg.first;
+        const int j0 = cur.s * 128, j = j0 + key, j16 = j0 + mine16;
+        const bool edge = j0 + 128 > sg.first + 1, news = p.kn != nullptr && j0 + 128 > sg.first;
         if (cur.s > s_first) {  // the values' and parts' places are free
           mbar_wait(&bars[1], outputs_done & 1, ctx, 0x3301u);
           ++outputs_done;
         }
-        copy_rows(vr, Core::kV);
+        copy_rows(1, Core::kV);
         cp_async_wait<1>();  // the keys
         fence_proxy_async_smem();
         __syncthreads();
         if (news) {
-          store_new(0, j, page, Core::kK);
+          store_new(0, j16, page, Core::kK);
           __syncthreads();  // (the next keys overwrite what is read here)
         }
         if (warp == 0) {
@@ -200,95 +205,98 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
         const int page_now = page;
         if (cur.s + 1 < cur.end) {  // (looked up a tile ahead)
           page = page_next;
-          page_next = cur.s + 2 < cur.end ? page_at(j + 256) : 0;
+          page_next = cur.s + 2 < cur.end ? page_at(j16 + 256) : 0;
         }
         mbar_wait(&bars[0], scores_done & 1, ctx, 0x3302u);
         ++scores_done;
         tc_fence_after_sync();
         if (cur.s + 1 < cur.end) {
-          locate(j + 128, page);
-          copy_rows(kr, Core::kK);
+          locate(cur.s + 1, page);
+          copy_rows(0, Core::kK);
         } else {
           cp_async_commit();
         }
-        float s[R];
-        tmem_ld_32x32f(tmem + lanes, s);
+        const bool there = there_s[cur.s & 1][key];
+        uint32_t raw_s[RH];
+        tmem_ld_32x16(tmem + lanes + r0, raw_s);
         tmem_ld_wait();
-        if (edge) {
+        float s[RH];
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (!there || j > limit_s[r]) s[r] = -INFINITY;
-        } else if (!there) {
+        for (int i = 0; i < RH; ++i) s[i] = __uint_as_float(raw_s[i]);
+        if (edge || !there) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) s[r] = -INFINITY;
+          for (int i = 0; i < RH; ++i)
+            if (!there || j > limit_s[r0 + i]) s[i] = -INFINITY;
         }
         if (p.scores != nullptr && j < sg.n) {
+          float* to = sg.score_row(p, sg.rb * R + r0) + j;
 #pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (sg.rb * R + r < p.R) sg.score_row(p, sg.rb * R + r)[j] = s[r] * p.scale;
+          for (int i = 0; i < RH; ++i)
+            if (sg.rb * R + r0 + i < p.R) to[i * p.scores_ld] = s[i] * p.scale;
         }
         bool moves = false;
 #pragma unroll
-        for (int r = 0; r < R; ++r) moves |= s[r] > over_s[r];
+        for (int i = 0; i < RH; i += 4) {
+          const float4 o = *reinterpret_cast<const float4*>(over_s + r0 + i);
+          moves |= s[i] > o.x || s[i + 1] > o.y || s[i + 2] > o.z || s[i + 3] > o.w;
+        }
         if (__syncthreads_or(moves)) {
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float m = warp_max(s[r]);
-            if (lane == 0) red[warp][r] = m;
+          for (int i = 0; i < RH; ++i) {
+            const float m = warp_max(s[i]);
+            if (lane == 0) red[warp][i] = m;
           }
           __syncthreads();
           if (tid < R) {
-            float m = red[0][tid];
-#pragma unroll
-            for (int w = 1; w < NW; ++w) m = fmaxf(m, red[w][tid]);
-            m = fmaxf(m * p.scale, ref_s[tid]);
+            const int w0 = tid / RH * 4, i = tid % RH;
+            const float m = fmaxf(fmaxf(fmaxf(red[w0][i], red[w0 + 1][i]), fmaxf(red[w0 + 2][i], red[w0 + 3][i])) * p.scale, ref_s[tid]);
             fac_s[tid] = rebase(ref_s[tid], m);
             ref_s[tid] = m;
             over_s[tid] = (m + kDecLazy) * p.unscale;
           }
           __syncthreads();
 #pragma unroll
-          for (int r = 0; r < R; ++r) sum[r] *= fac_s[r];
-          if (cur.s > s_first) {
+          for (int i = 0; i < RH; ++i) sum[i] *= fac_s[r0 + i];
+          if (cur.s > s_first) {  // the first four warps rescale the first parts' columns, the others the second parts'
+            uint32_t o[32];
+            const uint32_t columns = tmem + lanes + kColO + (warp >> 2) * 32;
+            tmem_ld_32x32(columns, o);
+            tmem_ld_wait();
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              uint32_t o[32];
-              tmem_ld_32x32(tmem + lanes + kColO + part * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int r = 0; r < R; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * fac_s[r]);
-              tmem_st_32x32(tmem + lanes + kColO + part * 32, o);
-              tmem_st_wait();
-            }
+            for (int r = 0; r < R; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * fac_s[r]);
+            tmem_st_32x32(columns, o);
+            tmem_st_wait();
           }
         }
-        // exponentials, their sums, and their parts: a row of the operand, first parts in its first 64 bytes
+        // exponentials, their sums, and their parts: half a row of the operand, first parts in the row's first 64 bytes
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < RH / 8; ++c) {
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int r = c * 8 + 2 * e;
-            const float x0 = ex2(fmaf(s[r], p.scale, -ref_s[r])), x1 = ex2(fmaf(s[r + 1], p.scale, -ref_s[r + 1]));
-            sum[r] += x0;
-            sum[r + 1] += x1;
+            const int i = c * 8 + 2 * e;
+            const float2 ref = *reinterpret_cast<const float2*>(ref_s + r0 + i);
+            const float x0 = ex2(fmaf(s[i], p.scale, -ref.x)), x1 = ex2(fmaf(s[i + 1], p.scale, -ref.y));
+            sum[i] += x0;
+            sum[i + 1] += x1;
             const __nv_bfloat162 h = __floats2bfloat162_rn(x0, x1);
             hi[e] = *reinterpret_cast<const uint32_t*>(&h);
             const __nv_bfloat162 l = __floats2bfloat162_rn(x0 - __uint_as_float(hi[e] << 16), x1 - __uint_as_float(hi[e] & 0xffff0000u));
             lo[e] = *reinterpret_cast<const uint32_t*>(&l);
           }
-          *reinterpret_cast<uint4*>(smem + Core::kP + place(tid, c, 0)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(smem + Core::kP + place(tid, c + 4, 0)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          const int piece = r0 / 8 + c;
+          *reinterpret_cast<uint4*>(smem + Core::kP + place(key, piece, 0)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(smem + Core::kP + place(key, piece + 4, 0)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         cp_async_wait<1>();  // the values
         if (edge) {
           // a value that some rows attend and others do not must be finite to be multiplied by the others' zeros
           __syncthreads();
-          if (news) store_new(1, j, page_now, Core::kV);
+          if (news) store_new(1, j16, page_now, Core::kV);
           bool bad = false;
-          if (there)
+          if (there && r0 == 0)
             for (int c = 0; c < CH; ++c) {
-              const uint4 x = *reinterpret_cast<const uint4*>(smem + Core::kV + place(tid, c, 16384));
+              const uint4 x = *reinterpret_cast<const uint4*>(smem + Core::kV + place(key, c, 16384));
               const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
@@ -300,13 +308,13 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
             extra = true;
             __syncthreads();
             if (tid < DP)  // a thread per element: this one's column of x, and of the values
-              for (int key = 0; key < 128; ++key) {
-                uint16_t* v = reinterpret_cast<uint16_t*>(smem + Core::kV + place(key, tid >> 3, 16384)) + (tid & 7);
+              for (int k = 0; k < 128; ++k) {
+                uint16_t* v = reinterpret_cast<uint16_t*>(smem + Core::kV + place(k, tid >> 3, 16384)) + (tid & 7);
                 if ((*v & 0x7f80u) != 0x7f80u) continue;
                 const float val = __uint_as_float(static_cast<uint32_t>(*v) << 16);
                 for (int r = 0; r < R; ++r)
-                  if (j0 + key <= limit_s[r]) {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(smem + Core::kP + place(key, r >> 3, 0)) + (r & 7);
+                  if (j0 + k <= limit_s[r]) {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(smem + Core::kP + place(k, r >> 3, 0)) + (r & 7);
                     const float pr = __uint_as_float(static_cast<uint32_t>(*h) << 16);
                     x[r * DP + tid] += pr * val;
                   }
@@ -332,35 +340,36 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
       mbar_wait(&bars[1], outputs_done & 1, ctx, 0x3303u);
       ++outputs_done;
       tc_fence_after_sync();
-      // sums over the keys, then every thread has an element of all rows
+      // sums over the keys, then every thread has an element of its rows
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const float l = warp_sum(sum[r]);
-        if (lane == 0) red[warp][r] = l;
+      for (int i = 0; i < RH; ++i) {
+        const float l = warp_sum(sum[i]);
+        if (lane == 0) red[warp][i] = l;
       }
-      float hi[R], lo[R];
-      tmem_ld_32x32f(tmem + lanes + kColO, hi);
-      tmem_ld_32x32f(tmem + lanes + kColO + 32, lo);
+      uint32_t hi[RH], lo[RH];
+      tmem_ld_32x16(tmem + lanes + kColO + r0, hi);
+      tmem_ld_32x16(tmem + lanes + kColO + 32 + r0, lo);
       tmem_ld_wait();
       tc_fence_before_sync();
       __syncthreads();
       const bool whole = s_first == 0 && cur.s == cur.steps;
       const int64_t piece = worker * 2 + (first_piece ? 0 : 1);
-      if (tid < p.D) {
+      if (key < p.D) {
+        const int w0 = r0 / RH * 4;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int row = sg.rb * R + r;
+        for (int i = 0; i < RH; ++i) {
+          const int r = r0 + i, row = sg.rb * R + r;
           if (row >= p.R) continue;
-          const float l = (red[0][r] + red[1][r]) + (red[2][r] + red[3][r]);
-          float o = hi[r] + lo[r];
-          if (extra) o += reinterpret_cast<const float*>(smem + Core::kX)[r * DP + tid];
+          const float l = (red[w0][i] + red[w0 + 1][i]) + (red[w0 + 2][i] + red[w0 + 3][i]);
+          float o = __uint_as_float(hi[i]) + __uint_as_float(lo[i]);
+          if (extra) o += reinterpret_cast<const float*>(smem + Core::kX)[r * DP + key];
           if (whole) {
             char* to = p.out + sg.b * p.os[0] + (sg.h * p.G + row / p.T) * p.os[1] + (row % p.T) * p.os[2];
-            reinterpret_cast<__nv_bfloat16*>(to)[tid] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * (p.keep / l) : 0.f);
+            reinterpret_cast<__nv_bfloat16*>(to)[key] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * (p.keep / l) : 0.f);
           } else {
-            p.part[(piece * p.prows + r) * Core::kDim + tid] = o;
+            p.part[(piece * p.prows + r) * Core::kDim + key] = o;
           }
-          if (tid == 0 && (!whole || p.scores != nullptr)) {
+          if (key == 0 && (!whole || p.scores != nullptr)) {
             float* to = whole ? p.ml + (sg.index(p) * p.prows + r) * 2 : p.part_ml + (piece * p.prows + r) * 2;
             *reinterpret_cast<float2*>(to) = make_float2(ref_s[r], l);
           }
