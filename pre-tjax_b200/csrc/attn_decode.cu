@@ -9,8 +9,6 @@ constexpr int kMaxRows = 4096;      // query rows of a key head
 constexpr int kLeastKeys = 64;      // keys that a stretch of the list has at least
 constexpr int kMostPieces = 1024;   // pieces of a sequence of the capacity's length, about
 
-constexpr int kManyRows = 16;       // query rows of a key head beyond which the tcgen05 kernel takes over
-
 bool new_rows_aligned(const ptj_kv_cache& c, const ptj_new_tokens& t) {
   return !t.k || (view_aligned(t.k, t.k_strides, c, c.kv_heads, t.tokens) && view_aligned(t.v, t.v_strides, c, c.kv_heads, t.tokens));
 }
@@ -24,7 +22,11 @@ DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const Paged
   pl.es = static_cast<int>(dtype_size(c.dtype));
   const bool tc = c.dtype == PTJ_BF16 && c.d_head <= 128;
   pl.dim = c.d_head <= 64 && (tc || pl.es == 4) ? 64 : (c.d_head <= 128 && (tc || pl.es == 4) ? 128 : 256);
-  pl.wide = tc && R > kManyRows && aligned;
+  // More rows than the registers' products take in one pass at memory speed, and tiles enough that the tcgen05 kernel's longer chain
+  // and its second pass do not show: 32 rows on 32 caches of 30k keys of 128 take 118 us on it, 198 in registers, 24 rows 112 and
+  // 106; of 2k keys, 32 rows on 128 caches, 57 and 48; 20 rows of 64 elements, 30k keys, 89 and 121.
+  pl.wide = tc && aligned && R > (pl.dim == 64 ? 16 : 24) &&
+            c.batch * c.kv_heads * ceil_div(R, 32) * ceil_div(rows.capacity, 128) >= 12ll * decode_wide_blocks() * kNumSMs;
   // the core with the fewest blocks of rows (each reads the keys and values again, mostly from L2), of those the smallest
   if (tc) {
     const int most = pl.dim == 64 ? 32 : 24;

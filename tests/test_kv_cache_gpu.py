@@ -24,8 +24,14 @@ def check_out(out, want, spread, dtype):
     assert not out.isnan().any() and bool((err <= bound).all()), float((err / bound.clamp(min=1e-30)).max())
 
 
-def run(q, kp, vp, table, lengths, counts=None, weights=None, p=0.1, **kw):
+def run(q, kp, vp, table, lengths, counts=None, weights=None, p=0.1, wide_table=0, **kw):
+    """wide_table: keys that a row of the table has room for, at least; the choice of a kernel goes by the room."""
     ops = pkg("operators")
+    page = kp.shape[2]
+    if wide_table > table.shape[1] * page:
+        table = torch.cat([table, torch.full((table.shape[0], -(-wide_table // page) - table.shape[1]), -9, dtype=torch.int32)], dim=1)
+        if weights is not None:
+            weights = torch.cat([weights, weights.new_zeros((*weights.shape[:2], table.shape[1] * page - weights.shape[2]))], dim=2)
     dev = lambda t: None if t is None else (t.cuda() if t.is_contiguous() else t.transpose(1, 2).contiguous().cuda().transpose(1, 2))
     kp, vp, w = dev(kp), dev(vp), dev(weights)
     out = ops.attn_decode(q.cuda(), kp, vp, table.cuda(), lengths.cuda(), counts=dev(counts), weights=w, p=p, **kw)
@@ -81,8 +87,12 @@ def test_attention(case, with_weights):
     if weights is not None:  # what new keys and slots behind the last key hold does not matter
         for b in range(B):
             weights[b, :, max(lengths[b] - int(counts[b]), 0):] = float("nan")
-    out, _, _, w = run(q, kp, vp, table, lens, counts, weights)
+    many = dtype == BF16 and H // Hk * T > 16  # (room for long sequences: the tcgen05 kernel)
     want, w_want, spread = ref.attend(q, kp, vp, table, lens, counts, before, p=0.1)
+    if many:
+        out, _, _, _ = run(q, kp, vp, table, lens, counts, before, wide_table=1 << 20)
+        check_out(out, want, spread, dtype)
+    out, _, _, w = run(q, kp, vp, table, lens, counts, weights)
     check_out(out, want, spread, dtype)
     if with_weights:
         w = w.double().cpu()
@@ -176,16 +186,16 @@ def test_append_and_attend(dtype, D, T):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 def test_many_rows_read_only_what_they_attend(D, bad):
-    """24 query rows per key head: later tokens' keys and values that are not finite, across the border of two tiles of 128."""
-    T = 12
-    kp, vp, table, lens = ref.paged([262, 12, 300], 1, D, 16, BF16)
+    """32 query rows per key head: later tokens' keys and values that are not finite, across the border of two tiles of 128."""
+    T = 16
+    kp, vp, table, lens = ref.paged([262, 16, 300], 1, D, 16, BF16)
     q = torch.randn((3, 2, T, D), generator=torch.Generator().manual_seed(20)).to(BF16)
     counts = torch.full((3,), T, dtype=torch.int32)
     want, _, spread = ref.attend(q, kp, vp, table, lens, counts, p=0.0)
-    for b, n in enumerate((262, 12)):
+    for b, n in enumerate((262, 16)):
         for pool, at in ((vp, n - 1), (kp, n - 2), (vp, n - 3)):
             pool[int(table[b, at // 16]), :, at % 16, 5:9] = bad
-    out, _, _, _ = run(q, kp, vp, table, lens, counts, p=0.0)
+    out, _, _, _ = run(q, kp, vp, table, lens, counts, p=0.0, wide_table=1 << 20)
     check_out(out[:2, :, :T - 3], want[:2, :, :T - 3], spread[:2, :, :T - 3], BF16)
     check_out(out[2], want[2], spread[2], BF16)
     assert not out[:2, :, T - 3, 5:9].isfinite().any() and out[:2, :, T - 3, 9:].isfinite().all()
@@ -193,9 +203,9 @@ def test_many_rows_read_only_what_they_attend(D, bad):
 
 
 def test_many_rows_append_split_and_replay():
-    """24 rows, long and short sequences: new rows are written, the pieces of a sequence joined, twice the same bits."""
+    """28 rows, long and short sequences: new rows are written, the pieces of a sequence joined, twice the same bits."""
     ops = pkg("operators")
-    lengths, Hk, H, T, D, page = [20000, 6, 0, 1500], 2, 8, 6, 128, 32
+    lengths, Hk, H, T, D, page = [20000, 6, 0, 1500], 2, 8, 7, 128, 32
     kp, vp, table, lens = ref.paged(lengths, Hk, D, page, BF16)
     counts = torch.clamp(lens, max=T)
     new = torch.randn((4, T, H + 2 * Hk, D), generator=torch.Generator().manual_seed(21)).to(BF16)
@@ -209,14 +219,16 @@ def test_many_rows_append_split_and_replay():
     dnew = new.cuda()
     dq, dk, dv = (x.transpose(1, 2) for x in (dnew[:, :, :H], dnew[:, :, H:H + Hk], dnew[:, :, H + Hk:]))
     w = torch.zeros((4, Hk, table.shape[1] * page))
-    out, k_got, v_got, got = run(dq, kp, vp, table, lens, counts, w, k=dk, v=dv)
+    out, k_got, v_got, got = run(dq, kp, vp, table, lens, counts, w, wide_table=1 << 19, k=dk, v=dv)
+    got = got[:, :, :w.shape[2]]
     same = lambda a, b: torch.equal(a.cpu().nan_to_num(7.0), b.nan_to_num(7.0))
     assert same(k_got, k_want) and same(v_got, v_want)
     want, w_want, spread = ref.attend(q, k_want, v_want, table, lens, counts, w, p=0.1)
     check_out(out, want, spread, BF16)
     rel = ref.attention_error(6.0 * D**0.5, 20000, D) + (H // Hk * T + 2) * 2.0**-23
     assert bool(((got.double().cpu() - w_want).abs() <= rel * w_want + 1e-30).all())
-    again = ops.attn_decode(dq, k_got, v_got, table.cuda(), lens.cuda(), counts=counts.cuda(), p=0.1)
+    room = torch.cat([table, torch.full((4, (1 << 19) // page - table.shape[1]), -9, dtype=torch.int32)], dim=1).cuda()
+    again = ops.attn_decode(dq, k_got, v_got, room, lens.cuda(), counts=counts.cuda(), p=0.1)
     assert torch.equal(out, again)
 
 
