@@ -19,6 +19,9 @@
 // segments; nothing but the warp itself waits for it. Sums are kept relative to a reference exponent that only moves when a
 // score outgrows it by more than 2^8, so that a step costs one vote instead of a reduction over lanes.
 #pragma once
+#include <atomic>
+#include <type_traits>
+
 #include "cluster.cuh"
 #include "kv_cache.cuh"
 
@@ -300,17 +303,29 @@ __device__ __forceinline__ void add_weights(const DecodeAttn& p, const Segment& 
       const int j = jj + u * N;
       w[u] = j < j1 && j < sg.first && in != nullptr ? in[j] : 0.f;
     }
-    for (int r = 0; r < p.R; ++r) {
-      if (sg.limit(p, r) < 0) continue;
-      const float2 ml = row_ml(r);
-      const float base = ml.x;
-      const float* s = p.scores + (bh * p.R + r) * p.scores_ld;
+    // RB rows' scores are on their way at a time
+    const auto rows = [&](auto rb) {
+      constexpr int RB = decltype(rb)::value;
+      for (int r0 = 0; r0 < p.R; r0 += RB) {
+        float s[RB][U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = jj + u * N;
-        if (j < j1) w[u] = fmaf(ex2(__ldcg(s + j) - base), ml.y, w[u]);  // (other blocks' writes: not from L1)
+        for (int i = 0; i < RB; ++i)
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int r = min(r0 + i, p.R - 1), j = min(jj + u * N, j1 - 1);
+            s[i][u] = __ldcg(p.scores + (bh * p.R + r) * p.scores_ld + j);  // (other blocks' writes: not from L1)
+          }
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          if (r0 + i >= p.R || sg.limit(p, r0 + i) < 0) continue;
+          const float2 ml = row_ml(r0 + i);
+#pragma unroll
+          for (int u = 0; u < U; ++u) w[u] = fmaf(ex2(s[i][u] - ml.x), ml.y, w[u]);
+        }
       }
-    }
+    };
+    if (p.R < 4) rows(std::integral_constant<int, 1>{});
+    else rows(std::integral_constant<int, 4>{});
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (jj + u * N < j1) out[jj + u * N] = w[u];
@@ -862,12 +877,23 @@ attn_decode_weights_kernel(const __grid_constant__ DecodeAttn p, int rows_of_blo
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
-template <typename K>
-bool set_smem(K kernel, int bytes) {
-  if (bytes <= 48 * 1024) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess) return true;
-  (void)cudaGetLastError();
-  return false;
+// Needed once per kernel and device (each kernel is launched with one size), not per launch.
+template <auto Kernel>
+bool set_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  const uint64_t bit = 1ull << dev;
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  done.fetch_or(bit, std::memory_order_release);
+  return true;
 }
 
 // Joins the pieces that the stretches left and, where they are wanted, forms the weights.
@@ -894,7 +920,7 @@ int launch_decode(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
   constexpr int ring = kDecWarps * ring_bytes<Core>(), sums = kDecWarps * Core::kRows * (Core::kDim + 4) * 4;
   if (!pl.split) {
     constexpr int smem = ring > sums ? ring : sums;
-    if (!set_smem(attn_decode_direct_kernel<E, Core>, smem)) return PTJ_ERR_LAUNCH;
+    if (!set_smem<attn_decode_direct_kernel<E, Core>>(smem)) return PTJ_ERR_LAUNCH;
     launch_cluster_k(attn_decode_direct_kernel<E, Core>, dim3(static_cast<unsigned>(d.B * d.Hk * d.nrb * pl.cluster)), kDecWarps * 32,
                      pl.cluster, smem, st, d);
     PTJ_CHECK_LAUNCH();
@@ -904,7 +930,7 @@ int launch_decode(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
     (void)cudaGetLastError();
     return PTJ_ERR_LAUNCH;
   }
-  if (!set_smem(attn_decode_split_kernel<E, Core>, ring)) return PTJ_ERR_LAUNCH;
+  if (!set_smem<attn_decode_split_kernel<E, Core>>(ring)) return PTJ_ERR_LAUNCH;
   launch_k(attn_decode_split_kernel<E, Core>, d.workers / kDecWarps, kDecWarps * 32, ring, st, d);
   PTJ_CHECK_LAUNCH();
   return launch_join<E, Core>(d, pl, st);

@@ -390,7 +390,7 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
 template <int DP>
 int launch_wide(const DecodeAttn& d, const DecodePlan& pl, cudaStream_t st) {
   using Core = CoreWide<DP>;
-  if (!set_smem(attn_decode_wide_kernel<DP>, Core::kSmem)) return PTJ_ERR_LAUNCH;
+  if (!set_smem<attn_decode_wide_kernel<DP>>(Core::kSmem)) return PTJ_ERR_LAUNCH;
   launch_k(attn_decode_wide_kernel<DP>, d.workers, kWideThreads, Core::kSmem, st, d);
   PTJ_CHECK_LAUNCH();
   return launch_join<__nv_bfloat16, Core>(d, pl, st);

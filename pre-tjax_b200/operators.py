@@ -511,22 +511,22 @@ _DECODE_BYTES = {}                       # sizes of a call -> workspace bytes
 
 def _on_current_device(*tensors):
     """Launches go to the current device's stream: tensors elsewhere are refused."""
-    dev = None
+    dev = -2  # not asked for yet
     for t in tensors:
-        if t is None:
-            continue
-        at = t.get_device()
-        if at < 0:
-            raise RuntimeError("tensors must live on a CUDA device: there is no CPU implementation")
-        if dev is None:
-            dev = torch._C._cuda_getDevice()
-        if at != dev:
-            raise RuntimeError(f"tensor on cuda:{at}, but cuda:{dev} is the current device")
+        if t is not None:
+            at = t.get_device()
+            if at != dev:
+                if at < 0:
+                    raise RuntimeError("tensors must live on a CUDA device: there is no CPU implementation")
+                if dev < 0:
+                    dev = torch._C._cuda_getDevice()
+                if at != dev:
+                    raise RuntimeError(f"tensor on cuda:{at}, but cuda:{dev} is the current device")
 
 
 def _ints(t, shape, name):
     """An int32 tensor of this shape; rows of a table may be strided."""
-    if t.dtype != torch.int32 or t.shape != shape or t.stride(-1) != 1 and t.shape[-1] > 1:
+    if t.dtype is not torch.int32 or t.shape != shape or t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must be an int32 tensor of shape {list(shape)} with contiguous rows")
 
 
@@ -536,47 +536,47 @@ def _kv_cache(k_pages, v_pages, page_table, lengths):
     shape, dtype = k_pages.shape, k_pages.dtype
     if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("k_pages and v_pages must share one shape [pages, kv_heads, page_size, d_head]")
-    if v_pages.dtype != dtype:
+    if v_pages.dtype is not dtype:
         raise TypeError("k_pages and v_pages must share a dtype")
     pages, heads, page_size, d = shape
     k0, k1, k2, k3 = k_pages.stride()
     v0, v1, v2, v3 = v_pages.stride()
-    if d > 1 and (k3 != 1 or v3 != 1):
+    if (k3 != 1 or v3 != 1) and d > 1:
         raise ValueError("d_head must be contiguous")
     B, width = page_table.shape
-    if page_table.dtype != torch.int32 or (width > 1 and page_table.stride(1) != 1):
+    t0, t1 = page_table.stride()
+    if page_table.dtype is not torch.int32 or (t1 != 1 and width > 1):
         raise ValueError("page_table must be an int32 tensor [batch, pages of a sequence] with contiguous rows")
-    _ints(lengths, (B,), "lengths")
+    if lengths.dtype is not torch.int32 or lengths.shape != (B,) or (B > 1 and lengths.stride(0) != 1):
+        raise ValueError(f"lengths must be an int32 tensor of shape [{B}]")
     desc = _KV_CACHE.pack(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), B, heads, d, pages,
-                          page_size, width, page_table.stride(0) if B > 1 else width, k0, k1, k2, v0, v1, v2, _dt(k_pages))
+                          page_size, width, t0 if B > 1 else width, k0, k1, k2, v0, v1, v2, _dt(k_pages))
     return desc, (B, heads, d, page_size, width * page_size)
 
 
-def _view(t, shape, dtype, name):
+def _view(t, B, heads, T, d, dtype, name):
     """(address, strides of batch, head and token) of a view of new tokens."""
     if t is None:
         return 0, 0, 0, 0
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must have the cache's dtype {dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}")
-    s0, s1, s2, s3 = t.stride()
-    if s3 != 1 and shape[3] > 1:
-        raise ValueError(f"{name} must be {list(shape)} with d_head contiguous")
+    s0, s1, s2, s3 = t.stride() if t.dim() == 4 else (0, 0, 0, 0)
+    if t.shape != (B, heads, T, d) or (s3 != 1 and d > 1):
+        raise ValueError(f"{name} must be [{B}, {heads}, {T}, {d}] with d_head contiguous")
     return t.data_ptr(), s0, s1, s2
 
 
 def _new_tokens(sizes, q, k, v, out, counts, dtype):
     """(the bytes of the new tokens' descriptor, query heads, tokens)."""
-    B, Hk, d = sizes[:3]
+    B, Hk, d, _, _ = sizes
     some = k if q is None else q
     if some.dim() != 4:
         raise ValueError("new tokens must be [batch, heads, tokens, d_head]")
-    H, T = some.shape[1], some.shape[2]
-    qp, q0, q1, q2 = _view(q, (B, H, T, d), dtype, "q")
-    op, o0, o1, o2 = _view(out, (B, H, T, d), dtype, "out")
-    kp, k0, k1, k2 = _view(k, (B, Hk, T, d), dtype, "k")
-    vp, v0, v1, v2 = _view(v, (B, Hk, T, d), dtype, "v")
+    _, H, T, _ = some.shape
+    qp, q0, q1, q2 = _view(q, B, H, T, d, dtype, "q")
+    op, o0, o1, o2 = _view(out, B, H, T, d, dtype, "out")
+    kp, k0, k1, k2 = _view(k, B, Hk, T, d, dtype, "k")
+    vp, v0, v1, v2 = _view(v, B, Hk, T, d, dtype, "v")
     if counts is not None:
         _ints(counts, (B,), "counts")
     if q is not None and (H % Hk or H < 1):
@@ -587,10 +587,11 @@ def _new_tokens(sizes, q, k, v, out, counts, dtype):
 
 def _attended(weights, sizes, least, name):
     """Width of a tensor of accumulated weights."""
-    if weights.dtype != torch.float32 or weights.dim() != 3 or not weights.is_contiguous() or \
-            weights.shape[0] != sizes[0] or weights.shape[1] != sizes[1] or weights.shape[2] < least:
+    shape = weights.shape
+    if weights.dtype is not torch.float32 or len(shape) != 3 or not weights.is_contiguous() or \
+            shape[0] != sizes[0] or shape[1] != sizes[1] or shape[2] < least:
         raise ValueError(f"{name} must be a contiguous float32 tensor [{sizes[0]}, {sizes[1]}, >= {least}]")
-    return weights.shape[2]
+    return shape[2]
 
 
 def kv_append(k, v, k_pages, v_pages, page_table, lengths, counts=None):
@@ -676,8 +677,7 @@ def kv_evict(k_pages, v_pages, page_table, lengths, weights, budget, recent=0, *
         raise ValueError(f"dst_table must list pages for {most} keys of each sequence")
     width = dst_table.shape[1]
     _ints(dst_table, (B, width), "dst_table")
-    kept = torch.empty((B, Hk, budget), device=weights.device, dtype=torch.int32)
-    new_lengths = torch.empty_like(lengths)
+    kept, new_lengths = lengths.new_empty((B, Hk, budget)), lengths.new_empty(B)
     if B == 0:
         return kept, new_lengths
     rc = _lib.lib().ptj_kv_evict(cache, dst_table.data_ptr(), width, dst_table.stride(0) if B > 1 else width, budget, recent,
@@ -723,8 +723,7 @@ def verify_drafts(target_probs, draft_tokens, uniforms, draft_probs=None, counts
     if counts is not None:
         _ints(counts, (B,), "counts")
     draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
-    tokens = torch.empty((B, K + 1), device=target_probs.device, dtype=torch.int32)
-    accepted = torch.empty(B, device=target_probs.device, dtype=torch.int32)
+    tokens, accepted = draft_tokens.new_empty((B, K + 1)), draft_tokens.new_empty(B)
     if B == 0:
         return tokens, accepted
     rc = _lib.lib().ptj_verify_drafts(target_probs.data_ptr(), ts, _ptr(draft_probs), ds, draft_tokens.data_ptr(), _ptr(counts),
