@@ -22,38 +22,46 @@ DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const Paged
   pl.es = static_cast<int>(dtype_size(c.dtype));
   const bool tc = c.dtype == PTJ_BF16 && c.d_head <= 128;
   pl.dim = c.d_head <= 64 && (tc || pl.es == 4) ? 64 : (c.d_head <= 128 && (tc || pl.es == 4) ? 128 : 256);
+  int64_t segs = 0, longest = 0;
+  int per_sm = 0;
   // More rows than the registers' products take in one pass at memory speed, and tiles enough that the tcgen05 kernel's longer chain
   // and its second pass do not show: 32 rows on 32 caches of 30k keys of 128 take 118 us on it, 198 in registers, 24 rows 112 and
-  // 106; of 2k keys, 32 rows on 128 caches, 57 and 48; 20 rows of 64 elements, 30k keys, 89 and 121.
-  pl.wide = tc && aligned && R > (pl.dim == 64 ? 16 : 24) &&
-            c.batch * c.kv_heads * ceil_div(R, 32) * ceil_div(rows.capacity, 128) >= 12ll * decode_wide_blocks() * kNumSMs;
-  // the core with the fewest blocks of rows (each reads the keys and values again, mostly from L2), of those the smallest
-  if (tc) {
-    const int most = pl.dim == 64 ? 32 : 24;
-    pl.nrb = static_cast<int>(ceil_div(R, most));
-    const int need = static_cast<int>(ceil_div(R, pl.nrb));
-    pl.rows = need <= 4 ? 4 : need <= 8 ? 8 : (need <= 16 ? 16 : most);
-  } else {
-    const int most = pl.dim == 256 ? 4 : 8;
-    pl.nrb = static_cast<int>(ceil_div(R, most));
-    const int need = static_cast<int>(ceil_div(R, pl.nrb));
-    pl.rows = need <= 1 ? 1 : (need <= 4 ? 4 : most);
-  }
-  if (pl.wide) pl.rows = 32;
-  pl.nrb = static_cast<int>(ceil_div(R, pl.rows));
-  pl.prows = R < pl.rows ? R : pl.rows;
-  const int64_t segs = c.batch * c.kv_heads * pl.nrb;
-  const int ks = pl.wide ? 128 : (tc ? 16 : 4096 / (pl.dim * pl.es));  // keys of a step
-  const int64_t longest = ceil_div(rows.capacity, ks);
-  // A cluster per segment, of as many blocks as all fit on the GPU at once and have a step for each of their warps (more come in
-  // a second round: 16 x 12 float32 caches of 512 keys 15.5 us with one block each, 22.3 with two; 8 x 12 bf16 caches of 1024 with
-  // 1, 2, 4, 8 blocks: 15.6, 12.9, 10.8, 16.0). The list of stretches takes over where that could leave a warp more than 64 steps,
-  // or more than 16 with SMs idle.
-  const int per_sm = tc ? decode_tc_blocks(pl.dim, pl.rows) : decode_fma_blocks();
-  pl.cluster = 1;
-  while (pl.cluster < 8 && segs * pl.cluster * 2 <= per_sm * kNumSMs && longest > kDecWarps * pl.cluster) pl.cluster *= 2;
-  const int64_t most = ceil_div(longest, kDecWarps * pl.cluster);  // steps of a warp
-  pl.split = pl.wide || most > 64 || (most > 16 && segs * pl.cluster < kNumSMs) || (weights && pl.nrb > 1);
+  // 106; of 2k keys, 32 rows on 128 caches, 57 and 48; 20 rows of 64 elements, 30k keys, 89 and 121. Where the list of stretches is
+  // needed anyway it is taken from fewer rows on: 8 caches of 131k keys of 128, 12, 16 and 20 rows 109, 113 and 117 us on it, 118, 119
+  // and 210 in registers; one cache of 30k keys, 20 rows, 23 and 30; but 16 rows of 64 elements, 131k keys, 90 and 70.
+  auto share_out = [&](bool wide) {
+    pl.wide = wide;
+    // the core with the fewest blocks of rows (each reads the keys and values again, mostly from L2), of those the smallest
+    if (tc) {
+      const int most = pl.dim == 64 ? 32 : 24;
+      pl.nrb = static_cast<int>(ceil_div(R, most));
+      const int need = static_cast<int>(ceil_div(R, pl.nrb));
+      pl.rows = need <= 4 ? 4 : need <= 8 ? 8 : (need <= 16 ? 16 : most);
+    } else {
+      const int most = pl.dim == 256 ? 4 : 8;
+      pl.nrb = static_cast<int>(ceil_div(R, most));
+      const int need = static_cast<int>(ceil_div(R, pl.nrb));
+      pl.rows = need <= 1 ? 1 : (need <= 4 ? 4 : most);
+    }
+    if (pl.wide) pl.rows = 32;
+    pl.nrb = static_cast<int>(ceil_div(R, pl.rows));
+    pl.prows = R < pl.rows ? R : pl.rows;
+    segs = c.batch * c.kv_heads * pl.nrb;
+    const int ks = pl.wide ? 128 : (tc ? 16 : 4096 / (pl.dim * pl.es));  // keys of a step
+    longest = ceil_div(rows.capacity, ks);
+    // A cluster per segment, of as many blocks as all fit on the GPU at once and have a step for each of their warps (more come in
+    // a second round: 16 x 12 float32 caches of 512 keys 15.5 us with one block each, 22.3 with two; 8 x 12 bf16 caches of 1024 with
+    // 1, 2, 4, 8 blocks: 15.6, 12.9, 10.8, 16.0). The list of stretches takes over where that could leave a warp more than 64 steps,
+    // or more than 16 with SMs idle.
+    per_sm = tc ? decode_tc_blocks(pl.dim, pl.rows) : decode_fma_blocks();
+    pl.cluster = 1;
+    while (pl.cluster < 8 && segs * pl.cluster * 2 <= per_sm * kNumSMs && longest > kDecWarps * pl.cluster) pl.cluster *= 2;
+    const int64_t most = ceil_div(longest, kDecWarps * pl.cluster);  // steps of a warp
+    pl.split = pl.wide || most > 64 || (most > 16 && segs * pl.cluster < kNumSMs) || (weights && pl.nrb > 1);
+  };
+  share_out(tc && aligned && R > (pl.dim == 64 ? 16 : 24) &&
+            c.batch * c.kv_heads * ceil_div(R, 32) * ceil_div(rows.capacity, 128) >= 12ll * decode_wide_blocks() * kNumSMs);
+  if (tc && aligned && pl.split && R > (pl.dim == 64 ? 16 : 8)) share_out(true);
   if (pl.split) {
     pl.workers = pl.wide ? decode_wide_blocks() * kNumSMs : per_sm * kNumSMs * kDecWarps;
     // small stretches: where sequences may be long enough for 32 steps of a warp, and pieces of a few rows are small beside them

@@ -232,6 +232,29 @@ def test_many_rows_append_split_and_replay():
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("D", [64, 120, 128])
+@pytest.mark.parametrize("H,T", [(12, 1), (4, 5), (8, 4), (5, 7)])
+def test_many_rows_of_a_long_sequence(H, T, D, aligned):
+    """Few caches, one of them long: the work is shared out over its length, on and off 16-byte boundaries."""
+    lengths = [9000, 5, 0, 300]
+    kp, vp, table, lens = ref.paged(lengths, 1, D, 16, BF16)
+    counts = torch.clamp(lens, max=T)
+    q = torch.randn((4, H, T, D), generator=torch.Generator().manual_seed(22)).to(BF16)
+    w = torch.rand((4, 1, table.shape[1] * 16), generator=torch.Generator().manual_seed(23))
+    want, w_want, spread = ref.attend(q, kp, vp, table, lens, counts, w, p=0.1)
+    off = lambda t: t.cuda() if aligned else torch.cat([t.new_zeros(1), t.reshape(-1)]).cuda()[1:].view(t.shape)
+    got = w.cuda()
+    out = pkg("operators").attn_decode(off(q), off(kp), off(vp), table.cuda(), lens.cuda(), counts=counts.cuda(), p=0.1, weights=got)
+    check_out(out, want, spread, BF16)
+    got, rel = got.double().cpu(), (H * T + 2) * 2.0**-23
+    for b, n in enumerate(lengths):
+        bound = rel + ref.attention_error(6.0 * D**0.5, n, D)
+        assert bool(((got[b, :, :n] - w_want[b, :, :n]).abs() <= bound * w_want[b, :, :n] + 1e-30).all())
+    assert torch.equal(out, pkg("operators").attn_decode(off(q), off(kp), off(vp), table.cuda(), lens.cuda(), counts=counts.cuda(),
+                                                         p=0.1, weights_out=torch.empty_like(w, device="cuda")))
+
+
 def test_append_of_a_prompt():
     """Whole prompts of different lengths, padded on the right, go into empty caches."""
     ops = pkg("operators")
