@@ -430,8 +430,8 @@ int ptj_kv_append(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, void*
 /* Attention of the new tokens over the cache, evaluation semantics (the output is multiplied by 1 - p):
  *   out = (1 - p) softmax(q K^T / sqrt(d_head)) V over keys 0 .. position of the token.
  * With tokens->k and ->v the new rows are written to their pages as by ptj_kv_append and attended to. A token behind counts[b]
- * or below position 0 attends nothing: a zero row. out overlaps no input. Rows read only the keys they attend: what lies in other slots, an infinity
- * or a NaN included, reaches no output. Softmax statistics and sums are float32.
+ * or below position 0 attends nothing: a zero row. out overlaps no input. Rows read only the keys they attend: what lies in
+ * other slots, an infinity or a NaN included, reaches no output. Softmax statistics and sums are float32.
  * weights_out (optional, float[batch, kv_heads, weights_ld], weights_ld >= table_width * page_size): the attention that each
  * key received, summed over the query heads of its key head and the new tokens, plus weights (same layout; NULL = 0; may be
  * weights_out itself) for keys that are not new. Slots from lengths[b] on are left as they were.
@@ -442,7 +442,7 @@ int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, flo
 /* Cuts every sequence with more than `budget` keys down to `budget`, for each key head on its own: the last `recent` keys stay
  * (recent <= budget) and of the others those with the largest weights (float[batch, kv_heads, weights_ld], weights_ld >=
  * table_width * page_size), the lowest positions among equals; a NaN ranks below everything. Keys stay in order: key kept[i]
- * becomes key i of dst_table (rows of dst_ld entries; dst_table == cache->table: in place). Other sequences are only copied
+ * becomes key i of dst_table (rows of dst_ld entries; dst_table == cache->table, with its table_ld: in place). Other sequences are only copied
  * to dst_table. Destination pages of different sequences differ. In place is what the address says: a copy of cache->table, or
  * any other table that names a source page, is an error that is not noticed, since rows then move in no order.
  *   kept         int32[batch, kv_heads, budget]: positions that stay, -1 behind them

@@ -15,8 +15,8 @@
 //   128k keys of 8 heads of 128). A segment within one stretch is written by its warp; pieces of others (at most two per stretch)
 //   go to the workspace with their reference exponent and sum and are joined, in order, by a second kernel.
 //
-// Who computes a stretch does not matter to it: results do not depend on timing. A warp owns a ring of steps in shared memory that cp.async fills ahead of the arithmetic, across
-// segments; nothing but the warp itself waits for it. Sums are kept relative to a reference exponent that only moves when a
+// Who computes a stretch does not matter to it: results do not depend on timing. A warp owns a ring of steps in shared memory that
+// cp.async fills ahead of the arithmetic, across segments; nothing but the warp itself waits for it. Sums are kept relative to a reference exponent that only moves when a
 // score outgrows it by more than 2^8, so that a step costs one vote instead of a reduction over lanes.
 #pragma once
 #include <atomic>

@@ -314,7 +314,8 @@ extern "C" int ptj_kv_evict(const ptj_kv_cache* cache, const int32_t* dst_table,
     return PTJ_ERR_BAD_SHAPE;
   const int64_t most = budget < p.rows.capacity ? budget : p.rows.capacity;  // keys that a sequence keeps at most
   if (weights_ld < p.rows.capacity || (weights_out && weights_out_ld < most) || dst_width < ceil_div(most, cache->page_size) ||
-      (weights_out == weights && weights_out_ld != weights_ld))
+      (weights_out == weights && weights_out_ld != weights_ld) ||
+      (dst_table == cache->table && cache->batch > 1 && dst_ld != cache->table_ld))
     return PTJ_ERR_BAD_SHAPE;
   if (ptj_device_check() != PTJ_OK || (p.rows.fault = tc::fault_word()) == nullptr) return PTJ_ERR_DEVICE;
   p.dst_table = dst_table;

@@ -184,10 +184,11 @@ def test_library_refuses_on_its_own():
     assert lib.ptj_attn_decode_workspace_bytes(None, None, 0) == 0
     assert call(good(kv_heads=1), new(heads=4097)) == -1  # query rows of a key head
     assert lib.ptj_kv_append(ctypes.byref(good()), ctypes.byref(new()), None) == -1
-    evict = lambda dst=16, width=1, ld=1, budget=8, recent=0, w=16, wld=32, wo=16, wold=32, kept=16, nl=32: lib.ptj_kv_evict(
+    evict = lambda dst=16, width=1, ld=2, budget=8, recent=0, w=16, wld=32, wo=16, wold=32, kept=16, nl=32: lib.ptj_kv_evict(
         ctypes.byref(good()), dst, width, ld, budget, recent, w, wld, wo, wold, kept, nl, None)
     for kw in (dict(dst=None), dict(width=0), dict(ld=0), dict(budget=0), dict(recent=9), dict(recent=-1), dict(w=None), dict(wld=31),
-               dict(wold=7, wo=48), dict(wold=31), dict(kept=None), dict(nl=None), dict(nl=16), dict(budget=17)):
+               dict(wold=7, wo=48), dict(wold=31), dict(kept=None), dict(nl=None), dict(nl=16), dict(budget=17),
+               dict(ld=1)):  # (in place with rows of another length)
         assert evict(**kw) == -1, kw
     two = (ctypes.c_int64 * 2)(24, 8)
     verify = lambda t=16, ts=two, d=None, ds=None, tok=16, u=16, out=16, acc=16, B=2, K=2, V=8, dt=0: lib.ptj_verify_drafts(
