@@ -103,7 +103,7 @@ def probabilities(logits: torch.Tensor, temperature: float = 1.0) -> torch.Tenso
 
 def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, uniforms: torch.Tensor, drafts: int = 4,
               temperature: float = 1.0, prompt_lens: torch.Tensor = None, page_size: int = 16, budget: int = None, recent: int = 0):
-    """Samples at least new_tokens tokens behind each prompt: (tokens int32 [B, new_tokens], rounds).
+    """Samples new_tokens tokens behind each prompt: (tokens int32 [B, new_tokens], rounds). params, draft_params: as for decode_step.
 
     prompt int [B, P], padded on the right; prompt_lens int32 [B] (default P). Every round the draft model (same vocabulary and
     positions) proposes `drafts` tokens and the target accepts a part of them and adds one of its own, so that tokens are
@@ -112,7 +112,7 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
     when they run out. The target's cache is cut down to `budget` keys per head, the last `recent` among them, whenever it
     may hold that many more (None: it grows). One host synchronisation per round (the fewest tokens of a sequence so far)."""
     B, P = prompt.shape
-    dtype = params[0][0].dtype
+    dtype = (params[1]["w_emb"] if isinstance(params[0], GPT2Config) else params[0][0]).dtype
     target, draft = (_weights(x, dtype) for x in (params, draft_params))
     if target[0].vocab != draft[0].vocab:
         raise ValueError("target and draft model must share a vocabulary")
@@ -121,8 +121,8 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
     longest = P + new_tokens + drafts + 1
     if longest > min(target[0].seq, draft[0].seq):
         raise ValueError(f"{longest} positions (prompt, new tokens and drafts ahead) exceed the models'")
-    if budget is not None and not 0 <= recent <= budget:
-        raise ValueError("speculate needs 0 <= recent <= budget")
+    if budget is not None and not (0 <= recent <= budget and budget >= 1):
+        raise ValueError("speculate needs 0 <= recent <= budget and budget >= 1")
     room = longest if budget is None else min(longest, max(P, 2 * budget) + drafts + 1)
     device = prompt.device
     cache = PagedCache(target[0], B, room, page_size, dtype, device, track_weights=budget is not None)

@@ -184,3 +184,16 @@ def test_bf16_weights_run_together():
     tokens, rounds = sv.speculate(params, params, prompt, 40, u, drafts=4, budget=16, recent=8)
     assert tokens.shape == (5, 40) and bool(((tokens >= 0) & (tokens < V)).all()) and ops.last_kernel_fault() == 0
     assert rounds <= 40
+
+
+def test_speculation_takes_a_configuration_and_weights():
+    """(GPT2Config, Weights) in place of the pytree: the same tokens."""
+    sv, gpt2, ops = pkg("serving"), pkg("gpt2"), pkg("operators")
+    params = on_gpu(models(6, torch.bfloat16), torch.bfloat16)
+    cfg = gpt2.config_from_params(params, ops.DROPOUT_RATE)
+    laid_out = (cfg, gpt2.Weights.from_pytree(params, cfg, torch.bfloat16))
+    g = torch.Generator().manual_seed(8)
+    prompt = torch.randint(1, V, (2, 9), generator=g, dtype=torch.int32).cuda()
+    u = torch.rand((20, 2, 6), generator=g).cuda()
+    runs = [sv.speculate(x, x, prompt, 12, u, drafts=2) for x in (params, laid_out)]
+    assert torch.equal(runs[0][0], runs[1][0]) and runs[0][1] == runs[1][1]

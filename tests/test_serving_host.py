@@ -218,7 +218,7 @@ def test_cache_and_speculation_refusals():
 
 
 @pytest.mark.parametrize("change", [dict(drafts=0), dict(uniforms=torch.zeros(4, 2, 4)), dict(uniforms=torch.zeros(4, 3, 10)),
-                                    dict(new_tokens=40), dict(budget=3, recent=4)])
+                                    dict(new_tokens=40), dict(budget=3, recent=4), dict(budget=0)])
 def test_speculation_refusals(change, monkeypatch):
     sv, gpt2 = pkg("serving"), pkg("gpt2")
     cfg = gpt2.GPT2Config(vocab=10, dim=8, layers=1, heads=2, ffn=16, seq=32)
