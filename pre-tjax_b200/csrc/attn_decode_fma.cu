@@ -15,6 +15,7 @@ struct CoreFma {
   static constexpr int LPK = DP / VEC < 32 ? DP / VEC : 32, NV = DP / (VEC * LPK), KPW = 32 / LPK, W = VEC * NV;
   static constexpr int KS = 4096 / kRowBytes, KB = KS / KPW;  // keys of a step, of a lane
   static constexpr int REP = LPK / KB;                        // lanes that end with the same score
+  static constexpr int RG = RB < 4 ? RB : 4;                  // rows whose scores are on their way at a time
   static constexpr int kDepth = 3;
   static constexpr int kBlocks = 2;
   static constexpr int P = W / 2;  // pairs of elements: products run two elements wide
@@ -72,63 +73,86 @@ struct CoreFma {
     for (int e = 0; e < KB; ++e) read(stage, e * KPW + grp, k[e]);
 #pragma unroll
     for (int e = 0; e < KB; ++e) read(stage, KS + e * KPW + grp, v[e]);
+    const int own = sub_lane / REP * KPW + grp;  // place in the step of the key whose score this lane ends with
+    // RG rows side by side: one row's chain of shuffles, exponential and shuffles is long
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const int row = sg.rb * kRows + r;
-      if (RB > 1 && row >= p.R) break;
-      float s[KB];
+    for (int r0 = 0; r0 < RB; r0 += RG) {
+      const int row0 = sg.rb * kRows + r0;
+      if (RB > RG && row0 >= p.R) break;
+      float s[RG][KB];
 #pragma unroll
-      for (int e = 0; e < KB; ++e) {
-        uint64_t d = f2_mul(q[r][0], k[e][0]);
-#pragma unroll
-        for (int i = 1; i < P; ++i) d = f2_fma(q[r][i], k[e][i], d);
-        float lo, hi;
-        f2_unpack(d, lo, hi);
-        s[e] = lo + hi;
-      }
-      // to one score per lane: that of key `own`
-#pragma unroll
-      for (int n = KB / 2, x = LPK / 2; x > 0; n /= 2, x /= 2) {
-        if (n > 0) {
-          const bool up = sub_lane & x;
-#pragma unroll
-          for (int e = 0; e < n; ++e) {
-            const float give = up ? s[e] : s[e + n], stay = up ? s[e + n] : s[e];
-            s[e] = stay + __shfl_xor_sync(0xffffffffu, give, x);
-          }
-        } else {
-          s[0] += __shfl_xor_sync(0xffffffffu, s[0], x);
-        }
-      }
-      const int own = sub_lane / REP * KPW + grp;  // place in the step
-      float mine = s[0];
-      if (edge && (!((present >> own) & 1u) || j0 + own > limit[r])) mine = -INFINITY;
-      if (p.scores != nullptr && sub_lane % REP == 0 && j0 + own < sg.n) sg.score_row(p, row)[j0 + own] = mine * p.scale;
-      if (__any_sync(0xffffffffu, mine > over[r])) {
-        const float m = fmaxf(warp_max(mine) * p.scale, ref[r]);
-        const float f = rebase(ref[r], m);
-        ref[r] = m;
-        over[r] = (m + kDecLazy) * p.unscale;
-        sum[r] *= f;
-#pragma unroll
-        for (int i = 0; i < P; ++i) o[r][i] = f2_mul(o[r][i], f2_pack(f, f));
-      }
-      mine = ex2(fmaf(mine, p.scale, -ref[r]));
-      sum[r] += mine;
-#pragma unroll
-      for (int e = 0; e < KB; ++e) s[e] = __shfl_sync(0xffffffffu, mine, e * REP, LPK);
-      if (edge) {  // zero times what is not finite is not zero
+      for (int r = 0; r < RG; ++r)
 #pragma unroll
         for (int e = 0; e < KB; ++e) {
-          if (j0 + e * KPW + grp > limit[r]) continue;
+          uint64_t d = f2_mul(q[r0 + r][0], k[e][0]);
 #pragma unroll
-          for (int i = 0; i < P; ++i) o[r][i] = f2_fma(f2_pack(s[e], s[e]), v[e][i], o[r][i]);
+          for (int i = 1; i < P; ++i) d = f2_fma(q[r0 + r][i], k[e][i], d);
+          float lo, hi;
+          f2_unpack(d, lo, hi);
+          s[r][e] = lo + hi;
         }
-      } else {
+      // to one score per lane and row
 #pragma unroll
-        for (int e = 0; e < KB; ++e)
+      for (int n = KB / 2, x = LPK / 2; x > 0; n /= 2, x /= 2)
 #pragma unroll
-          for (int i = 0; i < P; ++i) o[r][i] = f2_fma(f2_pack(s[e], s[e]), v[e][i], o[r][i]);
+        for (int r = 0; r < RG; ++r) {
+          if (n > 0) {
+            const bool up = sub_lane & x;
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+              const float give = up ? s[r][e] : s[r][e + n], stay = up ? s[r][e + n] : s[r][e];
+              s[r][e] = stay + __shfl_xor_sync(0xffffffffu, give, x);
+            }
+          } else {
+            s[r][0] += __shfl_xor_sync(0xffffffffu, s[r][0], x);
+          }
+        }
+      float mine[RG];
+      bool moves = false;
+#pragma unroll
+      for (int r = 0; r < RG; ++r) {
+        mine[r] = s[r][0];
+        if (edge && (!((present >> own) & 1u) || j0 + own > limit[r0 + r])) mine[r] = -INFINITY;
+        moves |= mine[r] > over[r0 + r];
+      }
+      if (p.scores != nullptr && sub_lane % REP == 0 && j0 + own < sg.n)
+#pragma unroll
+        for (int r = 0; r < RG; ++r)
+          if (row0 + r < p.R) sg.score_row(p, row0 + r)[j0 + own] = mine[r] * p.scale;
+      if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+        for (int r = 0; r < RG; ++r) {
+          const float m = fmaxf(warp_max(mine[r]) * p.scale, ref[r0 + r]);
+          const float f = rebase(ref[r0 + r], m);
+          ref[r0 + r] = m;
+          over[r0 + r] = (m + kDecLazy) * p.unscale;
+          sum[r0 + r] *= f;
+#pragma unroll
+          for (int i = 0; i < P; ++i) o[r0 + r][i] = f2_mul(o[r0 + r][i], f2_pack(f, f));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RG; ++r) {
+        mine[r] = ex2(fmaf(mine[r], p.scale, -ref[r0 + r]));
+        sum[r0 + r] += mine[r];
+      }
+#pragma unroll
+      for (int r = 0; r < RG; ++r) {
+#pragma unroll
+        for (int e = 0; e < KB; ++e) s[r][e] = __shfl_sync(0xffffffffu, mine[r], e * REP, LPK);
+        if (edge) {  // zero times what is not finite is not zero
+#pragma unroll
+          for (int e = 0; e < KB; ++e) {
+            if (j0 + e * KPW + grp > limit[r0 + r]) continue;
+#pragma unroll
+            for (int i = 0; i < P; ++i) o[r0 + r][i] = f2_fma(f2_pack(s[r][e], s[r][e]), v[e][i], o[r0 + r][i]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < KB; ++e)
+#pragma unroll
+            for (int i = 0; i < P; ++i) o[r0 + r][i] = f2_fma(f2_pack(s[r][e], s[r][e]), v[e][i], o[r0 + r][i]);
+        }
       }
     }
   }
