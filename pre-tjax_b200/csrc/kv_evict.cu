@@ -1,6 +1,6 @@
 // Eviction from a paged key-value cache by accumulated attention weight.
 //
-// Two launches: one finds the keys that stay, one moves their rows.
+// Two launches: one finds the keys that stay, one moves their rows. (Few small caches: one launch for both.)
 //
 // Which stay: the weights are ordered as unsigned integers; the weight of the last key to stay is found digit by digit (8
 // bits) from histograms in shared memory. Above it all stay, of its equals the first ones. A cluster of C blocks shares a cache,
@@ -89,12 +89,9 @@ __device__ __forceinline__ void find_digit(SelectShared& sm, uint32_t (&hist)[kC
   __syncthreads();
 }
 
+// Positions that stay of the cache of cluster blockIdx.x / C.
 template <int C>
-__global__ void __launch_bounds__(kSelThreads)
-select_kernel(const __grid_constant__ Evict p) {
-  grid_dep_sync();
-  extern __shared__ __align__(16) uint8_t smem[];
-  SelectShared& sm = *reinterpret_cast<SelectShared*>(smem);
+__device__ __forceinline__ void select(const Evict& p, SelectShared& sm) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(cluster_rank<C>());
   const int seg = blockIdx.x / C, b = seg / p.Hk;
@@ -191,60 +188,44 @@ select_kernel(const __grid_constant__ Evict p) {
   }
 }
 
-// x: segment and column; y: keys and values, or weights; z: stretch of rows. A round: `round` rows, whose places (page and slot, from
-// and to) one thread each looks up; the next round's are looked up while this one's rows are on their way.
-template <typename V>
-__global__ void __launch_bounds__(kMoveThreads, 2)
-move_kernel(const __grid_constant__ Evict p) {
+template <int C>
+__global__ void __launch_bounds__(kSelThreads)
+select_kernel(const __grid_constant__ Evict p) {
   grid_dep_sync();
-  constexpr int U = kMovePieces;
-  __shared__ int2 from_s[3][kMoveRows], to_s[3][kMoveRows];
-  const int tid = threadIdx.x, seg = blockIdx.x / p.cols, col = blockIdx.x % p.cols, b = seg / p.Hk, h = seg % p.Hk;
-  const bool pools = blockIdx.y == 0, ordered = pools ? p.pools_in_place : p.weights_in_place;
-  const int keep = min(p.rows.length(p.lengths, b), p.budget);
-  const int32_t* kept = p.kept + static_cast<int64_t>(seg) * p.budget;
-  if (ordered && blockIdx.z > 0) return;
-  const int first = ordered ? 0 : blockIdx.z * p.chunk, last = ordered ? keep : min(keep, first + p.chunk);
-  if (first >= last) return;
-  if (!pools) {  // in place they are moved as rows of one column are
-    if (col != 0) return;
-    const float* w = p.weights + seg * p.weights_ld;
-    float* out = p.weights_out + seg * p.weights_out_ld;
-    for (int i0 = first; i0 < last; i0 += kMoveThreads * U) {
-      float x[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int i = i0 + k * kMoveThreads + tid;
-        if (i < last) x[k] = w[kept[i]];
-      }
-      if (ordered) __syncthreads();
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int i = i0 + k * kMoveThreads + tid;
-        if (i < last) out[i] = x[k];
-      }
-    }
-    return;
-  }
+  extern __shared__ __align__(16) uint8_t smem[];
+  select<C>(p, *reinterpret_cast<SelectShared*>(smem));
+}
+
+// Places of a round's rows, page and slot, from and to
+struct Places {
+  int2 from[3][kMoveRows], to[3][kMoveRows];
+};
+
+// Moves pieces [c_first, c_first + per_col) of rows [first, last) that stay, NT threads, U pieces of a thread at a time. A round: at
+// most `round` rows, whose places one thread each looks up; the next round's are looked up while this one's rows are on their way.
+template <typename V, int NT, int U>
+__device__ __forceinline__ void move_rows(const Evict& p, Places& at_s, int b, int h, const int32_t* kept, int c_first, int per_col,
+                                          int round, int first, int last) {
+  const int tid = threadIdx.x;
   const int32_t *src = p.rows.table + b * p.rows.table_ld, *dst = p.dst_table + b * p.dst_ld;
   auto look_up = [&](int r0, int buf) {
-    for (int i = tid; i < p.round && r0 + i < last; i += kMoveThreads) {
+    for (int i = tid; i < round && r0 + i < last; i += NT) {
       const int r = r0 + i, j = kept[r];
       int64_t pf = -1, pt = -1;
       int sf = 0, st = 0;
-      const bool stays = ordered && j == r;  // it lies where it belongs
+      const bool stays = p.pools_in_place && j == r;  // it lies where it belongs
       if (stays || !p.rows.locate(src, j, pf, sf) || !p.rows.locate(dst, r, pt, st)) pf = pt = -1;
-      from_s[buf][i] = make_int2(static_cast<int>(pf), sf);
-      to_s[buf][i] = make_int2(static_cast<int>(pt), st);  // page -1: nothing is moved
+      at_s.from[buf][i] = make_int2(static_cast<int>(pf), sf);
+      at_s.to[buf][i] = make_int2(static_cast<int>(pt), st);  // page -1: nothing is moved
     }
   };
-  const int row0 = tid / p.per_col, c0 = tid % p.per_col, rows_on = kMoveThreads / p.per_col, c_on = kMoveThreads % p.per_col;
+  const int row0 = tid / per_col, c0 = tid % per_col, rows_on = NT / per_col, c_on = NT % per_col;
   look_up(first, 0);
   __syncthreads();
   int buf = 0;
-  for (int r0 = first; r0 < last; r0 += p.round) {
+  for (int r0 = first; r0 < last; r0 += round) {
     V x[U], y[U];
-    const int n = min(p.round, last - r0);
+    const int n = min(round, last - r0);
     int row = row0, c = c0;
     auto on = [&](int k, int2& place, const int2* places) {  // k-th piece of this thread
       if (k == 0) {
@@ -253,35 +234,87 @@ move_kernel(const __grid_constant__ Evict p) {
       } else {
         row += rows_on;
         c += c_on;
-        if (c >= p.per_col) {
-          c -= p.per_col;
+        if (c >= per_col) {
+          c -= per_col;
           ++row;
         }
       }
-      if (row >= n || col * p.per_col + c >= p.pieces) return false;
+      if (row >= n || c_first + c >= p.pieces) return false;
       place = places[row];
       return place.x >= 0;
     };
     int2 at;
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      if (on(k, at, from_s[buf])) {
-        const int piece = col * p.per_col + c;
-        x[k] = reinterpret_cast<const V*>(p.pool[0] + p.rows.offset(0, at.x, h, at.y))[piece];
-        y[k] = reinterpret_cast<const V*>(p.pool[1] + p.rows.offset(1, at.x, h, at.y))[piece];
+      if (on(k, at, at_s.from[buf])) {
+        x[k] = reinterpret_cast<const V*>(p.pool[0] + p.rows.offset(0, at.x, h, at.y))[c_first + c];
+        y[k] = reinterpret_cast<const V*>(p.pool[1] + p.rows.offset(1, at.x, h, at.y))[c_first + c];
       }
     const int next = buf == 2 ? 0 : buf + 1;  // (a thread may still store to the places of the round before)
-    if (r0 + p.round < last) look_up(r0 + p.round, next);
+    if (r0 + round < last) look_up(r0 + round, next);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      if (on(k, at, to_s[buf])) {
-        const int piece = col * p.per_col + c;
-        reinterpret_cast<V*>(p.pool[0] + p.rows.offset(0, at.x, h, at.y))[piece] = x[k];
-        reinterpret_cast<V*>(p.pool[1] + p.rows.offset(1, at.x, h, at.y))[piece] = y[k];
+      if (on(k, at, at_s.to[buf])) {
+        reinterpret_cast<V*>(p.pool[0] + p.rows.offset(0, at.x, h, at.y))[c_first + c] = x[k];
+        reinterpret_cast<V*>(p.pool[1] + p.rows.offset(1, at.x, h, at.y))[c_first + c] = y[k];
       }
     buf = next;
   }
+}
+
+// The weights of rows [first, last) that stay; in order: a round's are read before any is written.
+template <int NT, int U>
+__device__ __forceinline__ void move_weights(const Evict& p, int seg, const int32_t* kept, int first, int last) {
+  const float* w = p.weights + seg * p.weights_ld;
+  float* out = p.weights_out + seg * p.weights_out_ld;
+  for (int i0 = first; i0 < last; i0 += NT * U) {
+    float x[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + k * NT + static_cast<int>(threadIdx.x);
+      if (i < last) x[k] = w[kept[i]];
+    }
+    if (p.weights_in_place) __syncthreads();
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + k * NT + static_cast<int>(threadIdx.x);
+      if (i < last) out[i] = x[k];
+    }
+  }
+}
+
+// x: segment and column; y: keys and values, or weights; z: stretch of rows.
+template <typename V>
+__global__ void __launch_bounds__(kMoveThreads, 2)
+move_kernel(const __grid_constant__ Evict p) {
+  grid_dep_sync();
+  __shared__ Places at_s;
+  const int seg = blockIdx.x / p.cols, col = blockIdx.x % p.cols, b = seg / p.Hk, h = seg % p.Hk;
+  const bool pools = blockIdx.y == 0, ordered = pools ? p.pools_in_place : p.weights_in_place;
+  const int keep = min(p.rows.length(p.lengths, b), p.budget);
+  const int32_t* kept = p.kept + static_cast<int64_t>(seg) * p.budget;
+  if (ordered && blockIdx.z > 0) return;
+  const int first = ordered ? 0 : blockIdx.z * p.chunk, last = ordered ? keep : min(keep, first + p.chunk);
+  if (first >= last) return;
+  if (pools) move_rows<V, kMoveThreads, kMovePieces>(p, at_s, b, h, kept, col * p.per_col, p.per_col, p.round, first, last);
+  else if (col == 0) move_weights<kMoveThreads, kMovePieces>(p, seg, kept, first, last);  // in place as rows of one column are
+}
+
+// Both at once, a block per cache.
+__global__ void __launch_bounds__(kSelThreads)
+evict_kernel(const __grid_constant__ Evict p) {
+  grid_dep_sync();
+  extern __shared__ __align__(16) uint8_t smem[];
+  static_assert(sizeof(Places) <= sizeof(SelectShared), "");
+  select<1>(p, *reinterpret_cast<SelectShared*>(smem));
+  __syncthreads();  // all positions are there, all weights and all of the shared memory have been read
+  constexpr int U = 2;
+  const int seg = blockIdx.x, b = seg / p.Hk, keep = min(p.rows.length(p.lengths, b), p.budget);
+  const int32_t* kept = p.kept + static_cast<int64_t>(seg) * p.budget;
+  if (p.weights_out != nullptr) move_weights<kSelThreads, U>(p, seg, kept, 0, keep);
+  move_rows<uint4, kSelThreads, U>(p, *reinterpret_cast<Places*>(smem), b, seg % p.Hk, kept, 0, p.pieces,
+                                   min(kSelThreads * U / p.pieces, kMoveRows), 0, keep);
 }
 
 void launch_select(const Evict& p, int segs, cudaStream_t st) {
@@ -353,6 +386,14 @@ extern "C" int ptj_kv_evict(const ptj_kv_cache* cache, const int32_t* dst_table,
   p.chunks = static_cast<int>(ceil_div(most, p.chunk));
   const bool one = in_place && (weights_out == weights || !weights_out);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // Few small caches: one launch. A second one takes the caller's thread 3 us, more than a block needs for 96 KB of keys. 8 x 12 bf16
+  // caches of 1024 keys of 64 cut to 512: 17.4 us a call with two launches, 15.3 with one (replayed from a graph 14.7 and 13.3); 4 x 8
+  // of 2048 of 128 to 1024: 17 and 30 replayed.
+  if (wide && segs <= kNumSMs && p.rows.capacity <= 4096 && most * p.rows.row_bytes <= 96 * 1024) {
+    launch_k(evict_kernel, dim3(static_cast<unsigned>(segs)), kSelThreads, sizeof(SelectShared), st, p);
+    PTJ_CHECK_LAUNCH();
+    return PTJ_OK;
+  }
   launch_select(p, segs, st);
   PTJ_CHECK_LAUNCH();
   const dim3 grid(static_cast<unsigned>(segs) * p.cols, weights_out ? 2 : 1, one ? 1 : p.chunks);

@@ -66,6 +66,12 @@ def test_long_sequences(n, budget, recent):
     check([n, 17, n // 3], 2, 64, 64, BF16, budget, recent)
 
 
+@pytest.mark.parametrize("n,budget,recent", [(5000, 1024, 128), (40000, 10007, 1000), (4096, 4000, 1), (2000, 700, 700)])
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F32, 64)])
+def test_long_sequences_into_other_pages(n, budget, recent, dtype, D):
+    check([n, 17, n // 3], 2, D, 48, dtype, budget, recent, in_place=False)
+
+
 def test_equal_weights_and_special_values():
     """Ties go to the lowest position; both zeros are equal, infinities rank at the ends, a NaN below all."""
     w = torch.zeros((1, 5, 400))
