@@ -1,14 +1,14 @@
 // Attention of new tokens over a paged cache, bf16 heads of up to 128: tensor cores.
 //
 // S^T = K Q^T and O^T = V^T P^T with m16n8k16: keys, then head elements, are the 16 rows of a product, eight query rows its columns,
-// so one to eight rows cost the same and each further eight half as much again. Which head element sits at which k of a product
+// so one to eight rows cost the same. Which head element sits at which k of a product
 // is free as long as Q and K agree, so a lane's 16 bytes of a key are its operands of two products, and its 16 bytes of four
 // values turn into operands of four products by picking halves of pairs (the transposition that V needs). P^T comes from S^T by
 // transposing 8 x 8 blocks in registers. Probabilities are multiplied in two bf16 parts (16 bits): rounding them to one would
 // cost as much accuracy as rounding the output does. Up to four rows take four columns with their first parts and the other four
-// with their second ones, so the second part costs nothing; more rows take a second product. A product takes 32 cycles of an SM's
-// quarter here (the form with operands in registers; 24 of them a step of 16 keys of 128 elements kept its pipe busy half of
-// the time), which is what bounds many rows.
+// with their second ones, so the second part costs nothing; more rows take a second product. The products are not what bounds it (one
+// takes 8 cycles of an SM's quarter, 21 in a chain): up to 16 rows memory does (4 x 8 caches of 30k keys of 128, 1, 8 and 16 rows: 91,
+// 92 and 95 us, floor 75), 24 rows fill the registers (103 us) and leave nothing for the list of stretches.
 #include "attn_decode.cuh"
 
 namespace ptj {

@@ -1,6 +1,6 @@
 // Attention of new tokens over a paged cache, bf16, many query rows per key head (drafted tokens of shared heads): tcgen05.
 //
-// The kernels with operands in registers are bound by their products beyond 16 rows (attn_decode_tc.cu). Here a block takes 128 keys
+// The kernels with operands in registers run out of registers beyond 16 to 24 rows (attn_decode_tc.cu). Here a block takes 128 keys
 // at a time: S^T = K Q^T (128 keys x 32 rows) and O^T += V^T P^T (128 elements x 64 columns: 32 rows' first bf16 parts of the
 // probabilities and their second ones) run from shared memory into tensor memory, so that two threads share a key: each has 16 of
 // its scores, exponentials and parts, half a row of the product's operand. (One thread with all 32 was a third slower: four warps
@@ -10,7 +10,7 @@
 //
 // Bound by the chain of a tile (keys arrive, product, scores, parts, product); two blocks per SM run theirs against each other, the
 // next tile's keys are on their way from the first product on and its values from the second. 4 x 8 caches of 30k keys of 128,
-// 32 rows: 118 us (198 with operands in registers, in two passes; floor 75).
+// 32 rows: 115 us (198 with operands in registers, in two passes; floor 75).
 #include "attn_decode.cuh"
 #include "tc_runtime.h"
 

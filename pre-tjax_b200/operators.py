@@ -554,33 +554,38 @@ def _kv_cache(k_pages, v_pages, page_table, lengths):
     return desc, (B, heads, d, page_size, width * page_size)
 
 
-def _view(t, B, heads, T, d, dtype, name):
+def _view(t, shape, dtype, name):
     """(address, strides of batch, head and token) of a view of new tokens."""
-    if t is None:
-        return 0, 0, 0, 0
     if t.dtype is not dtype:
         raise TypeError(f"{name} must have the cache's dtype {dtype}")
-    s0, s1, s2, s3 = t.stride() if t.dim() == 4 else (0, 0, 0, 0)
-    if t.shape != (B, heads, T, d) or (s3 != 1 and d > 1):
-        raise ValueError(f"{name} must be [{B}, {heads}, {T}, {d}] with d_head contiguous")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}")
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 and shape[3] > 1:
+        raise ValueError(f"{name} must have d_head contiguous")
     return t.data_ptr(), s0, s1, s2
 
 
 def _new_tokens(sizes, q, k, v, out, counts, dtype):
     """(the bytes of the new tokens' descriptor, query heads, tokens)."""
     B, Hk, d, _, _ = sizes
-    some = k if q is None else q
-    if some.dim() != 4:
+    shape = (k if q is None else q).shape
+    if len(shape) != 4:
         raise ValueError("new tokens must be [batch, heads, tokens, d_head]")
-    _, H, T, _ = some.shape
-    qp, q0, q1, q2 = _view(q, B, H, T, d, dtype, "q")
-    op, o0, o1, o2 = _view(out, B, H, T, d, dtype, "out")
-    kp, k0, k1, k2 = _view(k, B, Hk, T, d, dtype, "k")
-    vp, v0, v1, v2 = _view(v, B, Hk, T, d, dtype, "v")
+    _, H, T, _ = shape
+    qp = q0 = q1 = q2 = op = o0 = o1 = o2 = kp = k0 = k1 = k2 = vp = v0 = v1 = v2 = 0
+    if q is not None:
+        want = (B, H, T, d)
+        qp, q0, q1, q2 = _view(q, want, dtype, "q")
+        op, o0, o1, o2 = _view(out, want, dtype, "out")
+        if Hk < 1 or H % Hk or H < 1:
+            raise ValueError(f"{H} query heads do not share {Hk} key heads evenly")
+    if k is not None:
+        kp, k0, k1, k2 = _view(k, (B, Hk, T, d), dtype, "k")
+    if v is not None:
+        vp, v0, v1, v2 = _view(v, (B, Hk, T, d), dtype, "v")
     if counts is not None:
         _ints(counts, (B,), "counts")
-    if q is not None and (H % Hk or H < 1):
-        raise ValueError(f"{H} query heads do not share {Hk} key heads evenly")
     return _NEW_TOKENS.pack(qp, kp, vp, op, 0 if counts is None else counts.data_ptr(), H, T, q0, q1, q2, o0, o1, o2, k0, k1, k2,
                             v0, v1, v2), H, T
 
@@ -671,12 +676,13 @@ def kv_evict(k_pages, v_pages, page_table, lengths, weights, budget, recent=0, *
     most = min(budget, capacity)
     weights_out = weights if weights_out is None else weights_out
     ld_out = ld if weights_out is weights else _attended(weights_out, sizes, most, "weights_out")
-    if dst_table is None:
-        dst_table = page_table
-    if dst_table.dim() != 2 or dst_table.shape[1] * page_size < most:
-        raise ValueError(f"dst_table must list pages for {most} keys of each sequence")
-    width = dst_table.shape[1]
-    _ints(dst_table, (B, width), "dst_table")
+    if dst_table is None or dst_table is page_table:
+        dst_table, width = page_table, page_table.shape[1]
+    else:
+        if dst_table.dim() != 2 or dst_table.shape[1] * page_size < most:
+            raise ValueError(f"dst_table must list pages for {most} keys of each sequence")
+        width = dst_table.shape[1]
+        _ints(dst_table, (B, width), "dst_table")
     kept, new_lengths = lengths.new_empty((B, Hk, budget)), lengths.new_empty(B)
     if B == 0:
         return kept, new_lengths
