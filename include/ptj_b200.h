@@ -416,7 +416,8 @@ typedef struct {
   int dtype;                                   /* PTJ_F32 or PTJ_BF16: pools and new tokens */
 } ptj_kv_cache;
 /* The new tokens of a call: token t < counts[b] of sequence b sits at position lengths[b] - counts[b] + t; counts == NULL: all
- * `tokens` of every sequence. Views [batch, heads, tokens, d_head] with element strides batch, head, token. */
+ * `tokens` of every sequence. Views [batch, heads, tokens, d_head] with element strides batch, head, token. What
+ * a call writes (out; the pools) has no stride of 0 over more than one element. */
 typedef struct {
   const void *q, *k, *v;                       /* k, v: NULL where the cache holds the new rows already */
   void* out;

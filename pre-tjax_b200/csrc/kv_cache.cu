@@ -54,6 +54,14 @@ bool view_aligned(const void* p, const int64_t strides[3], const ptj_kv_cache& c
   return strided16(p, strides, sizes, 16 / static_cast<int64_t>(dtype_size(c.dtype)));
 }
 
+bool rows_overlap(const int64_t strides[3], int64_t a, int64_t b, int64_t c) {
+  return (a > 1 && strides[0] == 0) || (b > 1 && strides[1] == 0) || (c > 1 && strides[2] == 0);
+}
+
+bool pools_overlap(const ptj_kv_cache& c) {
+  return rows_overlap(c.k_strides, c.pages, c.kv_heads, c.page_size) || rows_overlap(c.v_strides, c.pages, c.kv_heads, c.page_size);
+}
+
 int check_new_tokens(const ptj_kv_cache& c, const ptj_new_tokens* t, bool need_q, bool need_kv) {
   if (!t || t->tokens < 1 || t->tokens > 4096) return PTJ_ERR_BAD_SHAPE;
   if ((t->k == nullptr) != (t->v == nullptr) || (need_kv && !t->k)) return PTJ_ERR_BAD_SHAPE;
@@ -62,6 +70,8 @@ int check_new_tokens(const ptj_kv_cache& c, const ptj_new_tokens* t, bool need_q
     if (need_q && (t->q_strides[i] < 0 || t->o_strides[i] < 0)) return PTJ_ERR_BAD_SHAPE;
     if (t->k && (t->k_strides[i] < 0 || t->v_strides[i] < 0)) return PTJ_ERR_BAD_SHAPE;
   }
+  // what is written has a place of its own
+  if ((need_q && rows_overlap(t->o_strides, c.batch, t->heads, t->tokens)) || (t->k && pools_overlap(c))) return PTJ_ERR_BAD_SHAPE;
   return PTJ_OK;
 }
 

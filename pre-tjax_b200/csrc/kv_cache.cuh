@@ -68,6 +68,9 @@ int make_paged_rows(const ptj_kv_cache* c, PagedRows& out);
 bool paged_rows_aligned(const ptj_kv_cache& c);
 // The same for a view [batch, heads, tokens, d_head]; strides of dimensions of size 1 do not matter.
 bool view_aligned(const void* p, const int64_t strides[3], const ptj_kv_cache& c, int64_t heads, int64_t tokens);
+// Rows that are written must not share a place: a stride of 0 over more than one element.
+bool rows_overlap(const int64_t strides[3], int64_t a, int64_t b, int64_t c);
+bool pools_overlap(const ptj_kv_cache& c);
 // Checks of the new tokens' descriptor; need_q: q and out are given.
 int check_new_tokens(const ptj_kv_cache& c, const ptj_new_tokens* t, bool need_q, bool need_kv);
 

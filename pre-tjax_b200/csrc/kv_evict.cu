@@ -343,7 +343,7 @@ extern "C" int ptj_kv_evict(const ptj_kv_cache* cache, const int32_t* dst_table,
   const int rc = make_paged_rows(cache, p.rows);
   if (rc != PTJ_OK) return rc;
   if (!dst_table || !weights || !kept || !new_lengths || budget < 1 || budget > (1 << 30) || recent < 0 || recent > budget ||
-      dst_width < 1 || dst_ld < dst_width || new_lengths == cache->lengths)
+      dst_width < 1 || dst_ld < dst_width || new_lengths == cache->lengths || pools_overlap(*cache))
     return PTJ_ERR_BAD_SHAPE;
   const int64_t most = budget < p.rows.capacity ? budget : p.rows.capacity;  // keys that a sequence keeps at most
   if (weights_ld < p.rows.capacity || (weights_out && weights_out_ld < most) || dst_width < ceil_div(most, cache->page_size) ||

@@ -184,6 +184,11 @@ def test_library_refuses_on_its_own():
     assert lib.ptj_attn_decode_workspace_bytes(None, None, 0) == 0
     assert call(good(kv_heads=1), new(heads=4097)) == -1  # query rows of a key head
     assert lib.ptj_kv_append(ctypes.byref(good()), ctypes.byref(new()), None) == -1
+    for o in ((0, 64, 64), (256, 0, 64)):  # sequences, heads that share their output
+        assert call(good(), new(o_strides=o)) == -1
+    shared = good(k_strides=(2048, 0, 64))  # heads that share their keys: read, not written
+    assert call(shared, new(k=16, v=16)) == -1 and lib.ptj_kv_append(ctypes.byref(shared), ctypes.byref(new(k=16, v=16)), None) == -1
+    assert lib.ptj_kv_evict(ctypes.byref(shared), 48, 1, 1, 8, 0, 16, 32, 16, 32, 16, 32, None) == -1
     evict = lambda dst=16, width=1, ld=2, budget=8, recent=0, w=16, wld=32, wo=16, wold=32, kept=16, nl=32: lib.ptj_kv_evict(
         ctypes.byref(good()), dst, width, ld, budget, recent, w, wld, wo, wold, kept, nl, None)
     for kw in (dict(dst=None), dict(width=0), dict(ld=0), dict(budget=0), dict(recent=9), dict(recent=-1), dict(w=None), dict(wld=31),
