@@ -180,7 +180,7 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
 #pragma unroll 1
       for (; cur.s < cur.end; ++cur.s) {
         const int j0 = cur.s * 128, j = j0 + key, j16 = j0 + mine16;
-        const bool edge = j0 + 128 > sg.first + 1, news = p.kn != nullptr && j0 + 128 > sg.first;
+        const bool edge = j0 + 128 > sg.first + 1, news = p.kn != nullptr && j0 + 128 > sg.first;  // edge: not all rows attend all keys
         if (cur.s > s_first) {  // the values' and parts' places are free
           mbar_wait(&bars[1], outputs_done & 1, ctx, 0x3301u);
           ++outputs_done;
@@ -289,10 +289,13 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
           *reinterpret_cast<uint4*>(smem + Core::kP + place(key, piece + 4, 0)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         cp_async_wait<1>();  // the values
+        if (news) {  // (all rows attend a first new key that ends a tile: no edge)
+          __syncthreads();
+          store_new(1, j16, page_now, Core::kV);
+        }
         if (edge) {
           // a value that some rows attend and others do not must be finite to be multiplied by the others' zeros
           __syncthreads();
-          if (news) store_new(1, j16, page_now, Core::kV);
           bool bad = false;
           if (there && r0 == 0)
             for (int c = 0; c < CH; ++c) {

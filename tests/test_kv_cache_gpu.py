@@ -232,6 +232,28 @@ def test_many_rows_append_split_and_replay():
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("wide_table", [0, 1 << 20])
+@pytest.mark.parametrize("T", [1, 2, 3])
+def test_new_rows_at_the_borders_of_tiles(T, wide_table):
+    """New rows that start, end or cross where a step or a tile of 128 keys does, all of them written."""
+    lengths, Hk, H, D, page = [128, 129, 130, 255, 256, 257, 16, 17, 144, 1], 1, 20, 128, 16
+    kp, vp, table, lens = ref.paged(lengths, Hk, D, page, BF16)
+    counts = torch.clamp(lens, max=T)
+    q, k, v = (torch.randn((len(lengths), h, T, D), generator=torch.Generator().manual_seed(30 + h)).to(BF16) for h in (H, Hk, Hk))
+    v = v + 1
+    k_want, v_want = kp.clone(), vp.clone()
+    for b, n in enumerate(lengths):
+        for t in range(int(counts[b])):
+            at = n - int(counts[b]) + t
+            for pool, x in ((k_want, k), (v_want, v)):
+                pool[int(table[b, at // page]), :, at % page] = x[b, :, t]
+    out, k_got, v_got, _ = run(q, kp, vp, table, lens, counts, wide_table=wide_table, k=k.cuda(), v=v.cuda())
+    same = lambda a, b: torch.equal(a.cpu().nan_to_num(7.0), b.nan_to_num(7.0))
+    assert same(k_got, k_want) and same(v_got, v_want)
+    want, _, spread = ref.attend(q, k_want, v_want, table, lens, counts, p=0.1)
+    check_out(out, want, spread, BF16)
+
+
 @pytest.mark.parametrize("aligned", [True, False])
 @pytest.mark.parametrize("D", [64, 120, 128])
 @pytest.mark.parametrize("H,T", [(12, 1), (4, 5), (8, 4), (5, 7)])
