@@ -416,3 +416,38 @@ def test_pages_and_lengths_out_of_range_are_reported():
             assert ops.last_kernel_fault() in (0x3202, 0x3201)
         run(q, kp, vp, table, lens, torch.tensor([2, 1], dtype=torch.int32))
         assert ops.last_kernel_fault() == 0x3202
+
+
+@pytest.mark.parametrize("wide_table", [0, 1 << 20])
+@pytest.mark.parametrize("D", [64, 128])
+def test_missing_pages_and_many_rows(D, wide_table):
+    """20 query rows per key head: pages and lengths out of range are skipped and reported, nothing is written for them."""
+    ops = pkg("operators")
+    kp, vp, table, lens = ref.paged([300, 40], 1, D, 16, BF16)
+    q, k, v = (torch.randn((2, h, 1, D), generator=torch.Generator().manual_seed(40 + i)).to(BF16) for i, h in enumerate((20, 1, 1)))
+    one = torch.ones(2, dtype=torch.int32)
+    want, _, spread = ref.attend(q, kp, vp, table, lens, one, p=0.1)
+    ops.last_kernel_fault()
+    for page in (-1, kp.shape[0], -(1 << 31), (1 << 31) - 1):
+        broken = table.clone()
+        broken[0, 9] = page
+        out, _, _, _ = run(q, kp, vp, broken, lens, wide_table=wide_table)
+        assert ops.last_kernel_fault() == 0x3201
+        check_out(out[1:], want[1:], spread[1:], BF16)
+        keep = torch.cat([torch.arange(144), torch.arange(160, 300)])  # the keys of the missing page count as absent
+        kk, vv = (ref.gather(x, table[0], 300, 0)[keep] for x in (kp, vp))
+        a = torch.softmax(q[0, :, 0].double() @ kk.T / D**0.5, dim=1) @ vv
+        bound = torch.finfo(BF16).eps / 2 * a.abs() + 1.01 * spread[0, :, 0]
+        assert bool(((out[0, :, 0].double().cpu() - 0.9 * a).abs() <= bound).all())
+    broken = table.clone()
+    broken[0, 18] = -1  # the page of the new row
+    _, k_got, v_got, _ = run(q, kp, vp, broken, lens, wide_table=wide_table, k=k.cuda(), v=v.cuda())
+    assert ops.last_kernel_fault() == 0x3201
+    at = int(table[1, 2])
+    kp[at, :, 7], vp[at, :, 7] = k[1, :, 0], v[1, :, 0]
+    same = lambda x, y: torch.equal(x.cpu().nan_to_num(7.0), y.nan_to_num(7.0))
+    assert same(k_got, kp) and same(v_got, vp)
+    run(q, kp, vp, table, torch.tensor([-1, 40], dtype=torch.int32), wide_table=wide_table)
+    assert ops.last_kernel_fault() == 0x3202
+    run(q, kp, vp, table, lens, torch.tensor([2, 1], dtype=torch.int32), wide_table=wide_table)
+    assert ops.last_kernel_fault() == 0x3202
