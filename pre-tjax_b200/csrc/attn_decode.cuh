@@ -403,31 +403,36 @@ attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
   fetcher.set_head(p, sg.h);
   fetcher.clear(p, ring, ring_bytes<Core>());
   Core core;
-  core.init(p, sg);
   const int plain = fetcher.plain_steps(sg);
-  int slot = 0, free_slot = 0, number = 0;
+  for (bool careful = false;; careful = true) {  // a second time where the sums say so
+    core.init(p, sg);
+    int slot = 0, free_slot = 0, number = 0;
 #pragma unroll 1
-  for (int s = s0 - (D - 1) * stride; s < steps; s += stride) {  // (D - 1 rounds ahead: steps to come are fetched only)
-    if (s >= 0) {
-      cp_async_wait<D - 2>();
-      __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
+    for (int s = s0 - (D - 1) * stride; s < steps; s += stride) {  // (D - 1 rounds ahead: steps to come are fetched only)
+      if (s >= 0) {
+        cp_async_wait<D - 2>();
+        __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
+      }
+      const int ahead = s + (D - 1) * stride;
+      if (ahead < steps) {
+        if (number == fetcher.base + 32) fetcher.look_up(p, sg.table, ahead, stride, number);
+        uint8_t* stage = ring + free_slot * stage_bytes<Core>();
+        if (ahead >= plain || !fetcher.plain(p, ahead, number, stage)) fetcher.general(p, sg, ahead, stage);
+        ++number;
+      }
+      cp_async_commit();
+      free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
+      if (s < 0) continue;
+      uint8_t* stage = ring + slot * stage_bytes<Core>();
+      if (s >= plain) fetcher.store_new(p, sg, s, stage);
+      core.step(p, sg, s, stage, careful);
+      slot = slot + 1 == D ? 0 : slot + 1;
     }
-    const int ahead = s + (D - 1) * stride;
-    if (ahead < steps) {
-      if (number == fetcher.base + 32) fetcher.look_up(p, sg.table, ahead, stride, number);
-      uint8_t* stage = ring + free_slot * stage_bytes<Core>();
-      if (ahead >= plain || !fetcher.plain(p, ahead, number, stage)) fetcher.general(p, sg, ahead, stage);
-      ++number;
-    }
-    cp_async_commit();
-    free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
-    if (s < 0) continue;
-    const uint8_t* stage = ring + slot * stage_bytes<Core>();
-    if (s >= plain) fetcher.store_new(p, sg, s, stage);
-    core.step(p, sg, s, stage);
-    slot = slot + 1 == D ? 0 : slot + 1;
+    cp_async_wait<0>();
+    if (careful || !core.spoiled()) break;
+    fetcher.look_up(p, sg.table, s0, stride, 0);
+    __syncwarp();  // all lanes have left the ring
   }
-  cp_async_wait<0>();
   __syncthreads();
   // the warps' sums over the rings, then the block's over the first warp's
   float* os = reinterpret_cast<float*>(smem);
@@ -695,25 +700,38 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
   for (;;) {  // segments
     const int s_first = cur.s, cur_plain = fetcher.plain_steps(cur.sg);
     Core core;
-    core.init(p, cur.sg);
+    for (bool careful = false;; careful = true) {  // a second time where the sums say so, step by step through the ring's free place
+      core.init(p, cur.sg);
 #pragma unroll 1
-    for (;;) {
-      if (lead == 0) {
-        cp_async_wait<D - 2>();
-        __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
+      for (;;) {
+        uint8_t* stage = ring + free_slot * stage_bytes<Core>();
+        if (careful) {
+          __syncwarp();
+          fetcher.general(p, cur.sg, cur.s, stage);
+          cp_async_commit();
+          cp_async_wait<0>();
+          __syncwarp();
+        } else {
+          if (lead == 0) {
+            cp_async_wait<D - 2>();
+            __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
+          }
+          fetch_ahead(stage);
+          cp_async_commit();
+          free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
+          if (lead > 0) {
+            --lead;
+            continue;
+          }
+          stage = ring + slot * stage_bytes<Core>();
+          if (cur.s >= cur_plain) fetcher.store_new(p, cur.sg, cur.s, stage);
+          slot = slot + 1 == D ? 0 : slot + 1;
+        }
+        core.step(p, cur.sg, cur.s, stage, careful);
+        if (++cur.s == cur.end) break;
       }
-      fetch_ahead(ring + free_slot * stage_bytes<Core>());
-      cp_async_commit();
-      free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
-      if (lead > 0) {
-        --lead;
-        continue;
-      }
-      const uint8_t* stage = ring + slot * stage_bytes<Core>();
-      if (cur.s >= cur_plain) fetcher.store_new(p, cur.sg, cur.s, stage);
-      core.step(p, cur.sg, cur.s, stage);
-      slot = slot + 1 == D ? 0 : slot + 1;
-      if (++cur.s == cur.end) break;
+      if (careful || !core.spoiled()) break;
+      cur.s = s_first;
     }
     const bool whole = s_first == 0 && cur.s == cur.steps;
     const int64_t piece = stretch * 2 + (first_piece ? 0 : 1);

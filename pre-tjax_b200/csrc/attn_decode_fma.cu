@@ -64,7 +64,7 @@ struct CoreFma {
     }
   }
 
-  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) {
+  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage, bool) {
     const int j0 = sub * KS;
     const uint32_t present = present_keys<KS, kRowBytes>(stage);
     const bool edge = j0 + KS > sg.first + 1 || present != (1u << KS) - 1u;  // some rows do not attend all of its keys
@@ -156,6 +156,8 @@ struct CoreFma {
       }
     }
   }
+
+  __device__ __forceinline__ bool spoiled() const { return false; }  // probabilities are multiplied whole
 
   // f(row, element, four sums, reference exponent, sum of the row, true for one call per row)
   template <typename F>

@@ -77,8 +77,9 @@ struct CoreTc {
   __device__ __forceinline__ uint4 key(const uint8_t* stage, int i, int u) const {
     return *reinterpret_cast<const uint4*>(stage + ((key_at ^ ((u & 1) << 6)) + 8 * i * kRowBytes + (u >> 1) * 128));
   }
+  __device__ __forceinline__ uint32_t value_place(int i, int w) const { return value_at[i & 1] + 8 * (i >> 1) * kRowBytes + w * 128; }
   __device__ __forceinline__ uint4 value(const uint8_t* stage, int i, int w) const {
-    return *reinterpret_cast<const uint4*>(stage + (value_at[i & 1] + 8 * (i >> 1) * kRowBytes + w * 128));
+    return *reinterpret_cast<const uint4*>(stage + value_place(i, w));
   }
 
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -96,15 +97,32 @@ struct CoreTc {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  static __device__ __forceinline__ void values(float (&acc)[4], const uint4 (&v)[4], int j, const uint32_t (&ph)[2], const uint32_t (&pl)[2]) {
+  static __device__ __forceinline__ void operands(const uint4 (&v)[4], int j, uint32_t (&a)[4]) {
     const uint32_t v0 = word(v[0], j), v1 = word(v[1], j), v2 = word(v[2], j), v3 = word(v[3], j);
-    const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
-    const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
-    mma(acc, a0, a1, a2, a3, ph[0], ph[1]);
-    if constexpr (!HALF) mma(acc, a0, a1, a2, a3, pl[0], pl[1]);
+    a[0] = __byte_perm(v0, v1, 0x5410), a[1] = __byte_perm(v0, v1, 0x7632);
+    a[2] = __byte_perm(v2, v3, 0x5410), a[3] = __byte_perm(v2, v3, 0x7632);
+  }
+  static __device__ __forceinline__ void values(float (&acc)[4], const uint4 (&v)[4], int j, const uint32_t (&ph)[2], const uint32_t (&pl)[2]) {
+    uint32_t a[4];
+    operands(v, j, a);
+    mma(acc, a[0], a[1], a[2], a[3], ph[0], ph[1]);
+    if constexpr (!HALF) mma(acc, a[0], a[1], a[2], a[3], pl[0], pl[1]);
   }
 
-  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) {
+  // An infinite value times the second part of its probability (zero, or of either sign) makes NaN of an infinite sum. That is looked
+  // for once, in the sums at the end, and costs the steps nothing; where it was, they run again with `careful`.
+  __device__ __forceinline__ bool spoiled() const {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[i][j][e]) < INFINITY) && limit[i][e & 1] >= 0;
+    return __any_sync(0xffffffffu, bad);
+  }
+
+  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage, bool careful) {
     const int j0 = sub * KS;
     const bool edge = j0 + KS > sg.first + 1;  // some rows do not attend all of its keys
     float s[NR][4];
@@ -193,10 +211,7 @@ struct CoreTc {
         }
       }
     // a value that some rows of the step attend and others do not must be finite to be multiplied by the others' zeros
-    if (edge && not_finite(stage)) {
-      values_by_token(p, sg, j0, stage, ph, pl);
-      return;
-    }
+    if ((edge || careful) && not_finite(stage)) infinite_values(p, sg, j0, stage, ph, edge);
 #pragma unroll
     for (int w = 0; w < VW; ++w) {
       const uint4 v[4] = {value(stage, 0, w), value(stage, 1, w), value(stage, 2, w), value(stage, 3, w)};
@@ -222,31 +237,44 @@ struct CoreTc {
       }
     return __any_sync(0xffffffffu, bad);
   }
-  // The products of a step with values that are not finite: once per new token, with what it does not attend cleared, and added to
-  // its rows only.
-  __device__ __forceinline__ void values_by_token(const DecodeAttn& p, const Segment& sg, int j0, const uint8_t* stage,
-                                                  const uint32_t (&ph)[NR][2], const uint32_t (&pl)[NR][2]) {
+  static __device__ __forceinline__ uint32_t finite(uint32_t x) {  // zero in place of halves that are not
+    return ((x & 0x7f80u) == 0x7f80u ? 0u : x & 0xffffu) | ((x & 0x7f800000u) == 0x7f800000u ? 0u : x & 0xffff0000u);
+  }
+  // Takes the values of a step that are not finite out of it and adds their products, by the first parts of the probabilities only.
+  // At an edge once per new token, with what it does not attend cleared, and to its rows only.
+  __device__ __forceinline__ void infinite_values(const DecodeAttn& p, const Segment& sg, int j0, uint8_t* stage, const uint32_t (&ph)[NR][2],
+                                                  bool edge) {
+    const int tokens = edge ? sg.count : 1;
 #pragma unroll 1
-    for (int tok = 0; tok < sg.count; ++tok)
+    for (int tok = 0; tok < tokens; ++tok)
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         uint4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[i] = j0 + value_of(i) <= sg.first + tok ? value(stage, i, w) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 4; ++i) {
+          v[i] = !edge || j0 + value_of(i) <= sg.first + tok ? value(stage, i, w) : make_uint4(0u, 0u, 0u, 0u);
+          v[i] = make_uint4(v[i].x ^ finite(v[i].x), v[i].y ^ finite(v[i].y), v[i].z ^ finite(v[i].z), v[i].w ^ finite(v[i].w));
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int i = 0; i < NR; ++i) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            values(acc, v, j, ph[i], pl[i]);
+            uint32_t a[4];
+            operands(v, j, a);
+            mma(acc, a[0], a[1], a[2], a[3], ph[i][0], ph[i][1]);
+            if (HALF && c >= 2) continue;  // (columns of second parts)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (limit[i][e] == sg.first + tok) {
-                o[i][w * 4 + j][e] += acc[e];
-                o[i][w * 4 + j][e + 2] += acc[e + 2];
-              }
+            for (int e = 0; e < 4; ++e)
+              if (!edge || limit[i][e & 1] == sg.first + tok) o[i][w * 4 + j][e] += acc[e];
           }
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {  // (a lane's own pieces: nobody else reads them)
+        const uint4 v = value(stage, i, w);
+        *reinterpret_cast<uint4*>(stage + value_place(i, w)) = make_uint4(finite(v.x), finite(v.y), finite(v.z), finite(v.w));
       }
   }
 

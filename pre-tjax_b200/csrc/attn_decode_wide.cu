@@ -108,7 +108,7 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
   if (range0 < all) {
     Cursor<Core> cur;
     cur.set(p, seq_s, start_s, range0, min(st.q1, all - range0));
-    bool first_piece = true;
+    bool first_piece = true, careful = false;  // careful: an infinite value spoiled the segment's sums, it runs again
     for (;;) {  // segments
       const Segment& sg = cur.sg;
       // the rows' queries
@@ -293,8 +293,9 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
           __syncthreads();
           store_new(1, j16, page_now, Core::kV);
         }
-        if (edge) {
-          // a value that some rows attend and others do not must be finite to be multiplied by the others' zeros
+        if (edge || careful) {
+          // a value that some rows attend and others do not must be finite to be multiplied by the others' zeros; one that is not is
+          // multiplied by the first part of its probability only (the second is zero, or of either sign)
           __syncthreads();
           bool bad = false;
           if (there && r0 == 0)
@@ -354,7 +355,19 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
       tmem_ld_32x16(tmem + lanes + kColO + 32 + r0, lo);
       tmem_ld_wait();
       tc_fence_before_sync();
-      __syncthreads();
+      bool spoiled = false;
+      if (!careful && key < p.D) {
+#pragma unroll
+        for (int i = 0; i < RH; ++i) {
+          const float o = __uint_as_float(hi[i]) + __uint_as_float(lo[i]);
+          spoiled |= !(fabsf(o) < INFINITY) && limit_s[r0 + i] >= 0;
+        }
+      }
+      careful = __syncthreads_or(spoiled);
+      if (careful) {
+        cur.s = s_first;
+        continue;
+      }
       const bool whole = s_first == 0 && cur.s == cur.steps;
       const int64_t piece = worker * 2 + (first_piece ? 0 : 1);
       if (key < p.D) {
