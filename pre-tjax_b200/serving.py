@@ -52,14 +52,15 @@ class PagedCache:
             raise RuntimeError("eviction goes by attention weights: make the cache with track_weights=True")
         for l in range(self.cfg.layers):
             _, lengths = ops.kv_evict(self.k[l], self.v[l], self.page_table, self.lengths, self.weights[l], budget, recent)
-        self.lengths = lengths
+        self.lengths.copy_(lengths)
 
 
 def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tensor = None, p: float = None) -> torch.Tensor:
     """Appends the tokens ids [B, T] to the sequences of a cache and returns their logits [B, T, vocab] (train=False). counts int32
     [B]: the first counts[b] of a sequence's T ids are tokens (default T); what comes back behind them means nothing. params: the
     reference's pytree (model_torch_func.py:36-43) or (GPT2Config, gpt2.Weights). The caller sees to it that no sequence passes
-    the cache's capacity or the model's positions: keys beyond are reported by operators.last_kernel_fault."""
+    the cache's capacity or the model's positions: keys beyond are reported by operators.last_kernel_fault. A step with laid-out weights
+    may be recorded in a CUDA graph: every replay advances the cache, which keeps its tensors, by one more step of the ids then in place."""
     cfg, w = _weights(params, cache.k.dtype, p)
     if (cfg.layers, cfg.heads, cfg.d_head) != (cache.cfg.layers, cache.cfg.heads, cache.cfg.d_head):
         raise ValueError("the cache was made for another model")
@@ -69,8 +70,8 @@ def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tens
     D, H, dh, rows, p = cfg.dim, cfg.heads, cfg.d_head, B * T, cfg.dropout
     added = torch.full_like(cache.lengths, T) if counts is None else counts
     at = (cache.positions[:, None] + torch.arange(T, device=ids.device)).clamp_(max=cfg.seq - 1)
-    cache.lengths = cache.lengths + added
-    cache.positions = cache.positions + added
+    cache.lengths += added  # (in place, as all that changes the cache: a recorded step goes on where the last replay ended)
+    cache.positions += added
     x = ops.embed_fwd(ids.reshape(1, rows), w["w_emb"], w["w_pos"][at.reshape(-1)], False, 0, out_dtype=cache.k.dtype, p=p).view(rows, D)
     for l in range(cfg.layers):
         g = lambda n: w[f"l{l}.{n}"]
