@@ -643,19 +643,24 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, cou
         if weights is not None and _attended(weights, sizes, sizes[4], "weights") != ld:
             raise ValueError("weights and weights_out must share one shape")
     lib = _lib.lib()
+    key = None
     if workspace is None:
         key = (sizes, H, T, ld > 0, q.dtype)
         need = _DECODE_BYTES.get(key)
         if need is None:
-            if len(_DECODE_BYTES) > 4096:
-                _DECODE_BYTES.clear()
-            need = _DECODE_BYTES[key] = lib.ptj_attn_decode_workspace_bytes(cache, new, int(ld > 0))
+            need = lib.ptj_attn_decode_workspace_bytes(cache, new, int(ld > 0))
+        else:
+            key = None
         if need:
             workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
     rc = lib.ptj_attn_decode(cache, new, DROPOUT_RATE if p is None else p, _ptr(weights), _ptr(weights_out), ld,
                              _ptr(workspace), 0 if workspace is None else workspace.nbytes, _stream())
     if rc != 0:
         _lib.check(rc, "ptj_attn_decode")
+    if key is not None:  # (only now: for arguments it refuses the library answers 0)
+        if len(_DECODE_BYTES) > 4096:
+            _DECODE_BYTES.clear()
+        _DECODE_BYTES[key] = need
     return out
 
 
