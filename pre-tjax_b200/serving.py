@@ -158,19 +158,17 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
         guess = torch.cat(guesses, dim=1)
         probs = probabilities(decode_step(target, torch.cat([last, guess], dim=1), cache), temperature)
         tokens, accepted = ops.verify_drafts(probs, guess, u[:, drafts:2 * drafts + 1].contiguous(), draft_probs=torch.cat(dists, dim=1))
-        back = drafts - accepted
-        cache.rewind(back)
-        ahead.rewind(back)
         # accepted tokens and the one behind them to their places; zeros behind those are overwritten by the next round
-        place = (done[:, None] + columns).clamp_(max=out.shape[1] - 1)
+        place = done[:, None] + columns
         out.scatter_(1, place, torch.where((done < new_tokens)[:, None], tokens, out.gather(1, place)))
         last = tokens.gather(1, accepted[:, None].long())
-        # a sequence that has its tokens stays where it is: it is decoded along, one round over and over
-        more = torch.where(done < new_tokens, accepted + 1, 0)
-        stay = torch.where(done < new_tokens, 0, accepted + 1).to(torch.int32)
-        cache.rewind(stay)
-        ahead.rewind(stay)
-        done = done + more
+        # A sequence that has its tokens stays where it is and is decoded along, one round over and over. Its last round's tokens beyond
+        # those are taken back with the drafts that did not stand: the caches have room for one round behind the last token.
+        more = torch.minimum(accepted + 1, new_tokens - done)
+        back = drafts + 1 - more
+        cache.rewind(back)
+        ahead.rewind(back)
+        done += more
         rounds += 1
         most += drafts + 1
         least = int(done.min())

@@ -18,3 +18,47 @@ def test_a_refused_call_leaves_later_ones_alone(ops, refused):  # noqa: F811
     for _ in range(2):
         with pytest.raises(RuntimeError, match="sm_100"):
             ops.attn_decode(rows(4), **cache(), weights=w)
+
+
+class Rounds:
+    """speculate on the CPU with a model that knows no tokens: every step is checked against its cache's room, drafts stand as told."""
+
+    def __init__(self, monkeypatch, stands, seq=64):
+        sv, gpt2 = pkg("serving"), pkg("gpt2")
+        self.sv, self.stands, self.steps = sv, torch.tensor(stands, dtype=I32), []
+        cfg = gpt2.GPT2Config(vocab=10, dim=8, layers=1, heads=2, ffn=16, seq=seq)
+        monkeypatch.setattr(sv, "_weights", lambda params, dtype, p=None: (cfg, params))
+        monkeypatch.setattr(sv, "decode_step", self.decode_step)
+        monkeypatch.setattr(sv, "probabilities", lambda logits, temperature=1.0: logits)
+        monkeypatch.setattr(sv.ops, "verify_drafts", self.verify)
+
+    def decode_step(self, model, ids, cache, counts=None):
+        added = torch.full_like(cache.lengths, ids.shape[1]) if counts is None else counts
+        assert bool(((added >= 0) & (added <= ids.shape[1])).all())
+        cache.lengths += added
+        cache.positions += added
+        assert int(cache.lengths.max()) <= cache.capacity and int(cache.positions.max()) <= cache.cfg.seq
+        self.steps.append((cache, ids, counts))
+        return torch.zeros(*ids.shape, 10)
+
+    def verify(self, target, tokens, uniforms, draft_probs=None):
+        B, K = tokens.shape
+        out = torch.arange(K + 1, dtype=I32).repeat(B, 1)
+        n = torch.minimum(self.stands, torch.full((B,), K, dtype=I32))
+        return torch.where(out <= n[:, None], out, 0), n
+
+    def __call__(self, P, new, drafts, rounds, **kw):
+        B = len(self.stands)
+        return self.sv.speculate([[torch.zeros(1)]], [[torch.zeros(1)]], torch.ones(B, P, dtype=I32), new,
+                                 torch.zeros(rounds, B, 2 * drafts + 1), drafts=drafts, **kw)
+
+
+@pytest.mark.parametrize("drafts", [1, 2, 3, 5])
+@pytest.mark.parametrize("new", [1, 6, 13])
+def test_sequences_that_end_early_need_no_more_room(monkeypatch, drafts, new):
+    """All drafts of one sequence stand, none of another's: no step goes beyond the caches, and the tokens are the rounds' own."""
+    run = Rounds(monkeypatch, [drafts, 0, 1])
+    tokens, rounds = run(8, new, drafts, new, page_size=1)
+    assert rounds == new
+    for b, n in enumerate((drafts, 0, min(1, drafts))):
+        assert tokens[b].tolist() == [i % (n + 1) for i in range(new)]
