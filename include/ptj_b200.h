@@ -431,7 +431,7 @@ int ptj_kv_append(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, void*
 /* Attention of the new tokens over the cache, evaluation semantics (the output is multiplied by 1 - p):
  *   out = (1 - p) softmax(q K^T / sqrt(d_head)) V over keys 0 .. position of the token.
  * With tokens->k and ->v the new rows are written to their pages as by ptj_kv_append and attended to. A token behind counts[b]
- * or below position 0 attends nothing: a zero row. out overlaps no input. Rows read only the keys they attend: what lies in
+ * or below position 0, or none of whose keys' pages exists, attends nothing: a zero row. out overlaps no input. Rows read only the keys they attend: what lies in
  * other slots, an infinity or a NaN included, reaches no output. Softmax statistics and sums are float32.
  * weights_out (optional, float[batch, kv_heads, weights_ld], weights_ld >= table_width * page_size): the attention that each
  * key received, summed over the query heads of its key head and the new tokens, plus weights (same layout; NULL = 0; may be

@@ -381,7 +381,7 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
           if (extra) o += reinterpret_cast<const float*>(smem + Core::kX)[r * DP + key];
           if (whole) {
             char* to = p.out + sg.b * p.os[0] + (sg.h * p.G + row / p.T) * p.os[1] + (row % p.T) * p.os[2];
-            reinterpret_cast<__nv_bfloat16*>(to)[key] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * (p.keep / l) : 0.f);
+            reinterpret_cast<__nv_bfloat16*>(to)[key] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * sg.over(p, row, p.keep, l) : 0.f);
           } else {
             p.part[(piece * p.prows + r) * Core::kDim + key] = o;
           }
