@@ -68,17 +68,16 @@ def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tens
     if B != cache.batch:
         raise ValueError(f"{B} sequences for a cache of {cache.batch}")
     D, H, dh, rows, p = cfg.dim, cfg.heads, cfg.d_head, B * T, cfg.dropout
-    added = torch.full_like(cache.lengths, T) if counts is None else counts
+    added = T if counts is None else counts
+    lengths = cache.lengths + added
     at = (cache.positions[:, None] + torch.arange(T, device=ids.device)).clamp_(max=cfg.seq - 1)
-    cache.lengths += added  # (in place, as all that changes the cache: a recorded step goes on where the last replay ended)
-    cache.positions += added
     x = ops.embed_fwd(ids.reshape(1, rows), w["w_emb"], w["w_pos"][at.reshape(-1)], False, 0, out_dtype=cache.k.dtype, p=p).view(rows, D)
     for l in range(cfg.layers):
         g = lambda n: w[f"l{l}.{n}"]
         qkv = ops.gemm(ops.t_layernorm_fwd_t((g("g1"), g("b1")), x), g("w_qkv").view(3 * D, D))  # columns (head, q/k/v, d_head)
         q, k, v = qkv.view(B, T, H, 3, dh).permute(3, 0, 2, 1, 4).unbind(0)
         attn = x.new_empty((rows, D))
-        ops.attn_decode(q, cache.k[l], cache.v[l], cache.page_table, cache.lengths, k=k, v=v, counts=counts,
+        ops.attn_decode(q, cache.k[l], cache.v[l], cache.page_table, lengths, k=k, v=v, counts=counts,
                         weights=None if cache.weights is None else cache.weights[l], out=attn.view(B, T, H, dh).transpose(1, 2), p=p)
         x = ops.gemm(attn, g("w_o"), epilogue=_lib.EPI_DROPOUT_RESID, aux=x, dropout_args=(p, False, 0, 0))
         h = ops.gemm(ops.t_layernorm_fwd_t((g("g2"), g("b2")), x), g("w1"), bias=g("b1f"), epilogue=_lib.EPI_GELU)
@@ -86,6 +85,10 @@ def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tens
     x = ops.t_layernorm_fwd_t((w["g_f"], w["b_f"]), x)
     logits = x.new_empty((rows, (cfg.vocab + 127) // 128 * 128))
     ops.gemm(x, w["w_emb"], bias=w["b_head"], out=logits, N=cfg.vocab, ldc=logits.stride(0))
+    # Behind all calls: one that raises leaves no tokens counted that the cache does not hold. In place: a recorded step goes on where
+    # the last replay ended.
+    cache.lengths.copy_(lengths)
+    cache.positions += added
     return logits.view(B, T, -1)[:, :, :cfg.vocab]
 
 

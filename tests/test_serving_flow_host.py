@@ -62,3 +62,22 @@ def test_sequences_that_end_early_need_no_more_room(monkeypatch, drafts, new):
     assert rounds == new
     for b, n in enumerate((drafts, 0, min(1, drafts))):
         assert tokens[b].tolist() == [i % (n + 1) for i in range(new)]
+
+
+def small_cache(**kw):
+    sv, gpt2 = pkg("serving"), pkg("gpt2")
+    cfg = gpt2.GPT2Config(vocab=10, dim=8, layers=3, heads=2, ffn=16, seq=32)
+    c = sv.PagedCache(cfg, 2, capacity=20, page_size=4, device="cpu", **kw)
+    c.lengths += 6
+    c.positions += 7
+    return sv, cfg, c
+
+
+@pytest.mark.parametrize("counts", [None, torch.tensor([1, 0], dtype=I32), torch.tensor([1, 0])])
+def test_a_step_that_fails_leaves_the_cache_as_it_was(counts):
+    """(It fails here for want of a GPU.) What the cache counts is what it holds."""
+    sv, cfg, c = small_cache()
+    w = dict(w_emb=torch.zeros(10, 8), w_pos=torch.zeros(32, 8))
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        sv.decode_step((cfg, w), torch.zeros(2, 3, dtype=I32), c, counts)
+    assert c.lengths.tolist() == [6, 6] and c.positions.tolist() == [7, 7]
