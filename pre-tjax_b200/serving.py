@@ -36,6 +36,7 @@ class PagedCache:
         self.page_table = torch.arange(batch * width, device=device, dtype=torch.int32).view(batch, width)
         self.lengths = torch.zeros(batch, device=device, dtype=torch.int32)
         self.positions = torch.zeros(batch, device=device, dtype=torch.int64)
+        self._cut = 0  # layers that an unfinished eviction has cut
         self.weights = None
         if track_weights:
             self.weights = torch.zeros((cfg.layers, batch, cfg.heads, width * page_size), device=device, dtype=torch.float32)
@@ -50,9 +51,17 @@ class PagedCache:
         """Cuts every sequence down to `budget` keys per head: the last `recent` and the heaviest of the others."""
         if self.weights is None:
             raise RuntimeError("eviction goes by attention weights: make the cache with track_weights=True")
+        self.check_whole()
         for l in range(self.cfg.layers):
             _, lengths = ops.kv_evict(self.k[l], self.v[l], self.page_table, self.lengths, self.weights[l], budget, recent)
+            self._cut = l + 1
         self.lengths.copy_(lengths)
+        self._cut = 0
+
+    def check_whole(self) -> None:
+        """Raises where an eviction failed between two layers: no lengths fit all of them any more."""
+        if self._cut:
+            raise RuntimeError("an eviction from this cache failed behind some of its layers: its sequences have to be decoded anew")
 
 
 def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tensor = None, p: float = None) -> torch.Tensor:
@@ -64,6 +73,7 @@ def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tens
     cfg, w = _weights(params, cache.k.dtype, p)
     if (cfg.layers, cfg.heads, cfg.d_head) != (cache.cfg.layers, cache.cfg.heads, cache.cfg.d_head):
         raise ValueError("the cache was made for another model")
+    cache.check_whole()
     B, T = ids.shape
     if B != cache.batch:
         raise ValueError(f"{B} sequences for a cache of {cache.batch}")

@@ -81,3 +81,27 @@ def test_a_step_that_fails_leaves_the_cache_as_it_was(counts):
     with pytest.raises(RuntimeError, match="no CPU implementation"):
         sv.decode_step((cfg, w), torch.zeros(2, 3, dtype=I32), c, counts)
     assert c.lengths.tolist() == [6, 6] and c.positions.tolist() == [7, 7]
+
+
+def test_an_eviction_that_fails_half_way_is_not_decoded_on(monkeypatch):
+    """The first layer is cut, the second one's call raises: lengths stand for neither, so the cache refuses to go on. A call that is
+    refused before any layer is cut leaves it usable."""
+    sv, cfg, c = small_cache(track_weights=True)
+    done = []
+
+    def evict(k, v, table, lengths, weights, budget, recent):
+        if budget < 1:
+            raise ValueError("budget")
+        if len(done) == 1:
+            raise RuntimeError("out of memory")
+        done.append(1)
+        return None, torch.clamp(lengths, max=budget)
+
+    monkeypatch.setattr(sv.ops, "kv_evict", evict)
+    with pytest.raises(ValueError, match="budget"):
+        c.evict(0, 0)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        c.evict(4, 2)
+    for call in (lambda: c.evict(4, 2), lambda: sv.decode_step((cfg, None), torch.zeros(2, 1, dtype=I32), c)):
+        with pytest.raises(RuntimeError, match="some of its layers"):
+            call()
