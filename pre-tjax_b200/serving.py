@@ -80,7 +80,7 @@ def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tens
     D, H, dh, rows, p = cfg.dim, cfg.heads, cfg.d_head, B * T, cfg.dropout
     added = T if counts is None else counts
     lengths = cache.lengths + added
-    at = (cache.positions[:, None] + torch.arange(T, device=ids.device)).clamp_(max=cfg.seq - 1)
+    at = (cache.positions[:, None] + torch.arange(T, device=ids.device)).clamp_(0, cfg.seq - 1)
     x = ops.embed_fwd(ids.reshape(1, rows), w["w_emb"], w["w_pos"][at.reshape(-1)], False, 0, out_dtype=cache.k.dtype, p=p).view(rows, D)
     for l in range(cfg.layers):
         g = lambda n: w[f"l{l}.{n}"]

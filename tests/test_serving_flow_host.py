@@ -105,3 +105,13 @@ def test_an_eviction_that_fails_half_way_is_not_decoded_on(monkeypatch):
     for call in (lambda: c.evict(4, 2), lambda: sv.decode_step((cfg, None), torch.zeros(2, 1, dtype=I32), c)):
         with pytest.raises(RuntimeError, match="some of its layers"):
             call()
+
+
+@pytest.mark.parametrize("back", [9, 40, 1 << 20])
+def test_positions_before_the_first_are_no_index(back):
+    """More tokens taken back than were seen: the position table is read inside its rows (beyond them an index ends a GPU's context)."""
+    sv, cfg, c = small_cache()
+    c.rewind(torch.full((2,), back, dtype=I32))
+    w = dict(w_emb=torch.zeros(10, 8), w_pos=torch.zeros(32, 8))
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        sv.decode_step((cfg, w), torch.zeros(2, 3, dtype=I32), c)
