@@ -119,7 +119,7 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
               temperature: float = 1.0, prompt_lens: torch.Tensor = None, page_size: int = 16, budget: int = None, recent: int = 0):
     """Samples new_tokens tokens behind each prompt: (tokens int32 [B, new_tokens], rounds). params, draft_params: as for decode_step.
 
-    prompt int [B, P], padded on the right; prompt_lens int32 [B] (default P). Every round the draft model (same vocabulary and
+    prompt int [B, P], padded on the right; prompt_lens int32 [B], 1 to P (default P; read by the host). Every round the draft model (same vocabulary and
     positions) proposes `drafts` tokens and the target accepts a part of them and adds one of its own, so that tokens are
     distributed as if the target had drawn each. uniforms float32 [rounds, B, 2 * drafts + 2] in [0, 1): of round r, the first
     `drafts` draw the draft's tokens, the other drafts + 1 (and one unused) go to verify_drafts; the last round's are used again
@@ -132,6 +132,11 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
         raise ValueError("target and draft model must share a vocabulary")
     if drafts < 1 or uniforms.dim() != 3 or uniforms.shape[1] != B or uniforms.shape[2] < 2 * drafts + 1:
         raise ValueError(f"uniforms must be [rounds, {B}, >= {2 * drafts + 1}] and drafts >= 1")
+    if P < 1:
+        raise ValueError("a prompt has at least one token")
+    if prompt_lens is not None and (prompt_lens.dtype != torch.int32 or prompt_lens.shape != (B,) or
+                                    bool(((prompt_lens < 1) | (prompt_lens > P)).any())):
+        raise ValueError(f"prompt_lens must be an int32 tensor of shape [{B}] with values from 1 to {P}")
     longest = P + new_tokens + drafts + 1
     if longest > min(target[0].seq, draft[0].seq):
         raise ValueError(f"{longest} positions (prompt, new tokens and drafts ahead) exceed the models'")
@@ -147,8 +152,8 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
     ids = prompt.to(torch.int32)
     if P > 1:
         for model, c in ((target, cache), (draft, ahead)):
-            decode_step(model, ids[:, :P - 1], c, (lens - 1).clamp_(min=0))
-    last = ids[rows, (lens - 1).clamp(min=0).long()][:, None]
+            decode_step(model, ids[:, :P - 1], c, lens - 1)
+    last = ids[rows, lens.long() - 1][:, None]
     out = torch.zeros((B, new_tokens + drafts + 1), device=device, dtype=torch.int32)
     done = torch.zeros(B, device=device, dtype=torch.int64)
     least, most, rounds = 0, P, 0  # of the tokens so far; of a sequence's keys

@@ -115,3 +115,16 @@ def test_positions_before_the_first_are_no_index(back):
     w = dict(w_emb=torch.zeros(10, 8), w_pos=torch.zeros(32, 8))
     with pytest.raises(RuntimeError, match="no CPU implementation"):
         sv.decode_step((cfg, w), torch.zeros(2, 3, dtype=I32), c)
+
+
+@pytest.mark.parametrize("change", [dict(prompt=torch.ones(2, 0, dtype=I32)), dict(prompt_lens=torch.tensor([6, 2], dtype=I32)),
+                                    dict(prompt_lens=torch.tensor([5, 0], dtype=I32)), dict(prompt_lens=torch.tensor([-1, 5], dtype=I32)),
+                                    dict(prompt_lens=torch.tensor([5], dtype=I32)), dict(prompt_lens=torch.tensor([5, 5]))])
+def test_prompts_have_a_token_and_lengths_within_them(monkeypatch, change):
+    """The last token of each prompt is picked by its length: an index outside the prompt would end a GPU's context."""
+    run = Rounds(monkeypatch, [1, 0])
+    args = dict(prompt=torch.ones(2, 5, dtype=I32), new_tokens=3, uniforms=torch.zeros(9, 2, 5), drafts=2)
+    run.sv.speculate([[torch.zeros(1)]], [[torch.zeros(1)]], **args, prompt_lens=torch.tensor([1, 5], dtype=I32))
+    args.update(change)
+    with pytest.raises(ValueError, match="prompt"):
+        run.sv.speculate([[torch.zeros(1)]], [[torch.zeros(1)]], **args)
