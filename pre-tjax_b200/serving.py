@@ -13,6 +13,8 @@ A cache may be bounded: ``PagedCache.evict`` keeps the last keys and those that 
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib, operators as ops
@@ -109,8 +111,14 @@ def _weights(params, dtype, p=None):
     return cfg, Weights.from_pytree(params, cfg, dtype)
 
 
+def _check_temperature(temperature):
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"temperature must be positive and finite, not {temperature} (for the likeliest token take the logits' maximum)")
+
+
 def probabilities(logits: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
-    """softmax(logits / temperature) in float32 (bf16 log-probabilities would be off by percents)."""
+    """softmax(logits / temperature) in float32 (bf16 log-probabilities would be off by percents); temperature > 0."""
+    _check_temperature(temperature)
     x = logits.float()
     return ops.t_log_softmax_fwd_t(x if temperature == 1.0 else x / temperature).exp_()
 
@@ -142,6 +150,7 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
         raise ValueError(f"{longest} positions (prompt, new tokens and drafts ahead) exceed the models'")
     if budget is not None and not (0 <= recent <= budget and budget >= 1):
         raise ValueError("speculate needs 0 <= recent <= budget and budget >= 1")
+    _check_temperature(temperature)
     room = longest if budget is None else min(longest, max(P, 2 * budget) + drafts + 1)
     device = prompt.device
     cache = PagedCache(target[0], B, room, page_size, dtype, device, track_weights=budget is not None)

@@ -128,3 +128,15 @@ def test_prompts_have_a_token_and_lengths_within_them(monkeypatch, change):
     args.update(change)
     with pytest.raises(ValueError, match="prompt"):
         run.sv.speculate([[torch.zeros(1)]], [[torch.zeros(1)]], **args)
+
+
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan"), float("inf")])
+def test_temperatures_that_leave_no_probabilities_are_refused(monkeypatch, temperature):
+    """(Divided by 0, a row of logits has no softmax, and token 0 came of it.)"""
+    real = pkg("serving").probabilities
+    run = Rounds(monkeypatch, [1, 0])
+    with pytest.raises(ValueError, match="temperature"):
+        run(5, 3, 2, 9, temperature=temperature)
+    assert not run.steps
+    with pytest.raises(ValueError, match="temperature"):
+        real(torch.zeros(1, 4), temperature)
