@@ -13,8 +13,6 @@ A cache may be bounded: ``PagedCache.evict`` keeps the last keys and those that 
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib, operators as ops
@@ -112,8 +110,8 @@ def _weights(params, dtype, p=None):
 
 
 def _check_temperature(temperature):
-    if not 0.0 < temperature < math.inf:
-        raise ValueError(f"temperature must be positive and finite, not {temperature} (for the likeliest token take the logits' maximum)")
+    if not temperature > 0.0:
+        raise ValueError(f"temperature must be positive, not {temperature} (for the likeliest token take the logits' maximum)")
 
 
 def probabilities(logits: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
