@@ -125,12 +125,13 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
               temperature: float = 1.0, prompt_lens: torch.Tensor = None, page_size: int = 16, budget: int = None, recent: int = 0):
     """Samples new_tokens tokens behind each prompt: (tokens int32 [B, new_tokens], rounds). params, draft_params: as for decode_step.
 
-    prompt int [B, P], padded on the right; prompt_lens int32 [B], 1 to P (default P; read by the host). Every round the draft model (same vocabulary and
-    positions) proposes `drafts` tokens and the target accepts a part of them and adds one of its own, so that tokens are
-    distributed as if the target had drawn each. uniforms float32 [rounds, B, 2 * drafts + 2] in [0, 1): of round r, the first
-    `drafts` draw the draft's tokens, the other drafts + 1 (and one unused) go to verify_drafts; the last round's are used again
-    when they run out. The target's cache is cut down to `budget` keys per head, the last `recent` among them, whenever it
-    may hold that many more (None: it grows). One host synchronisation per round (the fewest tokens of a sequence so far)."""
+    prompt int [B, P], padded on the right; prompt_lens int32 [B], 1 to P (default P; read by the host). Every round the draft model
+    (same vocabulary and positions) proposes `drafts` tokens and the target accepts a part of them and adds one of its own, so that
+    tokens are distributed as if the target had drawn each. uniforms float32 [rounds, B, >= 2 * drafts + 1] in [0, 1): of round r, the
+    first `drafts` draw the draft's tokens, the next drafts + 1 go to verify_drafts. new_tokens rounds are always enough, fewer where
+    drafts stand; a call that runs out of them raises ValueError. The target's cache is cut down to `budget` keys per head, the last
+    `recent` among them, whenever it may hold that many more (None: it grows). One host synchronisation per round (the fewest tokens of
+    a sequence so far)."""
     B, P = prompt.shape
     dtype = (params[1]["w_emb"] if isinstance(params[0], GPT2Config) else params[0][0]).dtype
     target, draft = (_weights(x, dtype) for x in (params, draft_params))
@@ -167,7 +168,10 @@ def speculate(params, draft_params, prompt: torch.Tensor, new_tokens: int, unifo
     none = torch.empty((B, 0), device=device, dtype=torch.int32)
     columns = torch.arange(drafts + 1, device=device)
     while least < new_tokens:
-        u = uniforms[min(rounds, uniforms.shape[0] - 1)]
+        if rounds == uniforms.shape[0]:
+            raise ValueError(f"uniforms has numbers for {rounds} rounds, and {least} of {new_tokens} tokens are there (each round gives at "
+                             "least one)")
+        u = uniforms[rounds]
         if budget is not None and most + drafts + 1 > room:
             cache.evict(budget, recent)
             most = budget

@@ -140,3 +140,12 @@ def test_temperatures_that_leave_no_probabilities_are_refused(monkeypatch, tempe
     assert not run.steps
     with pytest.raises(ValueError, match="temperature"):
         real(torch.zeros(1, 4), temperature)
+
+
+def test_random_numbers_are_used_once(monkeypatch):
+    """Two rounds' numbers for what takes three: tokens of numbers used again would not be independent."""
+    run = Rounds(monkeypatch, [2, 0])
+    tokens, rounds = run(5, 3, 2, 3)
+    assert rounds == 3
+    with pytest.raises(ValueError, match="uniforms"):
+        run(5, 3, 2, 2)
