@@ -633,8 +633,6 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, cou
         if out.dim() == 4 and out.stride(3) != 1:
             out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     new, H, T = _new_tokens(sizes, q, k, v, out, counts, k_pages.dtype)
-    if sizes[0] == 0 or T == 0:
-        return out
     if weights_out is None:
         weights_out = weights
     ld = 0
@@ -642,6 +640,11 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, cou
         ld = _attended(weights_out, sizes, sizes[4], "weights_out")
         if weights is not None and _attended(weights, sizes, sizes[4], "weights") != ld:
             raise ValueError("weights and weights_out must share one shape")
+    if sizes[0] == 0 or T == 0:
+        if ld > 0 and weights_out is not weights:  # (nothing is added)
+            held = (torch.arange(ld, device=lengths.device) < lengths.clamp(max=sizes[4])[:, None])[:, None]
+            weights_out.copy_(torch.where(held, 0.0 if weights is None else weights, weights_out))
+        return out
     lib = _lib.lib()
     key = None
     if workspace is None:

@@ -149,3 +149,25 @@ def test_random_numbers_are_used_once(monkeypatch):
     assert rounds == 3
     with pytest.raises(ValueError, match="uniforms"):
         run(5, 3, 2, 2)
+
+
+def test_no_new_tokens_leave_the_weights_they_were_given(ops):  # noqa: F811
+    """T == 0: weights_out holds what the call adds nothing to, below each length; slots behind are left as they were. Tensors that do
+    not fit are refused as ever."""
+    c = cache()
+    c["lengths"].copy_(torch.tensor([5, 0], dtype=I32))
+    w, out = torch.rand(2, 2, 33), torch.full((2, 2, 33), 7.0)
+    assert ops.attn_decode(rows(T=0), **c, weights=w, weights_out=out).shape == (2, 2, 0, 64)
+    want = torch.full((2, 2, 33), 7.0)
+    want[0, :, :5] = w[0, :, :5]
+    assert torch.equal(out, want)
+    ops.attn_decode(rows(T=0), **c, weights_out=out)  # weights None: zeros
+    want[0, :, :5] = 0.0
+    assert torch.equal(out, want)
+    before = w.clone()
+    ops.attn_decode(rows(T=0), **c, weights=w)
+    assert torch.equal(w, before)
+    for bad in (dict(weights=torch.zeros(2, 2, 31)), dict(weights=torch.zeros(2, 2, 32, dtype=BF16)),
+                dict(weights=torch.zeros(2, 2, 32), weights_out=torch.zeros(2, 2, 33))):
+        with pytest.raises(ValueError):
+            ops.attn_decode(rows(T=0), **c, **bad)
