@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from conftest import pkg
-from test_serving_gpu import V
+from test_serving_gpu import V, test_speculative_sampling as sampling
 from test_serving_steps_gpu import laid_out
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +26,10 @@ def test_sequences_that_end_early_stay_inside_their_caches(drafts):
     assert ops.last_kernel_fault() == 0 and rounds > 4
     alone, few = sv.speculate(model, other, prompt[:1], new, u[:, :1].contiguous(), drafts=drafts, page_size=1)
     assert few == 4 and torch.equal(tokens[:1], alone) and ops.last_kernel_fault() == 0
+
+
+@pytest.mark.parametrize("budget,recent", [(None, 0), (14, 5)])
+def test_prompts_in_small_steps(budget, recent, monkeypatch):
+    """The same tokens as the float64 models' where prompts take several steps."""
+    monkeypatch.setattr(pkg("serving"), "PROMPT_TOKENS", 6)
+    sampling(budget, recent)

@@ -171,3 +171,21 @@ def test_no_new_tokens_leave_the_weights_they_were_given(ops):  # noqa: F811
                 dict(weights=torch.zeros(2, 2, 32), weights_out=torch.zeros(2, 2, 33))):
         with pytest.raises(ValueError):
             ops.attn_decode(rows(T=0), **c, **bad)
+
+
+@pytest.mark.parametrize("P,lens", [(1, [1, 1, 1]), (2, [2, 1, 2]), (101, [101, 1, 60]), (5000, [5000, 4097, 33])])
+def test_prompts_are_fed_in_bounded_steps(monkeypatch, P, lens):
+    """Every token of a prompt but its last once and in order, into both caches, never more tokens at once than a step is allowed."""
+    run = Rounds(monkeypatch, [1, 0, 2], seq=6000)
+    most = run.sv.PROMPT_TOKENS
+    monkeypatch.setattr(run.sv, "PROMPT_TOKENS", 96 if P < 1000 else most)
+    prompt = torch.arange(3 * P, dtype=I32).view(3, P)
+    run.sv.speculate([[torch.zeros(1)]], [[torch.zeros(1)]], prompt, 2, torch.zeros(2, 3, 5), drafts=2,
+                     prompt_lens=torch.tensor(lens, dtype=I32))
+    for c in {id(c): c for c, _, _ in run.steps}.values():
+        fed = [[] for _ in lens]
+        for _, ids, counts in (s for s in run.steps if s[0] is c and s[2] is not None):
+            assert ids.numel() <= run.sv.PROMPT_TOKENS and ids.shape[1] <= 4096
+            for b, n in enumerate(counts.tolist()):
+                fed[b] += ids[b, :n].tolist()
+        assert fed == [prompt[b, :n - 1].tolist() for b, n in enumerate(lens)]
