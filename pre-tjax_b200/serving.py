@@ -79,7 +79,7 @@ def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tens
     if B != cache.batch:
         raise ValueError(f"{B} sequences for a cache of {cache.batch}")
     D, H, dh, rows, p = cfg.dim, cfg.heads, cfg.d_head, B * T, cfg.dropout
-    added = T if counts is None else counts
+    added = T if counts is None else counts.clamp(0, T)  # (what the kernels bring out of range to its nearer bound)
     lengths = cache.lengths + added
     at = (cache.positions[:, None] + torch.arange(T, device=ids.device)).clamp_(0, cfg.seq - 1)
     x = ops.embed_fwd(ids.reshape(1, rows), w["w_emb"], w["w_pos"][at.reshape(-1)], False, 0, out_dtype=cache.k.dtype, p=p).view(rows, D)

@@ -50,3 +50,18 @@ def test_replays_of_a_recorded_step_equal_steps(dtype, track):
         assert torch.equal(logits, sv.decode_step(model, ids[:, 19:20], plain))
         assert recorded.lengths.tolist() == plain.lengths.tolist() == [8, 8]
     assert ops.last_kernel_fault() == 0
+
+
+@pytest.mark.parametrize("counts,held", [([9, 2], [3, 2]), ([-4, 3], [0, 3])])
+def test_counts_out_of_range_are_reported_and_counted_as_written(counts, held):
+    """The kernels take the nearer bound and report it; the cache counts the rows that were written, so that the next step is right."""
+    sv, ops = pkg("serving"), pkg("operators")
+    model = laid_out(0, torch.float32)
+    ids = torch.randint(1, V, (2, 20), generator=torch.Generator().manual_seed(1), dtype=torch.int32).cuda()
+    c, good = (sv.PagedCache(model[0], 2, capacity=40, page_size=8, dtype=torch.float32) for _ in range(2))
+    ops.last_kernel_fault()
+    sv.decode_step(model, ids[:, :3], c, torch.tensor(counts, device="cuda", dtype=torch.int32))
+    assert ops.last_kernel_fault() == 0x3202
+    sv.decode_step(model, ids[:, :3], good, torch.tensor(held, device="cuda", dtype=torch.int32))
+    assert c.lengths.tolist() == c.positions.tolist() == held
+    assert torch.equal(sv.decode_step(model, ids[:, 3:4], c), sv.decode_step(model, ids[:, 3:4], good)) and ops.last_kernel_fault() == 0
