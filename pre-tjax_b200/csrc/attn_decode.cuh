@@ -102,10 +102,10 @@ struct Segment {
   __device__ __forceinline__ int64_t index(const DecodeAttn& p) const {
     return (static_cast<int64_t>(b) * p.Hk + h) * p.nrb + rb;
   }
-  // x / sum, sum being that of row r's exponentials. Where it is zero: scores that are all -inf have no softmax, x / 0 makes NaN of the
-  // row; a row none of whose keys exists attends nothing and becomes zero.
-  __device__ __forceinline__ float over(const DecodeAttn& p, int r, float x, float sum) const {
-    return sum != 0.f || any_key(p, table, limit(p, r)) ? x / sum : 0.f;
+  // What row r's sums are divided by, sum being that of its exponentials. Where that is zero: scores that are all -inf have no softmax,
+  // 0 / 0 makes NaN of the row; a row none of whose keys exists attends nothing, 0 / inf makes zeros of it and of its weights.
+  __device__ __forceinline__ float divisor(const DecodeAttn& p, int r, float sum) const {
+    return sum != 0.f || any_key(p, table, limit(p, r)) ? sum : INFINITY;
   }
   static __device__ __noinline__ bool any_key(const DecodeAttn& p, const int32_t* table, int last) {
     for (int i = 0; last >= 0 && i <= p.rows.page_of(last); ++i)
@@ -496,7 +496,7 @@ attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
       l = fmaf(f, v[k].y, l);
     }
     fin[tid][0] = m;
-    fin[tid][1] = sg.over(p, sg.rb * Core::kRows + tid, 1.f, l);
+    fin[tid][1] = 1.f / sg.divisor(p, sg.rb * Core::kRows + tid, l);
   }
   // every block joins its share of the rows' elements
   const int pieces = rows * (Core::kDim / 4);
@@ -750,7 +750,8 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
       const int row = row0 + r;
       if (row >= p.R || d >= p.D) return;
       if (whole) {
-        store_out<E>(p, cur.sg, row, d, cur.sg.limit(p, row) >= 0 ? scaled(x, cur.sg.over(p, row, p.keep, sum)) : make_float4(0.f, 0.f, 0.f, 0.f));
+        sum = cur.sg.divisor(p, row, sum);
+        store_out<E>(p, cur.sg, row, d, cur.sg.limit(p, row) >= 0 ? scaled(x, p.keep / sum) : make_float4(0.f, 0.f, 0.f, 0.f));
       } else {
         *reinterpret_cast<float4*>(p.part + (piece * p.prows + r) * Core::kDim + d) = x;
       }
@@ -873,9 +874,10 @@ attn_decode_join_kernel(const __grid_constant__ DecodeAttn p) {
     }
   }
   if (!there || (some && !split)) return;
+  if (some) l = sg.divisor(p, r, l);
   if (split && p.scores != nullptr && lane == 0)
     *reinterpret_cast<float2*>(p.ml + (sg.index(p) * p.prows + rr) * 2) = make_float2(m, l);
-  const float f = some ? sg.over(p, r, p.keep, l) : 0.f;
+  const float f = p.keep / l;
   char* row = p.out + sg.b * p.os[0] + (sg.h * p.G + r / p.T) * p.os[1] + (r % p.T) * p.os[2];
 #pragma unroll
   for (int k = 0; k < VL; ++k)
@@ -890,14 +892,14 @@ attn_decode_weights_kernel(const __grid_constant__ DecodeAttn p, int rows_of_blo
   grid_dep_sync();
   extern __shared__ float2 row_ml[];  // [R]
   const int tid = threadIdx.x, id = blockIdx.x / chunks;
-  Segment sg;
-  sg.set_sequence(p, id / p.Hk);
-  sg.h = id % p.Hk;
   const float* ml = p.ml + static_cast<int64_t>(id) * p.nrb * p.prows * 2;
   for (int r = tid; r < p.R; r += kDecJoinThreads) {
     const float2 x = *reinterpret_cast<const float2*>(ml + (r / rows_of_block * p.prows + r % rows_of_block) * 2);
-    row_ml[r] = make_float2(x.x, sg.over(p, r, 1.f, x.y));
+    row_ml[r] = make_float2(x.x, 1.f / x.y);
   }
+  Segment sg;
+  sg.set_sequence(p, id / p.Hk);
+  sg.h = id % p.Hk;
   __syncthreads();
   const int j0 = blockIdx.x % chunks * kWeightsChunk;
   if (j0 < sg.n)

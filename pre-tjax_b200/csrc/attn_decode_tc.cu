@@ -112,14 +112,14 @@ struct CoreTc {
   // An infinite value times the second part of its probability (zero, or of either sign) makes NaN of an infinite sum. That is looked
   // for once, in the sums at the end, and costs the steps nothing; where it was, they run again with `careful`.
   __device__ __forceinline__ bool spoiled() const {
-    bool bad = false;
+    float sizes[4] = {0.f, 0.f, 0.f, 0.f};  // one addition per element; a sum that overflows only costs the second time
 #pragma unroll
     for (int i = 0; i < NR; ++i)
 #pragma unroll
       for (int j = 0; j < DP / 16; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[i][j][e]) < INFINITY) && limit[i][e & 1] >= 0;
-    return __any_sync(0xffffffffu, bad);
+        for (int e = 0; e < 4; ++e) sizes[e] += fabsf(o[i][j][e]);
+    return __any_sync(0xffffffffu, !((sizes[0] + sizes[1]) + (sizes[2] + sizes[3]) < INFINITY));
   }
 
   __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage, bool careful) {

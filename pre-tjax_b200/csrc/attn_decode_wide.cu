@@ -376,12 +376,13 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
         for (int i = 0; i < RH; ++i) {
           const int r = r0 + i, row = sg.rb * R + r;
           if (row >= p.R) continue;
-          const float l = (red[w0][i] + red[w0 + 1][i]) + (red[w0 + 2][i] + red[w0 + 3][i]);
+          float l = (red[w0][i] + red[w0 + 1][i]) + (red[w0 + 2][i] + red[w0 + 3][i]);
+          if (whole) l = sg.divisor(p, row, l);
           float o = __uint_as_float(hi[i]) + __uint_as_float(lo[i]);
           if (extra) o += reinterpret_cast<const float*>(smem + Core::kX)[r * DP + key];
           if (whole) {
             char* to = p.out + sg.b * p.os[0] + (sg.h * p.G + row / p.T) * p.os[1] + (row % p.T) * p.os[2];
-            reinterpret_cast<__nv_bfloat16*>(to)[key] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * sg.over(p, row, p.keep, l) : 0.f);
+            reinterpret_cast<__nv_bfloat16*>(to)[key] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * (p.keep / l) : 0.f);
           } else {
             p.part[(piece * p.prows + r) * Core::kDim + key] = o;
           }
