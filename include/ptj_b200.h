@@ -432,11 +432,14 @@ int ptj_kv_append(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, void*
  *   out = (1 - p) softmax(q K^T / sqrt(d_head)) V over keys 0 .. position of the token.
  * With tokens->k and ->v the new rows are written to their pages as by ptj_kv_append and attended to. A token behind counts[b]
  * or below position 0, or none of whose keys' pages exists, attends nothing: a zero row. out overlaps no input. Rows read only the keys they attend: what lies in
- * other slots, an infinity or a NaN included, reaches no output. Softmax statistics and sums are float32.
+ * other slots, an infinity or a NaN included, reaches no output. Scores, softmax statistics and sums are float32; with bf16 heads of up
+ * to 128 elements the exponentials are rounded to 16 bits (two bf16 parts) where they multiply the values, not where they are summed.
+ * Sums are divided at the end: finite values whose sum, times 2^8, passes the largest float overflow.
  * weights_out (optional, float[batch, kv_heads, weights_ld], weights_ld >= table_width * page_size): the attention that each
  * key received, summed over the query heads of its key head and the new tokens, plus weights (same layout; NULL = 0; may be
  * weights_out itself) for keys that are not new. Slots from lengths[b] on are left as they were.
- * workspace: ptj_attn_decode_workspace_bytes bytes, 16-byte aligned, contents irrelevant before and after; bit-reproducible. */
+ * workspace: ptj_attn_decode_workspace_bytes bytes, 16-byte aligned, contents irrelevant before and after; with weights it goes by the
+ * table's room: batch * heads * tokens * table_width * page_size floats and some. 0 for arguments that are refused. Bit-reproducible. */
 size_t ptj_attn_decode_workspace_bytes(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, int with_weights);
 int ptj_attn_decode(const ptj_kv_cache* cache, const ptj_new_tokens* tokens, float p, const float* weights,
                     float* weights_out, int64_t weights_ld, void* workspace, size_t workspace_bytes, void* stream);
@@ -460,7 +463,7 @@ int ptj_kv_evict(const ptj_kv_cache* cache, const int32_t* dst_table, int64_t ds
  *   draft     [batch, drafts, vocab]: the probabilities the drafts were drawn from; NULL: every draft had probability 1
  *   tokens    int32[batch, drafts], counts int32[batch] (NULL: all `drafts`): drafts of each sequence
  *   uniforms  float[batch, drafts + 1] in [0, 1)
- * Draft i is accepted while uniforms[i] * draft[i][x] < target[i][x] (exact; a token outside [0, vocab) is not). At the first
+ * (A count outside [0, drafts] is brought to the nearer bound.) Draft i is accepted while uniforms[i] * draft[i][x] < target[i][x] (exact; a token outside [0, vocab) is not). At the first
  * rejection n, or behind the last draft, the next token is the first j at which the running sum of
  * w = max(target[n] - draft[n], 0), or of target[n] behind the last draft, passes uniforms[drafts] times its total (sums and
  * products in float64; terms that are NaN count as 0; where all are 0: the largest target[n], the first among equals).

@@ -1,8 +1,9 @@
 // Attention of new tokens over a paged key-value cache: the list of work, the ring of keys and values, joining of pieces.
 //
-// out = softmax(q K^T / sqrt(d)) V for the R = group * tokens query rows that share a key head. Every key and value is read once
-// and multiplied with a handful of rows: memory bounds it, so the kernels are built to keep copies in flight and to share them out
-// evenly.
+// out = softmax(q K^T / sqrt(d)) V for the R = group * tokens query rows that share a key head, in blocks of 1 to 32 rows. Every key
+// and value is read once per block of rows and multiplied with a handful of them: memory bounds it, so the kernels are built to keep
+// copies in flight and to share them out evenly. (A block goes over all keys of its sequence, the ones that a prompt's earlier rows
+// do not attend among them.)
 //
 // The keys of a segment (sequence, key head, block of rows) are taken in steps of KS = 4 to 16. Two ways to share them out:
 //
@@ -16,8 +17,9 @@
 //   go to the workspace with their reference exponent and sum and are joined, in order, by a second kernel.
 //
 // Who computes a stretch does not matter to it: results do not depend on timing. A warp owns a ring of steps in shared memory that
-// cp.async fills ahead of the arithmetic, across segments; nothing but the warp itself waits for it. Sums are kept relative to a reference exponent that only moves when a
-// score outgrows it by more than 2^8, so that a step costs one vote instead of a reduction over lanes.
+// cp.async fills ahead of the arithmetic, across segments; nothing but the warp itself waits for it. Sums are kept relative to a
+// reference exponent that only moves when a score outgrows it by more than 2^8, so that a step costs one vote instead of a reduction
+// over lanes.
 #pragma once
 #include <atomic>
 #include <type_traits>

@@ -625,7 +625,7 @@ def attn_decode(q, k_pages, v_pages, page_table, lengths, *, k=None, v=None, cou
     weights float32 [B, kv_heads, capacity]: the attention that every key received so far; the call adds its own, summed over
     the query heads of a key head and the new tokens, into weights_out (default: weights; weights None counts as zeros). What
     weights holds for new keys does not matter. out overlaps no input; H / kv_heads * T <= 4096. workspace: optional uint8 tensor,
-    see ptj_attn_decode_workspace_bytes."""
+    see ptj_attn_decode_workspace_bytes; with weights it takes B * H * T * capacity floats."""
     _on_current_device(q, k_pages, v_pages, page_table, lengths, k, v, counts, weights, weights_out, out, workspace)
     cache, sizes = _kv_cache(k_pages, v_pages, page_table, lengths)
     if out is None:

@@ -22,7 +22,8 @@ from .gpt2 import GPT2Config, Weights, config_from_params
 class PagedCache:
     """Keys and values of `batch` sequences of a model, at most `capacity` keys each, in pages of `page_size`. One page table serves
     all layers; ``k[l]`` and ``v[l]`` are layer l's pools [pages, heads, page_size, d_head]. lengths int32 [batch]: keys kept;
-    positions int64 [batch]: tokens seen. weights (track_weights): the attention that every key received, per layer."""
+    positions int64 [batch]: tokens seen. weights (track_weights): the attention that every key received, per layer. All of them
+    change in place."""
 
     def __init__(self, cfg: GPT2Config, batch: int, capacity: int = None, page_size: int = 16, dtype=torch.bfloat16, device="cuda",
                  track_weights: bool = False):
@@ -69,7 +70,7 @@ def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tens
     [B]: the first counts[b] of a sequence's T ids are tokens (default T); what comes back behind them means nothing. A cache that
     tracks weights takes a workspace of B * heads * T * (slots of a sequence) floats: long prompts go in several steps. params: the
     reference's pytree (model_torch_func.py:36-43) or (GPT2Config, gpt2.Weights). The caller sees to it that no sequence passes
-    the cache's capacity or the model's positions: keys beyond are reported by operators.last_kernel_fault. A step with laid-out weights
+    the cache's capacity or the model's positions: keys beyond are reported by operators.last_kernel_fault. T <= 4096. A step with laid-out weights
     may be recorded in a CUDA graph: every replay advances the cache, which keeps its tensors, by one more step of the ids then in place."""
     cfg, w = _weights(params, cache.k.dtype, p)
     if (cfg.layers, cfg.heads, cfg.d_head) != (cache.cfg.layers, cache.cfg.heads, cache.cfg.d_head):
