@@ -107,10 +107,11 @@ struct Segment {
   // What row r's sums are divided by, sum being that of its exponentials. Where that is zero: scores that are all -inf have no softmax,
   // 0 / 0 makes NaN of the row; a row none of whose keys exists attends nothing, 0 / inf makes zeros of it and of its weights.
   __device__ __forceinline__ float divisor(const DecodeAttn& p, int r, float sum) const {
-    return sum != 0.f || any_key(p, table, limit(p, r)) ? sum : INFINITY;
+    return sum != 0.f || any_key(p, r) ? sum : INFINITY;
   }
-  static __device__ __noinline__ bool any_key(const DecodeAttn& p, const int32_t* table, int last) {
-    for (int i = 0; last >= 0 && i <= p.rows.page_of(last); ++i)
+  __device__ __forceinline__ bool any_key(const DecodeAttn& p, int r) const {
+    const int last = limit(p, r), pages = last < 0 ? 0 : p.rows.page_of(last) + 1;
+    for (int i = 0; i < pages; ++i)
       if (static_cast<unsigned int>(table[i]) < static_cast<unsigned int>(p.rows.pages)) return true;
     return false;
   }
@@ -371,6 +372,24 @@ constexpr int ring_bytes() { return Core::kDepth * stage_bytes<Core>(); }
 template <typename Core>
 __device__ __forceinline__ int steps_of(int n) { return (n + Core::KS - 1) / Core::KS; }
 
+// A warp's steps s, s + stride, .. below `end` once more, one by one through one place, infinite values with care (Core::spoiled).
+// Out of line: the loops that run ahead keep their registers.
+template <typename Core>
+__device__ __noinline__ Core steps_again(const DecodeAttn& p, const Segment sg, int s, int end, int stride, uint8_t* stage) {
+  Fetcher<Core::KS, Core::kRowBytes> fetcher;
+  Core core;
+  core.init(p, sg);
+  for (; s < end; s += stride) {
+    __syncwarp();  // all lanes have left the step before
+    fetcher.general(p, sg, s, stage);
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncwarp();
+    core.template step<true>(p, sg, s, stage);
+  }
+  return core;
+}
+
 // ---- a cluster of blocks per segment -----------------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned cluster_blocks() {
   unsigned r;
@@ -416,35 +435,32 @@ attn_decode_direct_kernel(const __grid_constant__ DecodeAttn p) {
   fetcher.clear(p, ring, ring_bytes<Core>());
   Core core;
   const int plain = fetcher.plain_steps(sg);
-  for (bool careful = false;; careful = true) {  // a second time where the sums say so
-    core.init(p, sg);
-    int slot = 0, free_slot = 0, number = 0;
+  core.init(p, sg);
+  int slot = 0, free_slot = 0, number = 0;
 #pragma unroll 1
-    for (int s = s0 - (D - 1) * stride; s < steps; s += stride) {  // (D - 1 rounds ahead: steps to come are fetched only)
-      if (s >= 0) {
-        cp_async_wait<D - 2>();
-        __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
-      }
-      const int ahead = s + (D - 1) * stride;
-      if (ahead < steps) {
-        if (number == fetcher.base + 32) fetcher.look_up(p, sg.table, ahead, stride, number);
-        uint8_t* stage = ring + free_slot * stage_bytes<Core>();
-        if (ahead >= plain || !fetcher.plain(p, ahead, number, stage)) fetcher.general(p, sg, ahead, stage);
-        ++number;
-      }
-      cp_async_commit();
-      free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
-      if (s < 0) continue;
-      uint8_t* stage = ring + slot * stage_bytes<Core>();
-      if (s >= plain) fetcher.store_new(p, sg, s, stage);
-      core.step(p, sg, s, stage, careful);
-      slot = slot + 1 == D ? 0 : slot + 1;
+  for (int s = s0 - (D - 1) * stride; s < steps; s += stride) {  // (D - 1 rounds ahead: steps to come are fetched only)
+    if (s >= 0) {
+      cp_async_wait<D - 2>();
+      __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
     }
-    cp_async_wait<0>();
-    if (careful || !core.spoiled()) break;
-    fetcher.look_up(p, sg.table, s0, stride, 0);
-    __syncwarp();  // all lanes have left the ring
+    const int ahead = s + (D - 1) * stride;
+    if (ahead < steps) {
+      if (number == fetcher.base + 32) fetcher.look_up(p, sg.table, ahead, stride, number);
+      uint8_t* stage = ring + free_slot * stage_bytes<Core>();
+      if (ahead >= plain || !fetcher.plain(p, ahead, number, stage)) fetcher.general(p, sg, ahead, stage);
+      ++number;
+    }
+    cp_async_commit();
+    free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
+    if (s < 0) continue;
+    uint8_t* stage = ring + slot * stage_bytes<Core>();
+    if (s >= plain) fetcher.store_new(p, sg, s, stage);
+    core.template step<false>(p, sg, s, stage);
+    slot = slot + 1 == D ? 0 : slot + 1;
   }
+  cp_async_wait<0>();
+  if constexpr (Core::kParts)
+    if (core.spoiled()) core = steps_again<Core>(p, sg, s0, steps, stride, ring);
   __syncthreads();
   // the warps' sums over the rings, then the block's over the first warp's
   float* os = reinterpret_cast<float*>(smem);
@@ -712,39 +728,28 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
   for (;;) {  // segments
     const int s_first = cur.s, cur_plain = fetcher.plain_steps(cur.sg);
     Core core;
-    for (bool careful = false;; careful = true) {  // a second time where the sums say so, step by step through the ring's free place
-      core.init(p, cur.sg);
+    core.init(p, cur.sg);
 #pragma unroll 1
-      for (;;) {
-        uint8_t* stage = ring + free_slot * stage_bytes<Core>();
-        if (careful) {
-          __syncwarp();
-          fetcher.general(p, cur.sg, cur.s, stage);
-          cp_async_commit();
-          cp_async_wait<0>();
-          __syncwarp();
-        } else {
-          if (lead == 0) {
-            cp_async_wait<D - 2>();
-            __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
-          }
-          fetch_ahead(stage);
-          cp_async_commit();
-          free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
-          if (lead > 0) {
-            --lead;
-            continue;
-          }
-          stage = ring + slot * stage_bytes<Core>();
-          if (cur.s >= cur_plain) fetcher.store_new(p, cur.sg, cur.s, stage);
-          slot = slot + 1 == D ? 0 : slot + 1;
-        }
-        core.step(p, cur.sg, cur.s, stage, careful);
-        if (++cur.s == cur.end) break;
+    for (;;) {
+      if (lead == 0) {
+        cp_async_wait<D - 2>();
+        __syncwarp();  // the step is there for all lanes, and all have left the one that is refilled
       }
-      if (careful || !core.spoiled()) break;
-      cur.s = s_first;
+      fetch_ahead(ring + free_slot * stage_bytes<Core>());
+      cp_async_commit();
+      free_slot = free_slot + 1 == D ? 0 : free_slot + 1;
+      if (lead > 0) {
+        --lead;
+        continue;
+      }
+      uint8_t* stage = ring + slot * stage_bytes<Core>();
+      if (cur.s >= cur_plain) fetcher.store_new(p, cur.sg, cur.s, stage);
+      core.template step<false>(p, cur.sg, cur.s, stage);
+      slot = slot + 1 == D ? 0 : slot + 1;
+      if (++cur.s == cur.end) break;
     }
+    if constexpr (Core::kParts)  // (the place that is refilled next is free)
+      if (core.spoiled()) core = steps_again<Core>(p, cur.sg, s_first, cur.s, 1, ring + free_slot * stage_bytes<Core>());
     const bool whole = s_first == 0 && cur.s == cur.steps;
     const int64_t piece = stretch * 2 + (first_piece ? 0 : 1);
     const int row0 = cur.sg.rb * Core::kRows;
@@ -752,7 +757,6 @@ attn_decode_split_kernel(const __grid_constant__ DecodeAttn p) {
       const int row = row0 + r;
       if (row >= p.R || d >= p.D) return;
       if (whole) {
-        sum = cur.sg.divisor(p, row, sum);
         store_out<E>(p, cur.sg, row, d, cur.sg.limit(p, row) >= 0 ? scaled(x, p.keep / sum) : make_float4(0.f, 0.f, 0.f, 0.f));
       } else {
         *reinterpret_cast<float4*>(p.part + (piece * p.prows + r) * Core::kDim + d) = x;
@@ -875,9 +879,10 @@ attn_decode_join_kernel(const __grid_constant__ DecodeAttn p) {
       for (int e = 0; e < VL; ++e) x[e] = fmaf(f, part_s[slot][k][d + e], x[e]);
     }
   }
-  if (!there || (some && !split)) return;
+  if (!there || (some && !split && sg.any_key(p, r))) return;
+  // (a row that lies in one stretch is there already; where it has no key it is looked at here, the pass has no registers to spare)
   if (some) l = sg.divisor(p, r, l);
-  if (split && p.scores != nullptr && lane == 0)
+  if (some && p.scores != nullptr && lane == 0)
     *reinterpret_cast<float2*>(p.ml + (sg.index(p) * p.prows + rr) * 2) = make_float2(m, l);
   const float f = p.keep / l;
   char* row = p.out + sg.b * p.os[0] + (sg.h * p.G + r / p.T) * p.os[1] + (r % p.T) * p.os[2];

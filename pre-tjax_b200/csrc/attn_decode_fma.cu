@@ -18,6 +18,7 @@ struct CoreFma {
   static constexpr int RG = RB < 4 ? RB : 4;                  // rows whose scores are on their way at a time
   static constexpr int kDepth = 3;
   static constexpr int kBlocks = 2;
+  static constexpr bool kParts = false;  // probabilities are multiplied whole
   static constexpr int P = W / 2;  // pairs of elements: products run two elements wide
   uint64_t q[RB][P], o[RB][P];
   float ref[RB], sum[RB], over[RB];  // over: scores beyond it (not scaled) move the reference
@@ -64,7 +65,8 @@ struct CoreFma {
     }
   }
 
-  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage, bool) {
+  template <bool>
+  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, const uint8_t* stage) {
     const int j0 = sub * KS;
     const uint32_t present = present_keys<KS, kRowBytes>(stage);
     const bool edge = j0 + KS > sg.first + 1 || present != (1u << KS) - 1u;  // some rows do not attend all of its keys
@@ -156,8 +158,6 @@ struct CoreFma {
       }
     }
   }
-
-  __device__ __forceinline__ bool spoiled() const { return false; }  // probabilities are multiplied whole
 
   // f(row, element, four sums, reference exponent, sum of the row, true for one call per row)
   template <typename F>

@@ -19,6 +19,7 @@ struct CoreTc {
   static_assert(!HALF || NR == 1, "");
   static constexpr int KS = 16, kRows = HALF ? 4 : 8 * NR, kDim = DP, kRowBytes = 2 * DP, KU = DP / 32, VW = DP / 64;
   static constexpr int kDepth = DP == 64 ? (NR == 1 ? 3 : 4) : 3;
+  static constexpr bool kParts = true;  // probabilities are multiplied in parts: spoiled()
   static constexpr int kBlocks = DP == 64 ? (NR == 1 ? 4 : 3) : 2;  // resident per SM
   uint4 q[NR][KU];
   float o[NR][DP / 16][4];
@@ -109,8 +110,9 @@ struct CoreTc {
     if constexpr (!HALF) mma(acc, a[0], a[1], a[2], a[3], pl[0], pl[1]);
   }
 
-  // An infinite value times the second part of its probability (zero, or of either sign) makes NaN of an infinite sum. That is looked
-  // for once, in the sums at the end, and costs the steps nothing; where it was, they run again with `careful`.
+  // A value that is not finite makes NaN of sums that it does not belong to: of rows that do not attend it, times their zeros, and of
+  // those that do, times the second part of a probability (zero, or of either sign). No sum that it meets stays finite, so it is looked
+  // for once, in the sums at the end, and costs the steps nothing; where there was one, they run again with CAREFUL.
   __device__ __forceinline__ bool spoiled() const {
     float sizes[4] = {0.f, 0.f, 0.f, 0.f};  // one addition per element; a sum that overflows only costs the second time
 #pragma unroll
@@ -122,7 +124,8 @@ struct CoreTc {
     return __any_sync(0xffffffffu, !((sizes[0] + sizes[1]) + (sizes[2] + sizes[3]) < INFINITY));
   }
 
-  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage, bool careful) {
+  template <bool CAREFUL>
+  __device__ __forceinline__ void step(const DecodeAttn& p, const Segment& sg, int sub, uint8_t* stage) {
     const int j0 = sub * KS;
     const bool edge = j0 + KS > sg.first + 1;  // some rows do not attend all of its keys
     float s[NR][4];
@@ -210,8 +213,7 @@ struct CoreTc {
           pl[i][k] = transpose8(lo);
         }
       }
-    // a value that some rows of the step attend and others do not must be finite to be multiplied by the others' zeros
-    if ((edge || careful) && not_finite(stage)) infinite_values(p, sg, j0, stage, ph, edge);
+    if (CAREFUL && not_finite(stage)) infinite_values(p, sg, j0, stage, ph, edge);
 #pragma unroll
     for (int w = 0; w < VW; ++w) {
       const uint4 v[4] = {value(stage, 0, w), value(stage, 1, w), value(stage, 2, w), value(stage, 3, w)};

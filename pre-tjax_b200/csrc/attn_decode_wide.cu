@@ -33,6 +33,39 @@ struct CoreWide {
 // 16-byte piece c of row r of an operand with rows of DP elements in blocks of 64 (`block` bytes each)
 __device__ __forceinline__ int place(int r, int c, int block) { return (c >> 3) * block + r * 128 + (((c & 7) ^ (r & 7)) << 4); }
 
+// A value that is not finite makes NaN of sums that it does not belong to: of rows that do not attend it, times their zeros, and of
+// those that do, times the second part of a probability (zero, or of either sign). No sum that it meets stays finite, so it is looked
+// for once, in the sums of a segment; where there was one, the segment runs again, and of each tile this takes such values out and
+// multiplies them by the first parts of the rows that attend them. Out of line: inside the loop it made calls 4 % longer.
+template <int DP>
+__device__ __noinline__ void take_out(uint8_t* smem, const int* limit_s, int j0) {
+  using Core = CoreWide<DP>;
+  const int tid = threadIdx.x;
+  __syncthreads();  // all values and parts are there
+  bool bad = false;
+  if (tid < 128)
+    for (int c = 0; c < DP / 8; ++c) {
+      const uint4 x = *reinterpret_cast<const uint4*>(smem + Core::kV + place(tid, c, 16384));
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
+    }
+  if (!__syncthreads_or(bad)) return;
+  float* x = reinterpret_cast<float*>(smem + Core::kX);  // [rows][DP]
+  if (tid < DP)  // a thread per element: this one's column of x, and of the values
+    for (int k = 0; k < 128; ++k) {
+      uint16_t* v = reinterpret_cast<uint16_t*>(smem + Core::kV + place(k, tid >> 3, 16384)) + (tid & 7);
+      if ((*v & 0x7f80u) != 0x7f80u) continue;
+      const float val = __uint_as_float(static_cast<uint32_t>(*v) << 16);
+      for (int r = 0; r < Core::kRows; ++r)
+        if (j0 + k <= limit_s[r]) {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(smem + Core::kP + place(k, r >> 3, 0)) + (r & 7);
+          x[r * DP + tid] += __uint_as_float(static_cast<uint32_t>(*h) << 16) * val;
+        }
+      *v = 0;
+    }
+}
+
 template <int DP>
 __global__ void __launch_bounds__(kWideThreads, kWideBlocks)
 attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
@@ -108,7 +141,7 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
   if (range0 < all) {
     Cursor<Core> cur;
     cur.set(p, seq_s, start_s, range0, min(st.q1, all - range0));
-    bool first_piece = true, careful = false;  // careful: an infinite value spoiled the segment's sums, it runs again
+    bool first_piece = true, careful = false;  // careful: the segment's sums are not finite, it runs again
     for (;;) {  // segments
       const Segment& sg = cur.sg;
       // the rows' queries
@@ -137,7 +170,8 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
       float sum[RH];
 #pragma unroll
       for (int i = 0; i < RH; ++i) sum[i] = 0.f;
-      bool extra = false;  // products with values that are not finite wait in shared memory
+      if (careful)  // products with values that are not finite
+        for (int i = tid; i < R * DP; i += N) reinterpret_cast<float*>(smem + Core::kX)[i] = 0.f;
 
       // A warp copies 16 keys; lane i < 16 has the address of the i-th key's row, lane 16 + i that of its value's. NULL: absent.
       const int mine16 = warp * 16 + (lane & 15), kv = lane >> 4;
@@ -293,40 +327,7 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
           __syncthreads();
           store_new(1, j16, page_now, Core::kV);
         }
-        if (edge || careful) {
-          // a value that some rows attend and others do not must be finite to be multiplied by the others' zeros; one that is not is
-          // multiplied by the first part of its probability only (the second is zero, or of either sign)
-          __syncthreads();
-          bool bad = false;
-          if (there && r0 == 0)
-            for (int c = 0; c < CH; ++c) {
-              const uint4 x = *reinterpret_cast<const uint4*>(smem + Core::kV + place(key, c, 16384));
-              const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7f80u) == 0x7f80u || (w[e] & 0x7f800000u) == 0x7f800000u;
-            }
-          if (__syncthreads_or(bad)) {
-            float* x = reinterpret_cast<float*>(smem + Core::kX);  // [R][DP]
-            if (!extra)
-              for (int i = tid; i < R * DP; i += N) x[i] = 0.f;
-            extra = true;
-            __syncthreads();
-            if (tid < DP)  // a thread per element: this one's column of x, and of the values
-              for (int k = 0; k < 128; ++k) {
-                uint16_t* v = reinterpret_cast<uint16_t*>(smem + Core::kV + place(k, tid >> 3, 16384)) + (tid & 7);
-                if ((*v & 0x7f80u) != 0x7f80u) continue;
-                const float val = __uint_as_float(static_cast<uint32_t>(*v) << 16);
-                for (int r = 0; r < R; ++r)
-                  if (j0 + k <= limit_s[r]) {
-                    const uint16_t* h = reinterpret_cast<const uint16_t*>(smem + Core::kP + place(k, r >> 3, 0)) + (r & 7);
-                    const float pr = __uint_as_float(static_cast<uint32_t>(*h) << 16);
-                    x[r * DP + tid] += pr * val;
-                  }
-                *v = 0;
-              }
-            __syncthreads();
-          }
-        }
+        if (careful) take_out<DP>(smem, limit_s, j0);
         fence_proxy_async_smem();
         tc_fence_before_sync();
         __syncthreads();
@@ -363,6 +364,7 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
           spoiled |= !(fabsf(o) < INFINITY) && limit_s[r0 + i] >= 0;
         }
       }
+      const bool second = careful;
       careful = __syncthreads_or(spoiled);
       if (careful) {
         cur.s = s_first;
@@ -376,10 +378,9 @@ attn_decode_wide_kernel(const __grid_constant__ DecodeAttn p) {
         for (int i = 0; i < RH; ++i) {
           const int r = r0 + i, row = sg.rb * R + r;
           if (row >= p.R) continue;
-          float l = (red[w0][i] + red[w0 + 1][i]) + (red[w0 + 2][i] + red[w0 + 3][i]);
-          if (whole) l = sg.divisor(p, row, l);
+          const float l = (red[w0][i] + red[w0 + 1][i]) + (red[w0 + 2][i] + red[w0 + 3][i]);
           float o = __uint_as_float(hi[i]) + __uint_as_float(lo[i]);
-          if (extra) o += reinterpret_cast<const float*>(smem + Core::kX)[r * DP + key];
+          if (second) o += reinterpret_cast<const float*>(smem + Core::kX)[r * DP + key];
           if (whole) {
             char* to = p.out + sg.b * p.os[0] + (sg.h * p.G + row / p.T) * p.os[1] + (row % p.T) * p.os[2];
             reinterpret_cast<__nv_bfloat16*>(to)[key] = __float2bfloat16_rn(limit_s[r] >= 0 ? o * (p.keep / l) : 0.f);
