@@ -25,10 +25,10 @@ DecodePlan make_plan(const ptj_kv_cache& c, const ptj_new_tokens& t, const Paged
   int64_t segs = 0, longest = 0;
   int per_sm = 0;
   // More rows than the registers' products take in one pass at memory speed, and tiles enough that the tcgen05 kernel's longer chain
-  // and its second pass do not show: 32 rows on 32 caches of 30k keys of 128 take 115 us on it, 198 in registers, 24 rows 112 and
-  // 106; of 2k keys, 32 rows on 128 caches, 57 and 48; 20 rows of 64 elements, 30k keys, 89 and 121. Where the list of stretches is
-  // needed anyway it is taken from fewer rows on: 8 caches of 131k keys of 128, 12, 16 and 20 rows 109, 113 and 117 us on it, 118, 119
-  // and 210 in registers; one cache of 30k keys, 20 rows, 23 and 30; but 16 rows of 64 elements, 131k keys, 90 and 70.
+  // and its second pass do not show: 32 rows on 32 caches of 30k keys of 128 take 113 us on it, 192 in registers, 24 rows 110 and
+  // 90; of 2k keys, 32 rows on 64 caches, 59 and 47; 20 rows of 64 elements, 30k keys, 87 and 94. Where the list of stretches is
+  // needed anyway it is taken from fewer rows on: 8 caches of 131k keys of 128, 12, 16 and 20 rows 108, 113 and 116 us on it, 117, 116
+  // and 151 in registers; one cache of 30k keys, 20 rows, 22 and 27; but 16 rows of 64 elements, 131k keys, 90 and 72.
   auto share_out = [&](bool wide) {
     pl.wide = wide;
     // the core with the fewest blocks of rows (each reads the keys and values again, mostly from L2), of those the smallest

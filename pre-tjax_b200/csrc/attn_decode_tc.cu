@@ -7,8 +7,8 @@
 // transposing 8 x 8 blocks in registers. Probabilities are multiplied in two bf16 parts (16 bits): rounding them to one would
 // cost as much accuracy as rounding the output does. Up to four rows take four columns with their first parts and the other four
 // with their second ones, so the second part costs nothing; more rows take a second product. The products are not what bounds it (one
-// takes 8 cycles of an SM's quarter, 21 in a chain): up to 16 rows memory does (4 x 8 caches of 30k keys of 128, 1, 8 and 16 rows: 91,
-// 92 and 95 us, floor 75), 24 rows fill the registers (103 us) and leave nothing for the list of stretches.
+// takes 8 cycles of an SM's quarter, 21 in a chain): up to 16 rows memory does (4 x 8 caches of 30k keys of 128, 1, 8 and 16 rows: 89,
+// 89 and 92 us, floor 75), 24 rows fill the registers (90 us) and leave nothing for the list of stretches.
 #include "attn_decode.cuh"
 
 namespace ptj {

@@ -10,7 +10,7 @@
 //
 // Bound by the chain of a tile (keys arrive, product, scores, parts, product); two blocks per SM run theirs against each other, the
 // next tile's keys are on their way from the first product on and its values from the second. 4 x 8 caches of 30k keys of 128,
-// 32 rows: 115 us (198 with operands in registers, in two passes; floor 75).
+// 32 rows: 114 us (192 with operands in registers, in two passes; floor 75).
 #include "attn_decode.cuh"
 #include "tc_runtime.h"
 
