@@ -66,12 +66,13 @@ class PagedCache:
 
 
 def decode_step(params, ids: torch.Tensor, cache: PagedCache, counts: torch.Tensor = None, p: float = None) -> torch.Tensor:
-    """Appends the tokens ids [B, T] to the sequences of a cache and returns their logits [B, T, vocab] (train=False). counts int32
-    [B]: the first counts[b] of a sequence's T ids are tokens (default T); what comes back behind them means nothing. A cache that
-    tracks weights takes a workspace of B * heads * T * (slots of a sequence) floats: long prompts go in several steps. params: the
-    reference's pytree (model_torch_func.py:36-43) or (GPT2Config, gpt2.Weights). The caller sees to it that no sequence passes
-    the cache's capacity or the model's positions: keys beyond are reported by operators.last_kernel_fault. T <= 4096. A step with laid-out weights
-    may be recorded in a CUDA graph: every replay advances the cache, which keeps its tensors, by one more step of the ids then in place."""
+    """Appends the tokens ids [B, T], T <= 4096, to the sequences of a cache and returns their logits [B, T, vocab] (train=False).
+    counts int32 [B]: the first counts[b] of a sequence's T ids are tokens (default T); what comes back behind them means nothing.
+    params: the reference's pytree (model_torch_func.py:36-43) or (GPT2Config, gpt2.Weights). A cache that tracks weights takes a
+    workspace of B * heads * T * (slots of a sequence) floats: long prompts go in several steps. The caller sees to it that no
+    sequence passes the cache's capacity or the model's positions: keys beyond are reported by operators.last_kernel_fault. A step
+    with laid-out weights may be recorded in a CUDA graph: every replay advances the cache, which keeps its tensors, by one more step
+    of the ids then in place."""
     cfg, w = _weights(params, cache.k.dtype, p)
     if (cfg.layers, cfg.heads, cfg.d_head) != (cache.cfg.layers, cache.cfg.heads, cache.cfg.d_head):
         raise ValueError("the cache was made for another model")
